@@ -24,13 +24,13 @@ LIBNAME = "liblevanter_b200.so"
 # What a process that only serves a model needs (``lib.use_serving_library``): a subset of the same objects in a library of its
 # own, so that the first run in a fresh checkout compiles these sources and no others.
 SERVING_LIBNAME = "liblevanter_b200_serving.so"
-SERVING_SOURCES = ("attention_any", "depth_stream", "elementwise", "flash_attn_fwd2", "gated_scan", "gemm_bf16", "gemm_pair", "gemm_skinny",
+SERVING_SOURCES = ("attention_any", "depth_stream", "elementwise", "flash_attn_fwd2", "gated_scan", "gemm_bf16", "gemm_int8", "gemm_pair", "gemm_skinny", "int8_rows",
                    "linear_attention", "linear_attention_umma", "moe_experts", "page_table", "paged_attention", "paged_latent", "qkv_prep",
                    "residual_stream", "sampler")
 
 # Kernels whose results are 32-bit throughout (norms of an fp32 stream, router scores, rotary angles, recurrences, fp32 attention, the
 # loss): no fast-math exponentials, divisions or square roots.
-ACCURATE_SOURCES = ("attention_any", "cross_entropy", "delta_chunks", "depth_stream", "gated_scan", "linear_attention", "linear_attention_umma", "moe_experts", "qkv_prep",
+ACCURATE_SOURCES = ("attention_any", "cross_entropy", "delta_chunks", "depth_stream", "gated_scan", "gemm_int8", "int8_rows", "linear_attention", "linear_attention_umma", "moe_experts", "qkv_prep",
                     "residual_stream")
 
 NVCC_FLAGS = [

@@ -1,0 +1,644 @@
+// Products of rows held in 8 bits: C[M,N] = (A[M,K] B[N,K]^T) scale_a[M] scale_b[N] (+ bias[N]) (+ residual[M,N]) for int8 A and B.
+//
+// The sums are whole numbers in 32 bits and exact (K <= 131071, as 128 * 128 * K has to fit), so their order and any split of them change nothing.
+// The scales are applied once, to the sum, in fp32; then bias and residual are added and the result is rounded once.
+//
+// Three kernels, for rows of activations that are few, some or many:
+//   few     up to 16 rows: a stream over the weights, which the lanes read straight into the fragments of warp-level matrix instructions;
+//   stream  up to a few hundred rows: weights are the 128 rows of a tcgen05 tile and the activations its columns, K is split over a cluster whose CTAs
+//           exchange their partial sums through distributed shared memory;
+//   pair    256 x 256 tiles on CTA pairs (tcgen05 cta_group::2, kind::i8), persistent, accumulators double-buffered in tensor memory.
+// Every wait is bounded (common.cuh).
+#include "cta_pair.cuh"
+
+namespace lvb {
+namespace int8_gemm {
+using namespace cta_pair;
+
+constexpr int BK = 128;      // bytes of K per stage: one 128-byte swizzled line per row
+constexpr int kUmmaK = 32;   // of which one matrix instruction takes 32
+constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA and tensor memory, warps 2-5 epilogue
+
+// The limit of dynamic shared memory is set once per kernel and device.
+template <auto kKernel>
+inline int allow_shared(int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
+  if (dev < 64 && done[dev]) return kErrOk;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return kErrCuda;
+  if (dev < 64) done[dev] = true;
+  return kErrOk;
+}
+
+enum Flags : int { kOutF32 = 1, kBias = 2, kBiasF32 = 4, kResidual = 8, kResidualF32 = 16 };
+
+struct Params {
+  void* C;
+  const float* scale_a;
+  const float* scale_b;
+  const void* bias;
+  const void* residual;
+  int M, N, K;
+  long long ldc, ldr;
+  int flags;
+  int* status;
+};
+
+// Instruction descriptor for kind::i8: signed 8-bit A and B, both K-major, 32-bit whole-number accumulator.
+__host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_i8_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_ss_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ float bias_at(const Params& p, int n) {
+  if (!(p.flags & kBias)) return 0.f;
+  return (p.flags & kBiasF32) ? __ldg(reinterpret_cast<const float*>(p.bias) + n)
+                              : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p.bias) + n));
+}
+// One element of the result: the sum of whole numbers, its scales, bias and residual.
+__device__ __forceinline__ void finish(const Params& p, int m, int n, int sum, float sa, float sb, float bias) {
+  float v = static_cast<float>(sum) * sa * sb + bias;
+  if (p.flags & kResidual)
+    v += (p.flags & kResidualF32) ? reinterpret_cast<const float*>(p.residual)[m * p.ldr + n]
+                                  : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.residual)[m * p.ldr + n]);
+  if (p.flags & kOutF32) reinterpret_cast<float*>(p.C)[m * p.ldc + n] = v;
+  else reinterpret_cast<__nv_bfloat16*>(p.C)[m * p.ldc + n] = __float2bfloat16(v);
+}
+
+// ================================================================ few rows
+// A warp takes 16 output channels and every 8th piece of 64 bytes of K.  A lane's 16 bytes of a channel are the four registers that two instructions
+// of K = 32 want from it, if K is counted in the order in which the lanes hold it; the activations' bytes are read in the same order, so nothing
+// passes through shared memory.  kTiles: groups of 8 rows.
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load_stream(const int8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+// The first `live` (1 to 16 or more) of 16 bytes, zeros for the others: what lies behind a row's end does not count.
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int live) {
+  auto keep = [live](uint32_t w, int at) { return live >= at + 4 ? w : live <= at ? 0u : w & ((1u << (8 * (live - at))) - 1u); };
+  return make_uint4(keep(v.x, 0), keep(v.y, 4), keep(v.z, 8), keep(v.w, 12));
+}
+
+constexpr int kFewWarps = 8;
+
+template <int kTiles>
+__global__ void __launch_bounds__(32 * kFewWarps) few_kernel(const int8_t* __restrict__ A, const int8_t* __restrict__ B, long long lda, long long ldb, Params p) {
+  constexpr int kUnroll = 4;
+  __shared__ int part[kFewWarps][8 * kTiles][17];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  const int pieces = (p.K + 63) / 64;
+  const int8_t* w0 = B + min(n0 + g, p.N - 1) * ldb + 16 * t;  // channels past the end read the last one, their sums are not stored
+  const int8_t* w1 = B + min(n0 + g + 8, p.N - 1) * ldb + 16 * t;
+  int c[kTiles][4] = {};
+  chain_wait();
+  for (int i0 = warp; i0 < pieces; i0 += kFewWarps * kUnroll) {
+    uint4 wa[kUnroll], wb[kUnroll], x[kUnroll][kTiles];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int k = (i0 + u * kFewWarps) * 64, live = p.K - k - 16 * t;
+      wa[u] = wb[u] = make_uint4(0, 0, 0, 0);
+      if (live > 0) {
+        wa[u] = load_stream(w0 + k);
+        wb[u] = load_stream(w1 + k);
+      }
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        x[u][j] = make_uint4(0, 0, 0, 0);
+        if (live > 0 && j * 8 + g < p.M) x[u][j] = first_bytes(__ldg(reinterpret_cast<const uint4*>(A + (j * 8 + g) * lda + 16 * t + k)), live);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        mma_s8(c[j], wa[u].x, wb[u].x, wa[u].y, wb[u].y, x[u][j].x, x[u][j].y);
+        mma_s8(c[j], wa[u].z, wb[u].z, wa[u].w, wb[u].w, x[u][j].z, x[u][j].w);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[warp][j * 8 + 2 * t + (e & 1)][g + 8 * (e >> 1)] = c[j][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * 8 * kTiles; i += 32 * kFewWarps) {
+    const int m = i >> 4, n = n0 + (i & 15);
+    if (m >= p.M || n >= p.N) continue;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) sum += part[w][m][i & 15];
+    finish(p, m, n, sum, __ldg(p.scale_a + m), __ldg(p.scale_b + n), bias_at(p, n));
+  }
+}
+
+int launch_few(const void* A, const void* B, long long lda, long long ldb, const Params& p, cudaStream_t s) {
+  const int8_t *a = reinterpret_cast<const int8_t*>(A), *b = reinterpret_cast<const int8_t*>(B);
+  const dim3 grid((p.N + 15) / 16), block(32 * kFewWarps);
+  const cudaError_t e = p.M <= 8 ? launch_chained(few_kernel<1>, grid, block, 0, s, a, b, lda, ldb, p) : launch_chained(few_kernel<2>, grid, block, 0, s, a, b, lda, ldb, p);
+  return e == cudaSuccess ? kErrOk : kErrCuda;
+}
+
+// ================================================================ some rows
+// Tile: 128 channels (TMEM lanes) x TN rows of activations (TMEM columns).  CTA r of a cluster takes the r-th share of K.  Its partial sums go to the CTA
+// that finishes them, a share of the rows each, so that every CTA reads, adds and writes as much as the others.
+constexpr int kMaxStages = 12;
+
+template <int TN>
+__global__ void __launch_bounds__(kThreads, 1)
+stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Params p, int stages, int kb_per_split) {
+  constexpr int kWBytes = 128 * BK;
+  constexpr int kXBytes = TN * BK;
+  constexpr int kStage = kWBytes + kXBytes;
+  constexpr int kCols = TN < 32 ? 32 : TN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* empty_bar = full_bar + kMaxStages;
+  uint64_t* tfull_bar = empty_bar + kMaxStages;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  uint8_t* ring = smem + 1024;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t splits;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int n0 = static_cast<int>(blockIdx.x / splits) * 128;
+  const int m0 = static_cast<int>(blockIdx.y) * TN;
+  const int k_blocks = (p.K + BK - 1) / BK;
+  const int kb0 = rank * kb_per_split;
+  const int n_kb = min(k_blocks, kb0 + kb_per_split) - kb0;  // at least one (the launcher sees to it)
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(tfull_bar, 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc<kCols>(tmem_holder);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  if (warp == 0 && blockIdx.y == 0 && lane < min(stages, n_kb)) tma_prefetch_2d(&tmW, (kb0 + lane) * BK, n0);  // weights: into the L2 while the kernel before ends
+  chain_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = 0; kb < n_kb; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 100, stage)) break;
+        uint8_t* sw = ring + stage * kStage;
+        mbar_expect_tx(&full_bar[stage], kStage);
+        tma_load_2d(sw, &tmW, &full_bar[stage], (kb0 + kb) * BK, n0);
+        tma_load_2d(sw + kWBytes, &tmX, &full_bar[stage], (kb0 + kb) * BK, m0);
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_i8(128, TN);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int kb = 0; kb < n_kb; ++kb) {
+        ok = mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 201, stage);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sw = smem_u32(ring + stage * kStage);
+        const uint64_t wdesc = make_smem_desc(sw, 16, 1024), xdesc = make_smem_desc(sw + kWBytes, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < BK / kUmmaK; ++k) umma_i8_ss(tmem, wdesc + k * 2, xdesc + k * 2, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&empty_bar[stage]);
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+      if (ok) umma_commit(tfull_bar);
+    }
+  }
+  __syncwarp();
+  // ---- every thread: the tile's sums are complete in this CTA
+  const bool ok = mbar_wait(tfull_bar, 0, abort_flag, p.status, 300, 0);
+  tc_fence_after();
+  const int quad = warp & 3;
+  const int live = min(TN, p.M - m0);
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+  constexpr int kLoad = TN < 32 ? 16 : 32;
+  if (splits == 1) {
+    if (warp >= 2 && __all_sync(0xffffffffu, ok)) {
+      const int n = n0 + quad * 32 + lane;
+      const bool in = n < p.N;
+      const float sb = in ? __ldg(p.scale_b + n) : 0.f, bias = in ? bias_at(p, n) : 0.f;
+      for (int c = 0; c < live; c += kLoad) {
+        uint32_t r[kLoad];
+        if constexpr (kLoad == 32) tmem_ld_32x32(taddr + c, r);
+        else tmem_ld_32x16(taddr + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < kLoad; ++j)
+          if (in && c + j < live) finish(p, m0 + c + j, n, static_cast<int>(r[j]), __ldg(p.scale_a + m0 + c + j), sb, bias);
+      }
+    }
+  } else {
+    // rows [i share, (i + 1) share) of the tile are finished by CTA i: its buffer is [source CTA][row][channel], where the ring was
+    const int share = (live + static_cast<int>(splits) - 1) / static_cast<int>(splits);
+    int* mine = reinterpret_cast<int*>(ring);
+    cluster_sync_all();  // every CTA of the cluster is done with its ring
+    if (warp >= 2 && __all_sync(0xffffffffu, ok)) {
+      for (int c = 0; c < live; c += kLoad) {
+        uint32_t r[kLoad];
+        if constexpr (kLoad == 32) tmem_ld_32x32(taddr + c, r);
+        else tmem_ld_32x16(taddr + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < kLoad; ++j) {
+          if (c + j < live) {
+            const int to = (c + j) / share;
+            const int* at = mine + (rank * share + (c + j - to * share)) * 128 + quad * 32 + lane;
+            uint32_t remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(at)), "r"(to));
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(r[j]) : "memory");
+          }
+        }
+      }
+    }
+    cluster_sync_all();  // all parts have arrived
+    if (ok && !*abort_flag && threadIdx.x < 128) {
+      const int n = n0 + static_cast<int>(threadIdx.x);
+      if (n < p.N) {
+        const float sb = __ldg(p.scale_b + n), bias = bias_at(p, n);
+        const int first = rank * share, count = min(share, live - first);
+        for (int i = 0; i < count; ++i) {
+          int sum = 0;
+          for (uint32_t s = 0; s < splits; ++s) sum += mine[(s * share + i) * 128 + threadIdx.x];
+          finish(p, m0 + first + i, n, sum, __ldg(p.scale_a + m0 + first + i), sb, bias);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<kCols>(tmem);
+  }
+}
+
+template <int TN>
+int launch_stream(const void* A, const void* B, long long lda, long long ldb, const Params& p, int splits, int stages, cudaStream_t s) {
+  constexpr int kStage = (128 + TN) * BK;
+  const int k_blocks = (p.K + BK - 1) / BK;
+  if (splits < 1) splits = 1;
+  if (splits > 8) splits = 8;
+  if (splits > k_blocks) splits = k_blocks;
+  const int per = (k_blocks + splits - 1) / splits;
+  splits = (k_blocks + per - 1) / per;  // no empty share
+  // the ring also holds the exchanged sums: at most TN + splits - 1 rows of 128 (one more per CTA where the rows do not divide)
+  const int exchange = splits > 1 ? (TN + splits) * 512 : 0;
+  if (stages > kMaxStages) stages = kMaxStages;
+  if (stages > 220 * 1024 / kStage) stages = 220 * 1024 / kStage;
+  if (stages > per) stages = per;
+  if (stages < 1) stages = 1;
+  // CTAs whose tensor memory does not fit beside that of others on their SM wait for it, and CTAs of clusters wait for one another: that could close a
+  // circle.  A share of shared memory that is at least the share of tensor memory keeps out what would not fit; 34 KB keeps out the pairs of
+  // the kernels with 256 x 256 tiles, which take all columns and all but 30 KB.
+  constexpr int kCols = TN < 32 ? 32 : TN;
+  constexpr int kLeast = kCols * 464 > 34 * 1024 ? kCols * 464 : 34 * 1024;
+  int bytes = stages * kStage > exchange ? stages * kStage : exchange;
+  if (bytes < kLeast) bytes = kLeast;
+  CUtensorMap tmW, tmX;
+  int rc = make_tmap_2d_u8(&tmW, B, p.N, p.K, ldb, 128);
+  if (rc == kErrOk) rc = make_tmap_2d_u8(&tmX, A, p.M, p.K, lda, TN);
+  if (rc != kErrOk) return rc;
+  rc = allow_shared<stream_kernel<TN>>(232448);
+  if (rc != kErrOk) return rc;
+  const long long row_tiles = (p.M + TN - 1) / TN;
+  if (row_tiles > 65535) return kErrTooLarge;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.N + 127) / 128 * splits), static_cast<unsigned>(row_tiles));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = 2048 + bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, stream_kernel<TN>, tmW, tmX, p, stages, per) == cudaSuccess ? kErrOk : kErrCuda;
+}
+
+// ================================================================ many rows
+constexpr int BN = 256, BMP = 256, BMC = 128;
+constexpr int kPairStage = (BMC + BN / 2) * BK;  // per CTA
+constexpr int kPairStages = 6;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + (2 * kPairStages + 4) * 8 + 16;
+
+__device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& mb, int& nb) {
+  constexpr int GM = 4;  // four row tiles stay in the L2 while the raster sweeps N
+  const int group = GM * tiles_n, g = t / group, first = g * GM, gm = min(GM, tiles_m - first), r = t - g * group;
+  mb = first + r % gm;
+  nb = r / gm;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kPairStages * kPairStage);
+  uint64_t* empty_bar = full_bar + kPairStages;
+  uint64_t* tfull_bar = empty_bar + kPairStages;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank();
+  const int tiles_m = (p.M + BMP - 1) / BMP, tiles_n = (p.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  const int k_blocks = (p.K + BK - 1) / BK;
+  const int first = static_cast<int>(cluster_id_x()), step = static_cast<int>(n_clusters_x());
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], 8);  // one arrival per epilogue warp of either CTA
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair<2 * BN>(tmem_holder);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers are initialised before anything is signalled on them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  chain_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        int mb, nb;
+        tile_coords(t, tiles_m, tiles_n, mb, nb);
+        const int m0 = mb * BMP + static_cast<int>(cta) * BMC, n0 = nb * BN + static_cast<int>(cta) * (BN / 2);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 100, stage);
+          if (!ok) break;
+          uint8_t* sa = smem + stage * kPairStage;
+          if (cta == 0) mbar_expect_tx(&full_bar[stage], 2 * kPairStage);  // both CTAs' loads of this stage
+          tma_load_2d_pair(sa, &tmA, &full_bar[stage], kb * BK, m0);
+          tma_load_2d_pair(sa + BMC * BK, &tmB, &full_bar[stage], kb * BK, n0);
+          if (++stage == kPairStages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && cta == 0) {
+      constexpr uint32_t idesc = make_idesc_i8(BMP, BN);
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, tphase = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        ok = mbar_wait(&tempty_bar[buf], tphase ^ 1, abort_flag, p.status, 200, buf);
+        if (!ok) break;
+        tc_fence_after();
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          ok = mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 201, stage);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * kPairStage);
+          const uint64_t adesc = make_smem_desc(sa, 16, 1024), bdesc = make_smem_desc(sa + BMC * BK, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < BK / kUmmaK; ++k) umma_i8_ss_pair(tmem_base + buf * BN, adesc + k * 2, bdesc + k * 2, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit_pair(&empty_bar[stage]);
+          if (++stage == kPairStages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        umma_commit_pair(&tfull_bar[buf]);
+        if (++buf == 2) { buf = 0; tphase ^= 1; }
+      }
+    }
+  } else {
+    // epilogue: a lane has one row of this CTA's 128 and sees it 32 columns at a time
+    const int quad = warp & 3;
+    int buf = 0;
+    uint32_t tphase = 0;
+    for (int t = first; t < tiles; t += step) {
+      int mb, nb;
+      tile_coords(t, tiles_m, tiles_n, mb, nb);
+      const bool ok = mbar_wait(&tfull_bar[buf], tphase, abort_flag, p.status, 300, buf);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const int m = mb * BMP + static_cast<int>(cta) * BMC + quad * 32 + lane;
+      const bool in = m < p.M;
+      const float sa = in ? __ldg(p.scale_a + m) : 0.f;
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + buf * BN;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        const int n0 = nb * BN + c;
+        if (n0 >= p.N) break;
+        uint32_t r[32];
+        tmem_ld_32x32(taddr + c, r);
+        tmem_ld_wait();
+        if (!in) continue;
+        const int cols = min(32, p.N - n0);
+        float v[32];
+        if (cols == 32 && (reinterpret_cast<uintptr_t>(p.scale_b) & 15) == 0) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 s = __ldg(reinterpret_cast<const float4*>(p.scale_b + n0) + q);
+            v[4 * q] = static_cast<float>(static_cast<int>(r[4 * q])) * sa * s.x;
+            v[4 * q + 1] = static_cast<float>(static_cast<int>(r[4 * q + 1])) * sa * s.y;
+            v[4 * q + 2] = static_cast<float>(static_cast<int>(r[4 * q + 2])) * sa * s.z;
+            v[4 * q + 3] = static_cast<float>(static_cast<int>(r[4 * q + 3])) * sa * s.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = j < cols ? static_cast<float>(static_cast<int>(r[j])) * sa * __ldg(p.scale_b + n0 + j) : 0.f;
+        }
+        if (p.flags & kBias) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < cols) v[j] += bias_at(p, n0 + j);
+        }
+        if (p.flags & kResidual) {
+          if (p.flags & kResidualF32) {
+            const float* rr = reinterpret_cast<const float*>(p.residual) + m * p.ldr + n0;
+            if (cols == 32 && (reinterpret_cast<uintptr_t>(rr) & 15) == 0) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float4 a = reinterpret_cast<const float4*>(rr)[q];
+                v[4 * q] += a.x; v[4 * q + 1] += a.y; v[4 * q + 2] += a.z; v[4 * q + 3] += a.w;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j < cols) v[j] += rr[j];
+            }
+          } else {
+            const __nv_bfloat16* rr = reinterpret_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + n0;
+            if (cols == 32 && (reinterpret_cast<uintptr_t>(rr) & 15) == 0) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint4 a = reinterpret_cast<const uint4*>(rr)[q];
+                const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  v[8 * q + 2 * j] += __uint_as_float(u[j] << 16);
+                  v[8 * q + 2 * j + 1] += __uint_as_float(u[j] & 0xFFFF0000u);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j < cols) v[j] += __bfloat162float(rr[j]);
+            }
+          }
+        }
+        if (p.flags & kOutF32) {
+          float* o = reinterpret_cast<float*>(p.C) + m * p.ldc + n0;
+          if (cols == 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) reinterpret_cast<float4*>(o)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < cols) o[j] = v[j];
+          }
+        } else {
+          __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n0;
+          if (cols == 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              reinterpret_cast<uint4*>(o)[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                                                          pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < cols) o[j] = __float2bfloat16(v[j]);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(&tempty_bar[buf]);
+      if (++buf == 2) { buf = 0; tphase ^= 1; }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA leaves or frees tensor memory while its peer may still signal or accumulate into it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair<2 * BN>(tmem_base);
+  }
+}
+
+int launch_pair(const void* A, const void* B, long long lda, long long ldb, const Params& p, cudaStream_t s) {
+  CUtensorMap tmA, tmB;
+  int rc = make_tmap_2d_u8(&tmA, A, p.M, p.K, lda, BMC);
+  if (rc == kErrOk) rc = make_tmap_2d_u8(&tmB, B, p.N, p.K, ldb, BN / 2);
+  if (rc != kErrOk) return rc;
+  rc = allow_shared<pair_kernel>(kPairSmem);
+  if (rc != kErrOk) return rc;
+  static int pairs = 0;  // as many as are resident at once; a GPC with an odd number of SMs has one that no pair takes
+  if (pairs == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (num_sms() / 2));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, pair_kernel, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = num_sms() / 2;
+    }
+    pairs = n;
+  }
+  const long long tiles = static_cast<long long>((p.M + BMP - 1) / BMP) * ((p.N + BN - 1) / BN);
+  if (tiles > 0x3FFFFFFF) return kErrTooLarge;
+  const unsigned grid = 2u * static_cast<unsigned>(tiles < pairs ? tiles : pairs);
+  return launch_chained(pair_kernel, dim3(grid), dim3(kThreads), kPairSmem, s, tmA, tmB, p) == cudaSuccess ? kErrOk : kErrCuda;
+}
+
+}  // namespace int8_gemm
+}  // namespace lvb
+
+// C[M,N] (bf16, or fp32 with flag 1; row stride ldc) = (A[M,K] B[N,K]^T) scale_a[M] scale_b[N] + bias[N] (flag 2; fp32 with flag 4, else bf16)
+// + residual[M,N] (flag 8; fp32 with flag 16, else bf16; row stride ldr).  A and B: int8, 16-byte aligned, row strides multiples of 16 that are at least K.
+// form: 0 lets the launcher choose; 1 few (M <= 16), 2 stream, 3 pair.  splits, stages: of the stream form, 0 lets the launcher choose.
+extern "C" int lvb_int8_gemm(const void* A, const void* B, const float* scale_a, const float* scale_b, void* C, int M, int N, int K, long long lda,
+                             long long ldb, long long ldc, int flags, const void* bias, const void* residual, long long ldr, int form, int splits, int stages,
+                             int* status, void* stream) {
+  using namespace lvb;
+  using namespace lvb::int8_gemm;
+  if (M <= 0 || N <= 0 || K <= 0 || K > 131071 || (lda & 15) || (ldb & 15) || lda < K || ldb < K || ldc < N) return kErrBadArg;
+  if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15) || A == nullptr || B == nullptr || C == nullptr || scale_a == nullptr ||
+      scale_b == nullptr)
+    return kErrBadArg;
+  if (((flags & kBias) && bias == nullptr) || ((flags & kResidual) && (residual == nullptr || ldr < N))) return kErrBadArg;
+  Params p{C, scale_a, scale_b, bias, residual, M, N, K, ldc, ldr, flags, status};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (form == 0) form = M <= 16 ? 1 : M <= 256 ? 2 : 3;
+  if (form == 1) return M <= 16 ? launch_few(A, B, lda, ldb, p, s) : kErrBadArg;
+  if (form == 3) return launch_pair(A, B, lda, ldb, p, s);
+  if (form != 2) return kErrBadArg;
+  if (splits == 0) {
+    const int tiles = (N + 127) / 128;
+    splits = num_sms() / tiles;
+  }
+  if (stages == 0) stages = kMaxStages;
+  if (M <= 16) return launch_stream<16>(A, B, lda, ldb, p, splits, stages, s);
+  if (M <= 32) return launch_stream<32>(A, B, lda, ldb, p, splits, stages, s);
+  if (M <= 64) return launch_stream<64>(A, B, lda, ldb, p, splits, stages, s);
+  if (M <= 128) return launch_stream<128>(A, B, lda, ldb, p, splits, stages, s);
+  return launch_stream<256>(A, B, lda, ldb, p, splits, stages, s);
+}

@@ -1,0 +1,372 @@
+"""Layers in 8-bit integers (the reference's ``QuantizationConfig(int8=True)``: Haliax ``Int8DotGeneralOp``, reached through
+src/levanter/trainer.py:648).
+
+A row is held as int8 numbers ``q = round(127 y / max |y|)`` (ties to even) and one fp32 scale ``max |y| / 127``: a row of activations has one scale per
+token, a row of a weight matrix ``[out, in]`` one per output channel (:class:`Int8Rows`).  Rows are quantised where they are made (``csrc/int8_rows.cu``):
+:func:`rms_norm_int8` with the residual's addition, :func:`gated_activation_int8`, :func:`quantize_rows`.  :func:`int8_product` multiplies
+quantised rows and weights on the tensor cores, in whole numbers, and applies both scales, bias and residual to the sums (``csrc/gemm_int8.cu``).
+
+:func:`int8_linear_many` is the differentiable form, which :class:`Int8Linear` trains with: activations and weights are quantised, several projections of the
+same rows share them, and the 8-bit rows are all that is kept of the activations for the backward pass.  Its gradients are those of the product at
+the values that the whole numbers stand for (the rounding counts as having slope one).  :class:`Int8ServingLinear` holds a layer's weights in
+8 bits for serving.
+
+A row whose largest magnitude is below 2^-100 is held as zeros; one with an infinity or a NaN has the scale NaN, and all that is made from it is NaN.
+The PyTorch statements are the CPU path and the test oracle."""
+from __future__ import annotations
+
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from ..utils.activation import ActivationFunctionEnum
+from . import lib
+from .glu import _ACT, GatedActivation, gated_activation
+
+TINY = 2.0 ** -100
+MAX_COLS = 131071  # 128 * 128 * cols has to fit into the 32-bit sums
+_FLOATS = (torch.bfloat16, torch.float32)
+_f = {}
+
+
+class Int8Rows(NamedTuple):
+    """Rows in 8 bits: ``values`` int8 ``[..., cols]`` and ``scale`` fp32 ``[...]``; they stand for ``values * scale``.  The rows that this module makes
+    start at multiples of 16 bytes, as the products want them; others are copied there by every product."""
+
+    values: torch.Tensor
+    scale: torch.Tensor
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """What the rows stand for, ``values * scale`` rounded once to ``dtype`` (bf16 or fp32)."""
+        _check_rows(self, "rows")
+        if dtype not in _FLOATS:
+            raise TypeError(f"rows come back as bf16 or fp32, not {dtype}")
+        v, s = self
+        if not (v.is_cuda and lib.available()):
+            return (v.float() * s.unsqueeze(-1)).to(dtype)
+        v2, ld = _rows_of(v, 1)
+        out = torch.empty(v.shape, dtype=dtype, device=v.device)
+        if out.numel():
+            with _on(v):
+                rc = _fn("lvb_int8_dequantize", "plplipi")(v2.data_ptr(), ld, s.contiguous().data_ptr(), v2.shape[0], v2.shape[1], out.data_ptr(), int(dtype == torch.float32),
+                                                           lib.stream_ptr())
+            lib.check_rc(rc, "lvb_int8_dequantize")
+        return out
+
+
+def _fn(name: str, args: str):
+    """The launcher ``name``: arguments by letter (p pointer, l long long, i int, f float), then the stream."""
+    if name not in _f:
+        kinds = {"p": lib.c_void_p, "l": lib.c_longlong, "i": lib.c_int, "f": lib.c_float}
+        _f[name] = lib.fn(name, [kinds[a] for a in args] + [lib.c_void_p])
+    return _f[name]
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def _on(t: torch.Tensor):
+    """The device of ``t`` as the current one, while a kernel is launched there."""
+    return _here if t.device.index == lib._current_device() else torch.cuda.device(t.device)
+
+
+def _check_rows(rows: Int8Rows, what: str) -> None:
+    v, s = rows
+    if v.dtype != torch.int8 or s.dtype != torch.float32:
+        raise TypeError(f"{what}: int8 values with fp32 scales expected, got {v.dtype} and {s.dtype}")
+    if v.dim() == 0 or s.shape != v.shape[:-1]:
+        raise ValueError(f"{what}: values {tuple(v.shape)} need one scale per row, got {tuple(s.shape)}")
+    if s.device != v.device:
+        raise ValueError(f"{what}: values on {v.device}, scales on {s.device}")
+
+
+def _check_floats(what: str, like: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    if like.dtype not in _FLOATS:
+        raise TypeError(f"{what}: rows in bf16 or fp32 expected, got {like.dtype}")
+    if like.dim() == 0 or like.shape[-1] == 0:
+        raise ValueError(f"{what}: rows of at least one element expected, got {tuple(like.shape)}")
+    for t in others:
+        if t is not None and (t.dtype != like.dtype or t.shape != like.shape or t.device != like.device):
+            raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} on {t.device} does not go with {tuple(like.shape)} {like.dtype} on {like.device}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (like, *others)):
+        raise RuntimeError(f"{what} has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
+
+
+def _rows_of(t: torch.Tensor, align: int) -> Tuple[torch.Tensor, int]:
+    """``t [..., cols]`` as rows and their stride in elements; copied unless the elements of a row lie side by side, rows do not overlap and start at
+    multiples of ``align`` bytes (a power of two)."""
+    cols = t.shape[-1]
+    t2 = t.reshape(-1, cols)
+    ld = t2.stride(0) if t2.shape[0] > 1 else -(-cols // 16) * 16
+    e = t.element_size()
+    if (cols > 1 and t2.stride(1) != 1) or ld < cols or (ld * e) % align or t2.data_ptr() % align:
+        t2 = _room(t2.shape, t.dtype, t.device, align // e or 1).copy_(t2)
+        ld = t2.stride(0) if t2.shape[0] > 1 else -(-cols // 16) * 16
+    return t2, ld
+
+
+def _room(shape, dtype: torch.dtype, device, multiple: int = 16) -> torch.Tensor:
+    """Empty rows whose stride is a multiple of that many elements."""
+    cols = shape[-1]
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    wide = torch.empty(rows, -(-cols // multiple) * multiple, dtype=dtype, device=device)
+    return wide[:, :cols].view(shape) if wide.shape[1] == cols else wide[:, :cols].unflatten(0, shape[:-1]) if len(shape) != 2 else wide[:, :cols]
+
+
+def _empty_rows(shape, device) -> Int8Rows:
+    if len(shape) == 1:
+        return Int8Rows(_room((1, shape[0]), torch.int8, device)[0], torch.empty((), dtype=torch.float32, device=device))
+    return Int8Rows(_room(shape, torch.int8, device), torch.empty(shape[:-1], dtype=torch.float32, device=device))
+
+
+def _kernels(t: torch.Tensor) -> bool:
+    return t.is_cuda and lib.available()
+
+
+# ------------------------------------------------------------------------------------------------ rows
+def quantize_reference(y: torch.Tensor, factor: Optional[torch.Tensor] = None) -> Int8Rows:
+    """PyTorch statement: the rows of ``factor * y`` (a positive number per row, which leaves the whole numbers as they are)."""
+    y = y.float()
+    top = y.abs().amax(-1, keepdim=True)
+    most = top if factor is None else top * factor
+    live = most >= TINY
+    q = torch.where(live & torch.isfinite(top), torch.round(y * 127.0 / top), torch.zeros_like(y))
+    scale = torch.where(live, most / 127.0, torch.zeros_like(most))
+    ok = torch.isfinite(top) & ~torch.isnan(most)
+    scale = torch.where(ok, scale, torch.full_like(scale, float("nan")))
+    values = _empty_rows(y.shape, y.device).values
+    return Int8Rows(values.copy_(torch.where(ok, q, torch.zeros_like(q))), scale.squeeze(-1))
+
+
+def quantize_rows(x: torch.Tensor) -> Int8Rows:
+    """The rows of ``x [..., cols]`` (bf16 or fp32, any strides) in 8 bits."""
+    _check_floats("quantize_rows", x)
+    return _quantize(x)
+
+
+def _quantize(x: torch.Tensor) -> Int8Rows:
+    x = x.detach()
+    if not _kernels(x):
+        return quantize_reference(x)
+    x2, ld = _rows_of(x, 1)
+    out = _empty_rows(x.shape, x.device)
+    if x.numel():
+        with _on(x):
+            rc = _fn("lvb_int8_quantize", "pilliplp")(x2.data_ptr(), int(x.dtype == torch.float32), ld, x2.shape[0], x2.shape[1],
+                                                                               out.values.data_ptr(), _ldq(x.shape[-1]), out.scale.data_ptr(), lib.stream_ptr())
+        lib.check_rc(rc, "lvb_int8_quantize")
+    return out
+
+
+def _ldq(cols: int) -> int:
+    return -(-cols // 16) * 16
+
+
+def rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6, *, w_offset: float = 0.0,
+                  residual: Optional[torch.Tensor] = None) -> Tuple[Int8Rows, Optional[torch.Tensor]]:
+    """``(rows, h)``: the RMS norm of ``h = x + residual`` (rounded to the type of ``x``; without a residual ``x`` itself, and the second item is None) times
+    ``weight + w_offset``, in 8 bits.  ``x [..., cols]`` and ``residual`` in bf16 or fp32, ``weight [cols]`` in bf16 or fp32 or None."""
+    _check_floats("rms_norm_int8", x, residual)
+    cols = x.shape[-1]
+    if weight is not None and (weight.shape != (cols,) or weight.dtype not in _FLOATS or weight.device != x.device):
+        raise ValueError(f"rms_norm_int8: weight [{cols}] in bf16 or fp32 on {x.device} expected, got {tuple(weight.shape)} {weight.dtype} on {weight.device}")
+    x = x.detach()
+    if not _kernels(x):
+        h = x if residual is None else (x.float() + residual.detach().float()).to(x.dtype)
+        f = h.float()
+        y = f if weight is None else f * (weight.detach().float() + w_offset)
+        return quantize_reference(y, torch.rsqrt(f.square().mean(-1, keepdim=True) + eps)), None if residual is None else h
+    x2, ldx = _rows_of(x, 1)
+    h = r2 = None
+    ldr = 0
+    if residual is not None:
+        r2, ldr = _rows_of(residual.detach(), 1)
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    w = None if weight is None else weight.detach().contiguous()
+    out = _empty_rows(x.shape, x.device)
+    if x.numel():
+        with _on(x):
+            rc = _fn("lvb_int8_rms_norm", "pppilllpiffliplp")(x2.data_ptr(), lib.ptr(r2), lib.ptr(h), int(x.dtype == torch.float32), ldx, ldr, cols, lib.ptr(w),
+                                                                  int(w is not None and w.dtype == torch.float32), float(w_offset), float(eps), x2.shape[0], cols,
+                                                                  out.values.data_ptr(), _ldq(cols), out.scale.data_ptr(), lib.stream_ptr())
+        lib.check_rc(rc, "lvb_int8_rms_norm")
+    return out, h
+
+
+def gated_activation_int8(gate: torch.Tensor, up: torch.Tensor, act: GatedActivation) -> Int8Rows:
+    """``act(gate) * up`` in 8 bits; ``gate`` and ``up [..., cols]`` in bf16 or fp32 may be the halves of a joint product's rows."""
+    _check_floats("gated_activation_int8", gate, up)
+    gate, up = gate.detach(), up.detach()
+    act = ActivationFunctionEnum(act) if isinstance(act, str) and not isinstance(act, ActivationFunctionEnum) else act
+    if act not in _ACT:  # bounded gates and the like: quantised as they come
+        return _quantize(gated_activation(gate, up, act))
+    if not _kernels(gate):
+        return quantize_reference(act.to_fn()(gate.float()) * up.float())
+    (g2, ldg), (u2, ldu) = _rows_of(gate, 1), _rows_of(up, 1)
+    cols = gate.shape[-1]
+    out = _empty_rows(gate.shape, gate.device)
+    if gate.numel():
+        with _on(gate):
+            rc = _fn("lvb_int8_glu", "ppilliliplp")(g2.data_ptr(), u2.data_ptr(), int(gate.dtype == torch.float32), ldg, ldu, _ACT[act], g2.shape[0], cols,
+                                                       out.values.data_ptr(), _ldq(cols), out.scale.data_ptr(), lib.stream_ptr())
+        lib.check_rc(rc, "lvb_int8_glu")
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ products
+F_OUT_F32, F_BIAS, F_BIAS_F32, F_RESIDUAL, F_RESIDUAL_F32 = 1, 2, 4, 8, 16
+
+
+def int8_product(rows: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(values_x values_w^T) scale_x scale_w + bias + residual`` of ``rows [..., in]`` and ``weight [out, in]`` -> ``[..., out]`` in bf16 or fp32.
+
+    The sums are exact whole numbers; scales, ``bias [out]`` and ``residual [..., out]`` (each in bf16 or fp32) are applied in fp32 and the result is
+    rounded once.  ``in`` is at most 131071."""
+    return _product(rows, weight, bias, residual, out_dtype)
+
+
+def _product(rows, weight, bias=None, residual=None, out_dtype=torch.bfloat16, form: int = 0, splits: int = 0, stages: int = 0) -> torch.Tensor:
+    _check_rows(rows, "int8_product: rows")
+    _check_rows(weight, "int8_product: weight")
+    v, w = rows.values, weight.values
+    K, dev = v.shape[-1], v.device
+    if w.dim() != 2 or w.shape[1] != K or w.device != dev:
+        raise ValueError(f"int8_product: rows {tuple(v.shape)} on {dev} and weight {tuple(w.shape)} on {w.device} do not go together")
+    if not 0 < K <= MAX_COLS:
+        raise ValueError(f"int8_product: rows of 1 to {MAX_COLS} elements expected, got {K}")
+    if out_dtype not in _FLOATS:
+        raise TypeError(f"int8_product: results in bf16 or fp32, not {out_dtype}")
+    N, shape = w.shape[0], (*v.shape[:-1], w.shape[0])
+    for t, want, what in ((bias, (N,), "bias"), (residual, shape, "residual")):
+        if t is not None and (tuple(t.shape) != want or t.dtype not in _FLOATS or t.device != dev):
+            raise ValueError(f"int8_product: {what} {want} in bf16 or fp32 on {dev} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (bias, residual)):
+        raise RuntimeError("int8_product has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
+    if not _kernels(v):
+        y = torch.matmul(v.double(), w.double().t()).float() * rows.scale.unsqueeze(-1) * weight.scale
+        for t in (bias, residual):
+            y = y if t is None else y + t.float()
+        return y.to(out_dtype)
+    (a, lda), (b, ldb) = _rows_of(v, 16), _rows_of(w, 16)
+    M = a.shape[0]
+    out = torch.empty(shape, dtype=out_dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    flags = F_OUT_F32 if out_dtype == torch.float32 else 0
+    ldr = 0
+    if bias is not None:
+        flags |= F_BIAS | (F_BIAS_F32 if bias.dtype == torch.float32 else 0)
+        bias = bias.contiguous()
+    if residual is not None:
+        flags |= F_RESIDUAL | (F_RESIDUAL_F32 if residual.dtype == torch.float32 else 0)
+        residual, ldr = _rows_of(residual, 1)
+        ldr = max(ldr, N)
+    sa, sb = rows.scale.contiguous(), weight.scale.contiguous()
+    with _on(v):
+        rc = _fn("lvb_int8_gemm", "pppppiiilllippliiip")(a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), out.data_ptr(), M, N, K, lda, ldb, N, flags,
+                                                                 lib.ptr(bias), lib.ptr(residual), ldr, form, splits, stages, lib.status_buffer().data_ptr(),
+                                                                 lib.stream_ptr())
+    lib.check_rc(rc, "lvb_int8_gemm")
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ training
+def _straight_through(x: torch.Tensor) -> torch.Tensor:
+    """What the 8-bit rows of ``x`` stand for, with the gradient passed on as it is."""
+    return x + (quantize_reference(x.detach()).dequantize(torch.float32).to(x.dtype) - x).detach()
+
+
+class _Int8ManyFn(torch.autograd.Function):
+    """Projections of the same rows.  Kept for the backward pass: the rows and the weights in 8 bits, 1 byte per activation instead of 2, once for all projections.
+
+    ``dx = sum dy w'`` and ``dw = dy^T x'`` are bf16 products of what the whole numbers stand for, rounded to bf16 (2^-9 of each value, as any operand
+    of a bf16 layer); output gradients are not quantised, their rows span too many magnitudes for one scale."""
+
+    @staticmethod
+    def forward(ctx, x, count, *tensors):
+        weights, biases = tensors[:count], tensors[count:]
+        rows = _quantize(x)
+        ws = [_quantize(w) for w in weights]
+        ys = tuple(_product(rows, w, b, out_dtype=x.dtype) for w, b in zip(ws, biases))
+        ctx.save_for_backward(rows.values, rows.scale, *[t for w in ws for t in w])
+        ctx.refs, ctx.bias_dtypes = weights, [None if b is None else b.dtype for b in biases]
+        ctx.x_shape = x.shape
+        ctx.set_materialize_grads(False)  # a product that nothing uses has no gradient, and its weight none
+        return ys
+
+    @staticmethod
+    def backward(ctx, *dys):
+        from .gemm import _weight_grad, col_sum, gemm
+
+        values, scale, *flat = ctx.saved_tensors
+        n = len(ctx.refs)
+        need_w = [dy is not None and need for dy, need in zip(dys, ctx.needs_input_grad[2:2 + n])]
+        x2 = None
+        if any(need_w):
+            x2 = Int8Rows(values, scale).dequantize().reshape(-1, values.shape[-1])
+        dx, dws, dbs = None, [None] * n, [None] * n
+        for i, dy in enumerate(dys):
+            if dy is None:
+                continue
+            dy2 = dy.reshape(-1, dy.shape[-1])
+            if dy2.dtype != torch.bfloat16:
+                dy2 = dy2.to(torch.bfloat16)
+            if ctx.needs_input_grad[0]:
+                w = Int8Rows(flat[2 * i], flat[2 * i + 1]).dequantize()
+                dx = gemm(dy2, w, b_mn=True, out=dx, accumulate=dx is not None)
+            if need_w[i]:
+                dws[i] = _weight_grad(ctx.refs[i], dy2, x2)
+            if ctx.bias_dtypes[i] is not None and ctx.needs_input_grad[2 + n + i]:
+                dbs[i] = col_sum(dy2, ctx.bias_dtypes[i])
+        return (None if dx is None else dx.view(ctx.x_shape), None, *dws, *dbs)
+
+
+def int8_linear_many(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: Optional[Sequence[Optional[torch.Tensor]]] = None) -> Tuple[torch.Tensor, ...]:
+    """``[x' w'^T + b for w, b in ...]`` with ``x [..., in]`` and the ``weights [out, in]`` held in 8 bits (``x'``, ``w'``: what their whole numbers stand for);
+    differentiable in ``x``, weights and biases.  bf16 with sizes that are multiples of 8 runs on the kernels, everything else on PyTorch's operations."""
+    weights = list(weights)
+    biases = [None] * len(weights) if biases is None else list(biases)
+    if not weights or len(biases) != len(weights):
+        raise ValueError(f"int8_linear_many: one bias (or None) per weight expected, got {len(biases)} for {len(weights)}")
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"int8_linear_many: rows in bf16 or fp32 expected, got {x.dtype}")
+    for w, b in zip(weights, biases):
+        if w.dim() != 2 or w.shape[1] != x.shape[-1] or not 0 < w.shape[1] <= MAX_COLS or w.device != x.device or w.dtype not in _FLOATS:
+            raise ValueError(f"int8_linear_many: x {tuple(x.shape)} on {x.device} and a weight {tuple(w.shape)} {w.dtype} on {w.device} do not go together")
+        if b is not None and (b.shape != (w.shape[0],) or b.device != x.device or b.dtype not in _FLOATS):
+            raise ValueError(f"int8_linear_many: bias [{w.shape[0]}] on {x.device} expected, got {tuple(b.shape)} {b.dtype} on {b.device}")
+    from .gemm import _tma_shapes_ok
+
+    if _kernels(x) and x.dtype == torch.bfloat16 and x.numel() and all(w.dtype == torch.bfloat16 and _tma_shapes_ok(w) and w.shape[0] > 0 for w in weights):
+        if lib.plain_call():
+            rows = _quantize(x)
+            return tuple(_product(rows, _quantize(w), b) for w, b in zip(weights, biases))
+        return _Int8ManyFn.apply(x, len(weights), *weights, *biases)
+    x8 = _straight_through(x)
+    return tuple(F.linear(x8, _straight_through(w).to(x.dtype), None if b is None else b.to(x.dtype)) for w, b in zip(weights, biases))
+
+
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`int8_linear_many` of one projection."""
+    return int8_linear_many(x, [weight], [bias])[0]

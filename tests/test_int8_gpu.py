@@ -1,0 +1,234 @@
+"""8-bit rows and their products on the GPU against the definition in 64 bits: sizes from one element to long rows, odd ones, strides, halves of joint
+rows, rows of zeros, infinities and NaN."""
+import pytest
+import torch
+
+from levanter_b200.ops import int8 as I
+from levanter_b200.ops import lib
+from levanter_b200.utils.activation import ActivationFunctionEnum as Act
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+STEP = {BF: 2.0 ** -8, F32: 2.0 ** -24}  # most that one rounding moves a value, relative to it
+
+
+def rand(*shape, seed=0, std=1.0, dtype=BF):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+def whole(y, factor=None):
+    """Whole numbers and scales of ``factor * y`` in 64 bits."""
+    y = y.double()
+    top = y.abs().amax(-1, keepdim=True)
+    most = top if factor is None else top * factor
+    live = most >= I.TINY
+    return torch.where(live, (127 * y / top).round(), 0.0), torch.where(live, most / 127, 0.0).squeeze(-1)
+
+
+def check_rows(rows, y, factor=None, slack=0.0):
+    """``slack``: how far, relative to itself, an element of ``y`` may be from the kernel's, so that near a tie either whole number is right."""
+    q, s = whole(y, factor)
+    got = rows.values.double()
+    off = (got - q).abs()
+    if slack == 0.0:
+        assert torch.equal(got, q)
+    else:
+        exact = 127 * y.double() / y.double().abs().amax(-1, keepdim=True)
+        # whole numbers one apart only where the quotient is within its own error (its element's and the largest one's) of the border
+        near = ((exact - exact.floor() - 0.5).abs() <= 127 * 2 * slack)
+        assert off.max() <= 1 and bool((near | (off == 0)).all())
+    # fp32 scale: the norm's factor (a sum over the row, a root), the largest element, a product and a quotient
+    assert ((rows.scale.double() - s).abs() <= (slack + 2.0 ** -20) * s).all()
+
+
+SIZES = [(1, 1), (3, 7), (5, 8), (2, 255), (9, 256), (4, 513), (7, 1000), (130, 1024), (3, 1025), (5, 2048), (2, 4096), (3, 5001), (2, 8192), (2, 14336), (3, 16385),
+         (1, 32768), (2, 40001)]
+
+
+@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantize_rows(rows, cols, dtype):
+    x = rand(rows, cols, seed=rows * 7 + cols, dtype=dtype)
+    x[0, cols // 2] = x[0].abs().max() / 2  # half of the largest value: a tie
+    check_rows(I.quantize_rows(x), x, slack=0.0 if dtype == BF else 2.0 ** -23)
+
+
+def test_quantize_rows_with_strides_and_more_dimensions():
+    wide = rand(6, 5, 700, seed=3)
+    for x in (wide[:, :, 3:500], wide[::2, 1:3], wide.transpose(0, 1), wide[:, :, ::2], wide[0, 0], rand(1, 300).expand(4, 300)):
+        rows = I.quantize_rows(x)
+        assert rows.shape == x.shape and rows.scale.shape == x.shape[:-1]
+        check_rows(rows, x)
+
+
+def test_rows_of_zeros_tiny_values_infinities_and_nan():
+    x = rand(8, 600, seed=4, dtype=F32)
+    x[0] = 0
+    x[1] *= 1e-33
+    x[2, 5] = float("inf")
+    x[3, 7] = float("nan")
+    x[4] *= 1e30
+    x[5] = 0
+    x[5, 9] = -3.0
+    x[6, 0] = -float("inf")
+    for dtype in (F32, BF):
+        rows = I.quantize_rows(x.to(dtype))
+        assert rows.scale[0] == 0 and rows.scale[1] == 0 and not rows.values[:2].any()
+        assert rows.scale[[2, 3, 6]].isnan().all() and not rows.values[[2, 3, 6]].any()
+        assert rows.values[5, 9] == -127 and rows.values[5].abs().sum() == 127
+        check_rows(I.Int8Rows(rows.values[4:6], rows.scale[4:6]), x[4:6].to(dtype), slack=0.0 if dtype == BF else 2.0 ** -23)
+        back = rows.dequantize(F32)
+        assert back[[2, 3, 6]].isnan().all() and not back[:2].any()
+    empty = I.quantize_rows(rand(0, 64))
+    assert empty.shape == (0, 64) and empty.dequantize().shape == (0, 64)
+
+
+@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("residual", [False, True])
+def test_rms_norm_int8(rows, cols, dtype, residual):
+    x, w = rand(rows, cols, seed=cols, dtype=dtype), (1 + rand(cols, seed=1, std=0.1, dtype=F32)).to(BF if cols % 2 else F32)
+    r = rand(rows, cols, seed=2, dtype=dtype) if residual else None
+    got, h = I.rms_norm_int8(x, w, 1e-5, residual=r)
+    want = x if r is None else (x.float() + r.float()).to(dtype)
+    assert (h is None) == (r is None) and (h is None or torch.equal(h, want))
+    d = want.double()
+    exact = dtype == BF and w.dtype == BF  # the product of two bf16 numbers is exact in fp32
+    check_rows(got, d * w.double(), (d.square().mean(-1, keepdim=True) + 1e-5).rsqrt(), slack=0.0 if exact else 2.0 ** -22)
+
+
+def test_rms_norm_int8_offset_no_weight_and_tiny_rows():
+    x = rand(5, 700, seed=8)
+    x[1] = 0
+    d = x.double()
+    f = (d.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    check_rows(I.rms_norm_int8(x, None)[0], d, f)
+    w = rand(700, seed=9, std=0.1)
+    check_rows(I.rms_norm_int8(x, w, w_offset=1.0)[0], d * (w.double() + 1.0), f, slack=2.0 ** -22)
+    x[2, 3] = float("nan")
+    x[3, 4] = float("inf")
+    rows, _ = I.rms_norm_int8(x, w)
+    assert rows.scale[[2, 3]].isnan().all() and not rows.scale[[0, 1, 4]].isnan().any()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 500), (2, 4096), (3, 5001), (2, 14336), (1, 40001)])
+@pytest.mark.parametrize("act", ["silu", "gelu_new", "gelu", "relu", "quick_gelu"])
+def test_gated_activation_int8(rows, cols, act):
+    y = rand(rows, 2 * cols, seed=cols, std=3.0)
+    got = I.gated_activation_int8(y[:, :cols], y[:, cols:], Act(act))
+    g, u = y.double().chunk(2, -1)
+    # the exponential's argument is rounded (|g| <= 20: 20 * 2^-23), the exponential, the quotient and the product each by 2^-22 at most; where 1 + tanh
+    # or 1 + erf cancels (g < 0), what is lost counts against 1 and not against the little that is left
+    want = Act(act).to_fn()(g) * u
+    top = want.abs().amax(-1, keepdim=True)
+    if act in ("gelu_new", "gelu"):
+        q, s = whole(want)
+        assert (got.values.double() - 127 * want / top.clamp(min=I.TINY)).abs().max() <= 0.5 + 127 * 2.0 ** -18
+        assert ((got.scale.double() - s).abs() <= 2.0 ** -18 * s).all()
+    else:
+        check_rows(got, want, slack=2.0 ** -18)
+
+
+def test_gated_activation_int8_of_fp32_rows_and_other_gates():
+    from levanter_b200.ops.glu import ClampedGlu
+
+    g, u = rand(3, 333, seed=1, dtype=F32), rand(3, 333, seed=2, dtype=F32)
+    check_rows(I.gated_activation_int8(g, u, Act.silu), torch.nn.functional.silu(g.double()) * u.double(), slack=2.0 ** -18)
+    g, u = g.to(BF), u.to(BF)
+    check_rows(I.gated_activation_int8(g, u, ClampedGlu(7.0)), ClampedGlu(7.0)(g, u))
+    check_rows(I.gated_activation_int8(g, u, Act.tanh), torch.tanh(g) * u)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 512), (700, 1000)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_dequantize(rows, cols, dtype):
+    held = I.quantize_rows(rand(rows, cols, seed=5))
+    assert torch.equal(held.dequantize(dtype), (held.values.float() * held.scale[:, None]).to(dtype))
+    part = I.Int8Rows(held.values[:, cols // 2:], held.scale)  # rows that start anywhere
+    assert torch.equal(part.dequantize(dtype), (part.values.float() * part.scale[:, None]).to(dtype))
+
+
+# ------------------------------------------------------------------------------------------------ products
+def int8(rows, cols, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    v = torch.randint(-128, 128, (rows, cols), generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
+    return I.Int8Rows(v, torch.rand(rows, generator=g, device="cuda") + 0.5)
+
+
+def check_product(rows, weight, bias=None, residual=None, out_dtype=BF, **form):
+    y = I._product(rows, weight, bias, residual, out_dtype, **form)
+    lib.check_status()
+    sums = rows.values.double() @ weight.values.double().t()
+    want = sums * rows.scale.double()[..., None] * weight.scale.double()
+    size = want.abs()
+    for t in (bias, residual):
+        if t is not None:
+            want, size = want + t.double(), size + t.double().abs()
+    # fp32: the sum of whole numbers and two scales rounded once each, two additions; then the rounding of the result
+    tol = 5 * 2.0 ** -24 * size + STEP[out_dtype] * want.abs()
+    assert y.dtype == out_dtype and y.shape == want.shape and bool(((y.double() - want).abs() <= tol).all())
+
+
+FORMS = [(1, 1, 1), (1, 16, 16), (2, 33, 100), (3, 17, 64), (7, 130, 513), (8, 256, 1000), (9, 300, 2048), (16, 64, 4096), (16, 5, 14336)]
+
+
+@pytest.mark.parametrize("M,N,K", FORMS)
+def test_product_of_few_rows(M, N, K):
+    check_product(int8(M, K, 1), int8(N, K, 2), form=1)
+    check_product(int8(M, K, 3), int8(N, K, 4), rand(N), rand(M, N), F32, form=1)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (5, 130, 100), (16, 128, 128), (17, 129, 1000), (33, 300, 640), (64, 257, 2048), (100, 128, 4096), (129, 384, 1111),
+                                   (256, 200, 768), (300, 130, 513), (513, 64, 256)])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
+def test_product_of_some_rows(M, N, K, splits):
+    check_product(int8(M, K, 1), int8(N, K, 2), form=2, splits=splits)
+    check_product(int8(M, K, 3), int8(N, K, 4), rand(N, dtype=F32), rand(M, N, dtype=F32), F32, form=2, splits=splits, stages=2)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (5, 130, 100), (256, 256, 128), (257, 300, 1000), (300, 513, 640), (1000, 777, 1111), (2048, 4096, 512)])
+def test_product_of_many_rows(M, N, K):
+    check_product(int8(M, K, 1), int8(N, K, 2), form=3)
+    check_product(int8(M, K, 3), int8(N, K, 4), rand(N, dtype=F32), rand(M, N), F32, form=3)
+    check_product(int8(M, K, 5), int8(N, K, 6), rand(N), rand(M, N, dtype=F32), BF, form=3)
+
+
+def test_product_of_the_largest_sums():
+    """-128 times -128 over the longest rows: the sum is 2^31 - 16384."""
+    K = I.MAX_COLS
+    for form, M in ((1, 3), (2, 20), (3, 20)):
+        v = torch.full((M, K), -128, dtype=torch.int8, device="cuda")
+        w = torch.full((5, K), -128, dtype=torch.int8, device="cuda")
+        y = I._product(I.Int8Rows(v, torch.ones(M, device="cuda")), I.Int8Rows(w, torch.ones(5, device="cuda")), out_dtype=F32, form=form)
+        assert bool((y == float(2 ** 31 - 16384)).all())
+
+
+def test_product_of_views():
+    """Rows with strides, rows that start anywhere, more dimensions, transposed biases and residuals."""
+    a, b = int8(40, 1000, 1), int8(70, 1000, 2)
+    check_product(I.Int8Rows(a.values[::2, 16:400], a.scale[::2]), I.Int8Rows(b.values[:, 16:400], b.scale))
+    check_product(I.Int8Rows(a.values[:, 3:502], a.scale), I.Int8Rows(b.values[:, 3:502], b.scale))
+    check_product(I.Int8Rows(a.values.view(4, 10, 1000), a.scale.view(4, 10)), b, residual=rand(10, 4, 70).transpose(0, 1))
+    check_product(I.Int8Rows(a.values.t().contiguous().t(), a.scale), b, bias=rand(70, 2)[:, 0], residual=rand(40, 100)[:, 7:77])
+    one = I.Int8Rows(a.values[0], a.scale[0])
+    assert torch.equal(I.int8_product(one, b), I.int8_product(I.Int8Rows(a.values[:1], a.scale[:1]), b)[0])
+    assert I.int8_product(I.Int8Rows(a.values[:0], a.scale[:0]), b).shape == (0, 70)
+    assert I.int8_product(a, I.Int8Rows(b.values[:0], b.scale[:0])).shape == (40, 0)
+
+
+def test_bytes_behind_a_row_do_not_count():
+    """A view's rows end inside 16 bytes whose rest belongs to others."""
+    for M, form in ((4, 1), (20, 2), (20, 3)):
+        a, b = int8(M, 512, 1), int8(33, 512, 2)
+        for cols in (1, 63, 65, 129, 500):
+            check_product(I.Int8Rows(a.values[:, :cols], a.scale), I.Int8Rows(b.values[:, :cols], b.scale), form=form)
+
+
+def test_nan_rows_stay_where_they_are():
+    x = rand(20, 256)
+    x[3, 4] = float("nan")
+    w = I.quantize_rows(rand(40, 256, seed=2))
+    y = I.int8_product(I.quantize_rows(x), w)
+    assert y[3].isnan().all() and int(y.isnan().sum()) == 40
