@@ -75,10 +75,47 @@ __device__ __forceinline__ float bias_at(const Params& p, int n) {
 __device__ __forceinline__ void finish(const Params& p, int m, int n, int sum, float sa, float sb, float bias) {
   float v = static_cast<float>(sum) * sa * sb + bias;
   if (p.flags & kResidual)
-    v += (p.flags & kResidualF32) ? reinterpret_cast<const float*>(p.residual)[m * p.ldr + n]
-                                  : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.residual)[m * p.ldr + n]);
+    v += (p.flags & kResidualF32) ? __ldg(reinterpret_cast<const float*>(p.residual) + m * p.ldr + n)
+                                  : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + n));
   if (p.flags & kOutF32) reinterpret_cast<float*>(p.C)[m * p.ldc + n] = v;
   else reinterpret_cast<__nv_bfloat16*>(p.C)[m * p.ldc + n] = __float2bfloat16(v);
+}
+// The same for the first `live` of kRows rows from m on in one column, whose lanes' neighbours hold the neighbouring columns: 32 of them write a line of
+// a row together.  `in`: the column exists.  sa: the rows' scales in shared memory, 16-byte aligned.
+template <int kRows>
+__device__ __forceinline__ void finish_column(const Params& p, int m, int live, int n, bool in, const int (&sum)[kRows], const float* sa, float sb, float bias) {
+  if (!in) return;
+  float v[kRows];
+#pragma unroll
+  for (int j = 0; j < kRows; j += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(sa + j);
+    v[j] = static_cast<float>(sum[j]) * f.x * sb + bias;
+    v[j + 1] = static_cast<float>(sum[j + 1]) * f.y * sb + bias;
+    v[j + 2] = static_cast<float>(sum[j + 2]) * f.z * sb + bias;
+    v[j + 3] = static_cast<float>(sum[j + 3]) * f.w * sb + bias;
+  }
+  if (p.flags & kResidual) {
+    if (p.flags & kResidualF32) {
+      const float* r = reinterpret_cast<const float*>(p.residual) + m * p.ldr + n;
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) v[j] += j < live ? __ldg(r + j * p.ldr) : 0.f;
+    } else {
+      const __nv_bfloat16* r = reinterpret_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + n;
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) v[j] += j < live ? __bfloat162float(__ldg(r + j * p.ldr)) : 0.f;
+    }
+  }
+  if (p.flags & kOutF32) {
+    float* o = reinterpret_cast<float*>(p.C) + m * p.ldc + n;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j, o += p.ldc)
+      if (j < live) *o = v[j];
+  } else {
+    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j, o += p.ldc)
+      if (j < live) *o = __float2bfloat16(v[j]);
+  }
 }
 
 // ================================================================ few rows
@@ -166,6 +203,10 @@ int launch_few(const void* A, const void* B, long long lda, long long ldb, const
 // that finishes them, a share of the rows each, so that every CTA reads, adds and writes as much as the others.
 constexpr int kMaxStages = 12;
 
+// Rows that each of `splits` CTAs finishes of `live` ones, and how far apart (in numbers) its channels lie in its buffer.
+__host__ __device__ inline int exchange_share(int live, int splits) { return ((live + splits - 1) / splits + 3) / 4 * 4; }
+__host__ __device__ inline int exchange_pitch(int share) { return 4 * (share / 4 | 1); }
+
 template <int TN>
 __global__ void __launch_bounds__(kThreads, 1)
 stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Params p, int stages, int kb_per_split) {
@@ -180,13 +221,14 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
   uint64_t* tfull_bar = empty_bar + kMaxStages;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  uint8_t* ring = smem + 1024;
+  float* s_scale = reinterpret_cast<float*>(smem + 1024);  // the rows' scales
+  uint8_t* ring = smem + 2048;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t splits;
+  int splits;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
   const int rank = static_cast<int>(cluster_ctarank());
-  const int n0 = static_cast<int>(blockIdx.x / splits) * 128;
+  const int n0 = static_cast<int>(blockIdx.x) / splits * 128;
   const int m0 = static_cast<int>(blockIdx.y) * TN;
   const int k_blocks = (p.K + BK - 1) / BK;
   const int kb0 = rank * kb_per_split;
@@ -248,62 +290,73 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
     }
   }
   __syncwarp();
+  // ---- the epilogue's operands, while the sums are made
+  const int quad = warp & 3;
+  const int live = min(TN, p.M - m0);
+  const int n = n0 + quad * 32 + lane;
+  const bool in = n < p.N;
+  float sb = 0.f, bias = 0.f;
+  if (warp >= 2) {
+    for (int i = threadIdx.x - 64; i < TN; i += 128) s_scale[i] = i < live ? __ldg(p.scale_a + m0 + i) : 0.f;
+    if (in) {
+      sb = __ldg(p.scale_b + n);
+      bias = bias_at(p, n);
+    }
+    named_bar_sync(1, 128);
+  }
   // ---- every thread: the tile's sums are complete in this CTA
   const bool ok = mbar_wait(tfull_bar, 0, abort_flag, p.status, 300, 0);
   tc_fence_after();
-  const int quad = warp & 3;
-  const int live = min(TN, p.M - m0);
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
   constexpr int kLoad = TN < 32 ? 16 : 32;
+  auto sums = [&](int c, int (&r)[kLoad]) {
+    uint32_t u[kLoad];
+    if constexpr (kLoad == 32) tmem_ld_32x32(taddr + c, u);
+    else tmem_ld_32x16(taddr + c, u);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < kLoad; ++j) r[j] = static_cast<int>(u[j]);
+  };
+  const bool all = __all_sync(0xffffffffu, ok);
   if (splits == 1) {
-    if (warp >= 2 && __all_sync(0xffffffffu, ok)) {
-      const int n = n0 + quad * 32 + lane;
-      const bool in = n < p.N;
-      const float sb = in ? __ldg(p.scale_b + n) : 0.f, bias = in ? bias_at(p, n) : 0.f;
+    if (warp >= 2 && all)
       for (int c = 0; c < live; c += kLoad) {
-        uint32_t r[kLoad];
-        if constexpr (kLoad == 32) tmem_ld_32x32(taddr + c, r);
-        else tmem_ld_32x16(taddr + c, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < kLoad; ++j)
-          if (in && c + j < live) finish(p, m0 + c + j, n, static_cast<int>(r[j]), __ldg(p.scale_a + m0 + c + j), sb, bias);
+        int r[kLoad];
+        sums(c, r);
+        finish_column<kLoad>(p, m0 + c, live - c, n, in, r, s_scale + c, sb, bias);
       }
-    }
   } else {
-    // rows [i share, (i + 1) share) of the tile are finished by CTA i: its buffer is [source CTA][row][channel], where the ring was
-    const int share = (live + static_cast<int>(splits) - 1) / static_cast<int>(splits);
-    int* mine = reinterpret_cast<int*>(ring);
+    // Rows [i share, (i + 1) share) of the tile are finished by CTA i: its buffer is [source CTA][channel][row], where the ring was.  Four rows travel
+    // together; the pitch of a channel is an odd multiple of 16 bytes, so that neighbouring lanes meet in no bank.
+    const int share = exchange_share(live, splits), pitch = exchange_pitch(share);
+    const uint32_t mine = smem_u32(ring);
+    const uint32_t slot = static_cast<uint32_t>((rank * 128 + quad * 32 + lane) * pitch * 4);
     cluster_sync_all();  // every CTA of the cluster is done with its ring
-    if (warp >= 2 && __all_sync(0xffffffffu, ok)) {
+    if (warp >= 2 && all)
       for (int c = 0; c < live; c += kLoad) {
-        uint32_t r[kLoad];
-        if constexpr (kLoad == 32) tmem_ld_32x32(taddr + c, r);
-        else tmem_ld_32x16(taddr + c, r);
-        tmem_ld_wait();
+        int r[kLoad];
+        sums(c, r);
 #pragma unroll
-        for (int j = 0; j < kLoad; ++j) {
+        for (int j = 0; j < kLoad; j += 4) {
           if (c + j < live) {
             const int to = (c + j) / share;
-            const int* at = mine + (rank * share + (c + j - to * share)) * 128 + quad * 32 + lane;
             uint32_t remote;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(at)), "r"(to));
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(r[j]) : "memory");
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(mine + slot + (c + j - to * share) * 4), "r"(to));
+            asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "r"(r[j]), "r"(r[j + 1]), "r"(r[j + 2]), "r"(r[j + 3]) : "memory");
           }
         }
       }
-    }
     cluster_sync_all();  // all parts have arrived
-    if (ok && !*abort_flag && threadIdx.x < 128) {
-      const int n = n0 + static_cast<int>(threadIdx.x);
-      if (n < p.N) {
-        const float sb = __ldg(p.scale_b + n), bias = bias_at(p, n);
-        const int first = rank * share, count = min(share, live - first);
-        for (int i = 0; i < count; ++i) {
-          int sum = 0;
-          for (uint32_t s = 0; s < splits; ++s) sum += mine[(s * share + i) * 128 + threadIdx.x];
-          finish(p, m0 + first + i, n, sum, __ldg(p.scale_a + m0 + first + i), sb, bias);
+    if (warp >= 2 && all && !*abort_flag) {
+      const int first = rank * share, count = min(share, live - first);
+      const int* part = reinterpret_cast<const int*>(ring) + (quad * 32 + lane) * pitch;
+      for (int i = 0; i < count; i += 4) {
+        int sum[4] = {0, 0, 0, 0};
+        for (int s = 0; s < splits; ++s) {
+          const int4 v = *reinterpret_cast<const int4*>(part + s * 128 * pitch + i);
+          sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
         }
+        finish_column<4>(p, m0 + first + i, count - i, n, in, sum, s_scale + first + i, sb, bias);
       }
     }
   }
@@ -324,8 +377,8 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
   if (splits > k_blocks) splits = k_blocks;
   const int per = (k_blocks + splits - 1) / splits;
   splits = (k_blocks + per - 1) / per;  // no empty share
-  // the ring also holds the exchanged sums: at most TN + splits - 1 rows of 128 (one more per CTA where the rows do not divide)
-  const int exchange = splits > 1 ? (TN + splits) * 512 : 0;
+  // the ring also holds the exchanged sums
+  const int exchange = splits > 1 ? splits * 128 * 4 * exchange_pitch(exchange_share(p.M < TN ? p.M : TN, splits)) : 0;
   if (stages > kMaxStages) stages = kMaxStages;
   if (stages > 220 * 1024 / kStage) stages = 220 * 1024 / kStage;
   if (stages > per) stages = per;
@@ -348,7 +401,7 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.N + 127) / 128 * splits), static_cast<unsigned>(row_tiles));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = 2048 + bytes;
+  cfg.dynamicSmemBytes = 3072 + bytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -365,7 +418,7 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
 constexpr int BN = 256, BMP = 256, BMC = 128;
 constexpr int kPairStage = (BMC + BN / 2) * BK;  // per CTA
 constexpr int kPairStages = 6;
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + (2 * kPairStages + 4) * 8 + 16;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 2 * BN * 4 + (2 * kPairStages + 4) * 8 + 16;
 
 __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& mb, int& nb) {
   constexpr int GM = 4;  // four row tiles stay in the L2 while the raster sweeps N
@@ -378,7 +431,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kPairStages * kPairStage);
+  float* s_scale = reinterpret_cast<float*>(smem + kPairStages * kPairStage);  // the columns' scales, of one tile and the next
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_scale + 2 * BN);
   uint64_t* empty_bar = full_bar + kPairStages;
   uint64_t* tfull_bar = empty_bar + kPairStages;
   uint64_t* tempty_bar = tfull_bar + 2;
@@ -466,15 +520,23 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     const int quad = warp & 3;
     int buf = 0;
     uint32_t tphase = 0;
+    bool alive = true;
     for (int t = first; t < tiles; t += step) {
       int mb, nb;
       tile_coords(t, tiles_m, tiles_n, mb, nb);
-      const bool ok = mbar_wait(&tfull_bar[buf], tphase, abort_flag, p.status, 300, buf);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
       const int m = mb * BMP + static_cast<int>(cta) * BMC + quad * 32 + lane;
       const bool in = m < p.M;
       const float sa = in ? __ldg(p.scale_a + m) : 0.f;
+      float* sb = s_scale + buf * BN;  // (the tile before the last one read it, and all four warps have been at a barrier since)
+#pragma unroll
+      for (int j = 0; j < BN; j += 128) {
+        const int at = j + static_cast<int>(threadIdx.x) - 64;
+        sb[at] = nb * BN + at < p.N ? __ldg(p.scale_b + nb * BN + at) : 0.f;
+      }
+      named_bar_sync(1, 128);
+      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&tfull_bar[buf], tphase, abort_flag, p.status, 300, buf));
+      if (!alive) continue;  // the other warps wait for this one at the barrier above, tile by tile
+      tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + buf * BN;
 #pragma unroll 1
       for (int c = 0; c < BN; c += 32) {
@@ -486,18 +548,13 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         if (!in) continue;
         const int cols = min(32, p.N - n0);
         float v[32];
-        if (cols == 32 && (reinterpret_cast<uintptr_t>(p.scale_b) & 15) == 0) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float4 s = __ldg(reinterpret_cast<const float4*>(p.scale_b + n0) + q);
-            v[4 * q] = static_cast<float>(static_cast<int>(r[4 * q])) * sa * s.x;
-            v[4 * q + 1] = static_cast<float>(static_cast<int>(r[4 * q + 1])) * sa * s.y;
-            v[4 * q + 2] = static_cast<float>(static_cast<int>(r[4 * q + 2])) * sa * s.z;
-            v[4 * q + 3] = static_cast<float>(static_cast<int>(r[4 * q + 3])) * sa * s.w;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = j < cols ? static_cast<float>(static_cast<int>(r[j])) * sa * __ldg(p.scale_b + n0 + j) : 0.f;
+        for (int q = 0; q < 8; ++q) {
+          const float4 f = *reinterpret_cast<const float4*>(sb + c + 4 * q);
+          v[4 * q] = static_cast<float>(static_cast<int>(r[4 * q])) * sa * f.x;
+          v[4 * q + 1] = static_cast<float>(static_cast<int>(r[4 * q + 1])) * sa * f.y;
+          v[4 * q + 2] = static_cast<float>(static_cast<int>(r[4 * q + 2])) * sa * f.z;
+          v[4 * q + 3] = static_cast<float>(static_cast<int>(r[4 * q + 3])) * sa * f.w;
         }
         if (p.flags & kBias) {
 #pragma unroll

@@ -2,154 +2,315 @@
 // the row is made: from the RMS norm of x (+ residual), from a gated activation, or from a row as it is.  And back: q[j] * scale.
 //
 // The mathematics.  A norm multiplies a row by a factor f = rsqrt(mean h^2 + eps) of its own, which leaves q as it is and joins the scale, so the sum
-// of squares and the largest |h w| are taken in one pass over the row and one exchange between its threads.  127 y / max |y| is the correctly
-// rounded quotient wherever rounding it to a whole number could go either way: the product with the reciprocal decides the rest, and the few
-// elements that it leaves within 1e-4 of a tie are divided (the product is off by at most 127 * 2^-22).  bf16 rows need this: half of the largest
-// value lies on a tie, and a row often holds it.  A row below 2^-100 is stored as zeros with scale 0 (its reciprocal could overflow); a row with an
+// of squares and the largest |h w| are taken in one pass over the row and one exchange between its threads.  127 y / max |y| is formed with the reciprocal
+// of max |y| (off by at most 127 * 2^-22); for elements that this leaves within 1e-4 of a tie the sign of 127 y - border max |y|, in one
+// fused operation, says on which side of it they are.  bf16 rows need this: half of the largest value lies on a tie, and a row often holds it.  A row below 2^-100 (or, ahead of its factor, below 2^-120) is stored as zeros with scale 0; a row with an
 // infinity or a NaN as zeros with scale NaN, so that everything made from it is NaN.
 //
 // What bounds it: memory.  One pass reads the inputs and writes 1 byte per element (and h, 2 or 4).  The threads of a row keep it in registers as
 // fp32 between the reduction and the write: a warp per row up to 1024 columns, up to 1024 threads per row beyond that, and above 32768
 // columns the row is read twice.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace lvb {
 namespace int8_rows {
 
-constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
+constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100
+constexpr float kLeast = 7.52316384526264e-37f;  // 2^-120: 127 over it is still a finite number
 
 enum Act : int { kSilu = 0, kGeluTanh = 1, kGelu = 2, kRelu = 3, kQuickGelu = 4 };
 
-__device__ __forceinline__ float activation(float g, int act) {
-  switch (act) {
-    case kSilu: return __fdividef(g, 1.f + __expf(-g));  // 2^-20 relative, far below half a step of the 8 bits
-    case kGeluTanh: return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
-    case kGelu: return 0.5f * g * (1.f + erff(g * 0.7071067811865476f));
-    case kRelu: return g != g ? g : fmaxf(g, 0.f);
-    default: return __fdividef(g, 1.f + __expf(-1.702f * g));
+// x sigmoid(a x) of two numbers, 2^-20 relative: far below half a step of the 8 bits.  An exponential that runs over makes the quotient 0, as it should be.
+__device__ __forceinline__ F32x2 swish2(F32x2 x, float a) {
+  const float k = -1.4426950408889634f * a;  // log2 e
+  float e0, e1;
+  f2_split(f2_mul(x, f2(k, k)), e0, e1);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
+  f2_split(f2_add(f2(e0, e1), f2(1.f, 1.f)), e0, e1);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e1));
+  return f2_mul(x, f2(e0, e1));
+}
+template <int kAct>
+__device__ __forceinline__ F32x2 activation2(F32x2 g) {
+  if constexpr (kAct == kSilu) return swish2(g, 1.f);
+  if constexpr (kAct == kQuickGelu) return swish2(g, 1.702f);
+  if constexpr (kAct == kGeluTanh) {  // (1 + tanh u) / 2 = sigmoid(2 u)
+    const F32x2 g2 = f2_mul(g, g), u = f2_mul(g, f2_fma(g2, f2(0.044715f, 0.044715f), f2(1.f, 1.f)));
+    const float k = -1.4426950408889634f * 2.f * 0.7978845608028654f;
+    float e0, e1;
+    f2_split(f2_mul(u, f2(k, k)), e0, e1);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
+    f2_split(f2_add(f2(e0, e1), f2(1.f, 1.f)), e0, e1);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e0));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e1));
+    return f2_mul(g, f2(e0, e1));
   }
+  float a, b;
+  f2_split(g, a, b);
+  if constexpr (kAct == kGelu) return f2(0.5f * a * (1.f + erff(a * 0.7071067811865476f)), 0.5f * b * (1.f + erff(b * 0.7071067811865476f)));
+  return f2(a != a ? a : fmaxf(a, 0.f), b != b ? b : fmaxf(b, 0.f));
 }
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-// Eight elements from column c on (`live` of them exist, the others are zero); 16-byte loads where the address allows.
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, int live, float (&v)[8]) {
-  if (live >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(u[j] << 16);
-      v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < live ? __bfloat162float(p[j]) : 0.f;
-  }
-}
-__device__ __forceinline__ void load8(const float* p, int live, float (&v)[8]) {
-  if (live >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < live ? p[j] : 0.f;
-  }
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, int live, const float (&v)[8]) {
-  if (live >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < live) p[j] = __float2bfloat16(v[j]);
-  }
-}
-__device__ __forceinline__ void store8(float* p, int live, const float (&v)[8]) {
-  if (live >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < live) p[j] = v[j];
-  }
-}
-
-// ---- where a row comes from: get() gives eight of its elements and adds what the row's factor needs to `ss`
+// ---- eight elements of a row
+// A row may start anywhere.  Where it does not start on 16 bytes, one aligned load more and a shift bring the eight elements (the neighbouring lanes'
+// loads overlap in the L1); at the ends of what the caller gave, [lo, hi), they come one by one.
 template <typename T>
-struct Plain {
-  const T* x;
-  long long ldx;
-  __device__ __forceinline__ void get(long long row, int c, int live, float (&y)[8], float&) const { load8(x + row * ldx + c, live, y); }
-  __device__ __forceinline__ float factor(float, int) const { return 1.f; }
-  static constexpr bool kSum = false;
+struct Span {
+  const T* p;
+  long long ld;
+  const char *lo, *hi;
+  Span() = default;
+  Span(const void* x, long long ld, long long rows, int cols)
+      : p(static_cast<const T*>(x)), ld(ld), lo(static_cast<const char*>(x)), hi(reinterpret_cast<const char*>(static_cast<const T*>(x) + (rows - 1) * ld + cols)) {}
 };
-
-template <typename T>
-struct Norm {
-  const T* x;
-  const T* r;  // may be null
-  T* h;        // written where there is a residual
-  const void* w;
-  long long ldx, ldr, ldh;
-  int w_f32;
-  float w_offset, eps;
-  static constexpr bool kSum = true;
-  __device__ __forceinline__ void get(long long row, int c, int live, float (&y)[8], float& ss) const {
-    load8(x + row * ldx + c, live, y);
-    if (r != nullptr) {
-      float b[8];
-      load8(r + row * ldr + c, live, b);
+// The words that follow the first `bytes` (even, below 16) of u, moved to its front.
+template <int kOut, int kIn>
+__device__ __forceinline__ void shift_words(uint32_t (&u)[kIn], uint32_t bytes) {
+  static_assert(kIn >= kOut + 4, "three words and a half may go");
+  if (bytes & 8)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[j] += b[j];
-        if constexpr (sizeof(T) == 2) y[j] = __bfloat162float(__float2bfloat16(y[j]));  // the sum in the rows' type is what goes on, here too
+    for (int j = 0; j < kOut + 2; ++j) u[j] = u[j + 2];
+  if (bytes & 4)
+#pragma unroll
+    for (int j = 0; j < kOut + 1; ++j) u[j] = u[j + 1];
+  if (bytes & 2)
+#pragma unroll
+    for (int j = 0; j < kOut; ++j) u[j] = __funnelshift_r(u[j], u[j + 1], 16);
+}
+template <typename T>
+struct Raw {  // eight elements as they lie in memory
+  static constexpr int kWords = 2 * sizeof(T);
+  uint32_t u[kWords];
+  template <bool kAligned>
+  __device__ __forceinline__ void load(const T* p, int live, const char* lo, const char* hi) {
+    if constexpr (kAligned) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 w = live > 0 ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+        u[4 * i] = w.x; u[4 * i + 1] = w.y; u[4 * i + 2] = w.z; u[4 * i + 3] = w.w;
       }
-      store8(h + row * ldh + c, live, y);
+      return;
     }
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const char* base = reinterpret_cast<const char*>(p) - off;
+    if (live >= 8 && off == 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
-    if (w != nullptr) {
-      float f[8];
-      if (w_f32) load8(reinterpret_cast<const float*>(w) + c, live, f);
-      else load8(reinterpret_cast<const __nv_bfloat16*>(w) + c, live, f);
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(base) + i);
+        u[4 * i] = w.x; u[4 * i + 1] = w.y; u[4 * i + 2] = w.z; u[4 * i + 3] = w.w;
+      }
+    } else if (live >= 8 && base >= lo && base + 4 * kWords + 16 <= hi) {
+      uint32_t e[kWords + 4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < live) y[j] *= f[j] + w_offset;
+      for (int i = 0; i < kWords / 4 + 1; ++i) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(base) + i);
+        e[4 * i] = w.x; e[4 * i + 1] = w.y; e[4 * i + 2] = w.z; e[4 * i + 3] = w.w;
+      }
+      shift_words<kWords>(e, off);
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) u[j] = e[j];
+    } else if constexpr (sizeof(T) == 2) {
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = (2 * j < live ? __ldg(q + 2 * j) : 0u) | (2 * j + 1 < live ? static_cast<uint32_t>(__ldg(q + 2 * j + 1)) << 16 : 0u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = j < live ? __float_as_uint(__ldg(p + j)) : 0u;
     }
   }
-  __device__ __forceinline__ float factor(float ss, int cols) const { return rsqrtf(ss / static_cast<float>(cols) + eps); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(u[j] << 16);
+        v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(u[j]);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(v[j]);
+    }
+  }
+  __device__ __forceinline__ void put(T* p, int from, int to) const {  // elements [from, to) one by one
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j >= from && j < to) {
+        if constexpr (sizeof(T) == 2) reinterpret_cast<unsigned short*>(p)[j] = static_cast<unsigned short>(u[j / 2] >> (16 * (j & 1)));
+        else reinterpret_cast<uint32_t*>(p)[j] = u[j];
+      }
+  }
+  // All lanes of a warp, each with the eight elements behind those of the lane before it (`live` of them exist, none where it is not positive).  Where they do not
+  // start on 16 bytes, a lane writes the aligned words up to its last whole ones, the first of them with the end of what the lane before it holds.
+  template <bool kAligned>
+  __device__ __forceinline__ void store(T* p, int live) const {
+    if constexpr (kAligned) {
+      if (live > 0) {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+      }
+      return;
+    }
+    const int lane = threadIdx.x & 31;
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    if (off == 0) {
+      if (live >= 8) {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+      } else if (live > 0) {
+        put(p, 0, live);
+      }
+      return;
+    }
+    uint32_t e[kWords + 4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = __shfl_up_sync(0xffffffffu, u[kWords - 4 + j], 1);
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) e[4 + j] = u[j];
+    const int tail = static_cast<int>(off / sizeof(T));  // elements of a lane that the next lane writes, if it has eight
+    if (live >= 8 && lane > 0) {
+      shift_words<kWords>(e, 16 - off);
+      uint4* q = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p) - off);
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) q[i] = make_uint4(e[4 * i], e[4 * i + 1], e[4 * i + 2], e[4 * i + 3]);
+      if (lane == 31 || live < 16) put(p, 8 - tail, 8);
+    } else if (live > 0) {
+      put(p, 0, lane == 0 && live >= 16 ? 8 - tail : min(live, 8));
+    }
+  }
 };
 
-template <typename T>
-struct Glu {
-  const T* g;
-  const T* u;
-  long long ldg, ldu;
-  int act;
+// ---- where a row comes from: load() starts the reads of eight of its elements, get() gives them and adds what the row's factor needs to `ss`.  All
+// lanes of a warp call get(); `live` of the elements exist (none where it is not positive), the others are zero.  kAligned: rows, and the groups of eight
+// in them, start on 16 bytes and are whole.
+template <typename T, bool kAligned>
+struct Plain {
+  Span<T> x;
+  using Type = T;
+  using In = Raw<T>;
   static constexpr bool kSum = false;
-  __device__ __forceinline__ void get(long long row, int c, int live, float (&y)[8], float&) const {
-    float b[8];
-    load8(g + row * ldg + c, live, y);
-    load8(u + row * ldu + c, live, b);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = activation(y[j], act) * b[j];
-  }
-  __device__ __forceinline__ float factor(float, int) const { return 1.f; }
+  __device__ __forceinline__ void load(In& in, long long row, int c, int live) const { in.template load<kAligned>(x.p + row * x.ld + c, live, x.lo, x.hi); }
+  __device__ __forceinline__ void get(const In& in, long long, int, int, float (&y)[8], F32x2&) const { in.get(y); }
+  __device__ __forceinline__ float factor(float) const { return 1.f; }
 };
+
+template <typename T, bool kResidual, bool kAligned>
+struct Norm {
+  Span<T> x, r;
+  T* h;  // written where there is a residual
+  const void* w;
+  long long ldh;
+  int w_f32;
+  float w_offset, eps, per_col;  // per_col: 1 / columns
+  struct In {
+    Raw<T> a, b;  // (without a residual the second is never loaded and takes no register)
+  };
+  using Type = T;
+  static constexpr bool kSum = true;
+  __device__ __forceinline__ void load(In& in, long long row, int c, int live) const {
+    in.a.template load<kAligned>(x.p + row * x.ld + c, live, x.lo, x.hi);
+    if constexpr (kResidual) in.b.template load<kAligned>(r.p + row * r.ld + c, live, r.lo, r.hi);
+  }
+  template <typename W>
+  __device__ __forceinline__ void weigh(const W* p, int live, float (&y)[8]) const {
+    Raw<W> raw;
+    raw.template load<kAligned>(p, live, nullptr, nullptr);
+    float f[8];
+    raw.get(f);
+    if (w_offset != 0.f) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] += w_offset;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) f2_split(f2_mul(f2(y[j], y[j + 1]), f2(f[j], f[j + 1])), y[j], y[j + 1]);
+  }
+  __device__ __forceinline__ void get(const In& in, long long row, int c, int live, float (&y)[8], F32x2& ss) const {
+    in.a.get(y);
+    if constexpr (kResidual) {
+      float b[8];
+      in.b.get(b);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) f2_split(f2_add(f2(y[j], y[j + 1]), f2(b[j], b[j + 1])), y[j], y[j + 1]);
+      Raw<T> sum;
+      sum.set(y);
+      sum.get(y);  // the sum in the rows' type is what goes on, here too
+      sum.template store<kAligned>(h + row * ldh + c, live);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) ss = f2_fma(f2(y[j], y[j + 1]), f2(y[j], y[j + 1]), ss);
+    if (w != nullptr && live > 0) {
+      if (w_f32) weigh(reinterpret_cast<const float*>(w) + c, live, y);
+      else weigh(reinterpret_cast<const __nv_bfloat16*>(w) + c, live, y);
+    }
+  }
+  __device__ __forceinline__ float factor(float ss) const { return rsqrtf(ss * per_col + eps); }
+};
+
+template <typename T, int kAct, bool kAligned>
+struct Glu {
+  Span<T> g, u;
+  struct In {
+    Raw<T> a, b;
+  };
+  using Type = T;
+  static constexpr bool kSum = false;
+  __device__ __forceinline__ void load(In& in, long long row, int c, int live) const {
+    in.a.template load<kAligned>(g.p + row * g.ld + c, live, g.lo, g.hi);
+    in.b.template load<kAligned>(u.p + row * u.ld + c, live, u.lo, u.hi);
+  }
+  __device__ __forceinline__ void get(const In& in, long long, int, int, float (&y)[8], F32x2&) const {
+    float b[8];
+    in.a.get(y);
+    in.b.get(b);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) f2_split(f2_mul(activation2<kAct>(f2(y[j], y[j + 1])), f2(b[j], b[j + 1])), y[j], y[j + 1]);
+  }
+  __device__ __forceinline__ float factor(float) const { return 1.f; }
+};
+
+// The largest of three magnitudes, NaN if one of them is
+__device__ __forceinline__ float largest_of(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // Eight whole numbers as bytes.  Adding 1.5 * 2^23 rounds to the nearest whole number, ties to even, and leaves it in the low bits.
 __device__ __forceinline__ uint2 whole8(const float (&y)[8], float top, float inv) {
   constexpr float kMagic = 12582912.f;
   uint32_t b[8];
+  float far = 0.f;  // how far the furthest lies from its whole number
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float t = y[j] * inv;
-    float m = t + kMagic;
-    if (fabsf(t - (m - kMagic)) > 0.4999f) m = __fdiv_rn(y[j] * 127.f, top) + kMagic;
-    b[j] = __float_as_uint(m);
+  for (int j = 0; j < 8; j += 2) {
+    const F32x2 v = f2(y[j], y[j + 1]), k = f2(inv, inv);
+    const F32x2 m = f2_fma(v, k, f2(kMagic, kMagic));
+    const F32x2 q = f2_add(f2(kMagic, kMagic), f2_mul(m, f2(-1.f, -1.f)));
+    float d0, d1, m0, m1;
+    f2_split(f2_fma(v, k, q), d0, d1);
+    f2_split(m, m0, m1);
+    far = largest_of(far, d0, d1);
+    b[j] = __float_as_uint(m0);
+    b[j + 1] = __float_as_uint(m1);
+  }
+  if (far > 0.4999f) {  // is 127 y above, on or below the border of two whole numbers, (floor + 1/2) max |y|?
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float border = floorf(y[j] * inv) + 0.5f;
+      const float above = fmaf(-border, top, y[j] * 127.f);
+      b[j] = __float_as_uint(__fadd_rn(above > 0.f ? border + 0.5f : above < 0.f ? border - 0.5f : border, kMagic));
+    }
   }
   uint2 o;
   o.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
@@ -157,137 +318,211 @@ __device__ __forceinline__ uint2 whole8(const float (&y)[8], float top, float in
   return o;
 }
 
-// G threads per row, each with kChunks groups of eight elements in registers; kChunks == 0: any number of them, each made twice.  q has room for
-// whole groups of eight up to the end of its row stride.
-template <class Src, int G, int kChunks>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) quantize_kernel(Src src, long long rows, int cols, int8_t* __restrict__ q, long long ldq,
-                                                                     float* __restrict__ scale) {
-  constexpr int kBlock = G < 128 ? 128 : G;
-  constexpr int kWarps = G / 32;
-  const int lane = threadIdx.x & 31;
-  const int t = threadIdx.x % G;
-  const long long row = static_cast<long long>(blockIdx.x) * (kBlock / G) + threadIdx.x / G;
-  chain_wait();
-  if (kWarps <= 1 && row >= rows) return;  // whole warps; a larger group is a whole CTA and has its row
-  float y[kChunks > 0 ? kChunks : 1][8];
-  float ss = 0.f;
-  uint32_t top = 0;  // magnitudes order as their bits, infinities and NaN last
-  auto note = [&](const float (&v)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-  };
-  if constexpr (kChunks > 0) {
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int c = (t + i * G) * 8;
-      if (c < cols) {
-        src.get(row, c, cols - c, y[i], ss);
-        note(y[i]);
-      }
-    }
-  } else {
-    for (int c = t * 8; c < cols; c += G * 8) {
-      src.get(row, c, cols - c, y[0], ss);
-      note(y[0]);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if constexpr (Src::kSum) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  }
-  if constexpr (kWarps > 1) {
-    __shared__ uint32_t s_top[32];
-    __shared__ float s_ss[32];
-    if (lane == 0) {
-      s_top[threadIdx.x >> 5] = top;
-      s_ss[threadIdx.x >> 5] = ss;
+constexpr int kRowWarps = 4;  // of a block whose warps have a row each
+constexpr int kBlockRegs = 65536;
+
+constexpr int kHeldGroups = 2;   // groups of eight per thread of a block that has a row
+constexpr int kMostThreads = 1024;
+
+// kWarp: a row per warp, else a row per block.  kChunks: groups of eight elements per thread, held in registers; 0: any number of them, each made twice.
+// A block goes through rows far apart and starts the reads of its next row before it reduces and writes the one it has.  q has room for whole groups of
+// eight up to the end of its row stride.
+template <class Src, bool kWarp, int kChunks>
+__global__ void __launch_bounds__(kWarp ? 32 * kRowWarps : kMostThreads) quantize_kernel(Src src, long long rows, int cols, int8_t* __restrict__ q,
+                                                                                               long long ldq, float* __restrict__ scale) {
+  __shared__ uint32_t s_top[2][32];
+  __shared__ float s_ss[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t = kWarp ? lane : static_cast<int>(threadIdx.x);
+  const int group = kWarp ? 32 : static_cast<int>(blockDim.x);
+  const int warps = group >> 5;
+  const long long step = kWarp ? static_cast<long long>(gridDim.x) * kRowWarps : gridDim.x;
+  long long row = kWarp ? static_cast<long long>(blockIdx.x) * kRowWarps + warp : blockIdx.x;
+  if constexpr (!kWarp) {
+    if (threadIdx.x < 32) {  // the partial results of warps that do not exist
+      s_top[0][lane] = s_top[1][lane] = 0;
+      s_ss[0][lane] = s_ss[1][lane] = 0.f;
     }
     __syncthreads();
-    top = lane < kWarps ? s_top[lane] : 0u;
-    ss = lane < kWarps ? s_ss[lane] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if constexpr (Src::kSum) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    }
   }
-  const float f = src.factor(ss, cols);
-  const float most = __uint_as_float(top);
-  const bool finite = top < 0x7F800000u && f == f;
-  const bool live = finite && most * f >= kTiny;
-  const float inv = live ? 127.f / most : 0.f;
-  const float s = live ? most * f / 127.f : finite ? 0.f : __uint_as_float(0x7FC00000u);
-  int8_t* out = q + row * ldq;
-  auto put = [&](int c, const float (&v)[8]) { *reinterpret_cast<uint2*>(out + c) = live ? whole8(v, most, inv) : make_uint2(0, 0); };
-  if constexpr (kChunks > 0) {
+  chain_wait();
+  constexpr int kHeld = kChunks > 0 ? kChunks : 1;
+  const int limit = (cols + 255) / 256 * 256;  // whole warps take part to the end of a row
+  typename Src::In in[kHeld];
+  auto load = [&](long long at) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int c = (t + i * G) * 8;
-      if (c < cols) put(c, y[i]);
+      const int c = (t + i * group) * 8;
+      src.load(in[i], at, c, cols - c);
     }
-  } else {
-    for (int c = t * 8; c < cols; c += G * 8) {
-      float again = 0.f;
-      src.get(row, c, cols - c, y[0], again);
-      put(c, y[0]);
+  };
+  if (row < rows) load(row);
+  for (int odd = 0; row < rows; row += step, odd ^= 1) {
+    float y[kHeld][8];
+    F32x2 ss2 = f2(0.f, 0.f);
+    float largest = 0.f;
+    auto note = [&](const float (&v)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) largest = largest_of(largest, v[j], v[j + 1]);
+    };
+    if constexpr (kChunks > 0) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = (t + i * group) * 8;
+        src.get(in[i], row, c, cols - c, y[i], ss2);
+        note(y[i]);
+      }
+      if (row + step < rows) load(row + step);
+    } else {
+      for (int c = t * 8; c < limit; c += group * 8) {
+        src.load(in[0], row, c, cols - c);
+        src.get(in[0], row, c, cols - c, y[0], ss2);
+        note(y[0]);
+      }
     }
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));  // magnitudes order as their bits, infinities and NaN last
+    float ss = 0.f;
+    if constexpr (Src::kSum) {
+      float a, b;
+      f2_split(ss2, a, b);
+      ss = warp_sum(a + b);
+    }
+    if constexpr (!kWarp) {
+      if (lane == 0) {
+        s_top[odd][warp] = top;
+        s_ss[odd][warp] = ss;
+      }
+      __syncthreads();  // (one per row: what this row reads is written again two rows on, behind the next row's)
+      const uint4* tops = reinterpret_cast<const uint4*>(s_top[odd]);
+      const float4* sums = reinterpret_cast<const float4*>(s_ss[odd]);
+      top = 0;
+      ss = 0.f;
+      for (int i = 0; i < warps; i += 4) {
+        const uint4 v = tops[i / 4];
+        top = max(max(top, max(v.x, v.y)), max(v.z, v.w));
+        if constexpr (Src::kSum) {
+          const float4 a = sums[i / 4];
+          ss += (a.x + a.y) + (a.z + a.w);
+        }
+      }
+    }
+    const float f = src.factor(ss);
+    const float most = __uint_as_float(top);
+    const bool finite = top < 0x7F800000u && f == f;
+    const bool live = finite && most * f >= kTiny && most >= kLeast;
+    // (the quick quotient is good for divisors up to 2^126; 1e30 keeps the quotient a normal number, too)
+    const float inv = !live ? 0.f : most < 1e30f ? __fdividef(127.f, most) : 127.f / most;
+    int8_t* out = q + row * ldq;
+    auto put = [&](int c, const float (&v)[8]) { *reinterpret_cast<uint2*>(out + c) = live ? whole8(v, most, inv) : make_uint2(0, 0); };
+    if constexpr (kChunks > 0) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = (t + i * group) * 8;
+        if (c < cols) put(c, y[i]);
+      }
+    } else {
+      for (int c = t * 8; c < limit; c += group * 8) {
+        F32x2 again = f2(0.f, 0.f);
+        src.load(in[0], row, c, cols - c);
+        src.get(in[0], row, c, cols - c, y[0], again);
+        if (c < cols) put(c, y[0]);
+      }
+    }
+    if (t == 0) scale[row] = live ? most * f / 127.f : finite ? 0.f : __uint_as_float(0x7FC00000u);
   }
-  if (t == 0) scale[row] = s;
 }
 
-template <class Src, int G, int kChunks>
-int launch(const Src& src, long long rows, int cols, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
-  constexpr int kBlock = G < 128 ? 128 : G;
-  const long long blocks = (rows + kBlock / G - 1) / (kBlock / G);
-  if (blocks > 0x7FFFFFFFll) return kErrTooLarge;
-  return launch_chained(quantize_kernel<Src, G, kChunks>, dim3(static_cast<unsigned>(blocks)), dim3(kBlock), 0, s, src, rows, cols, q, ldq, scale) == cudaSuccess
+template <class Src, bool kWarp, int kChunks>
+int launch(const Src& src, long long rows, int cols, int threads, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
+  const long long blocks = kWarp ? (rows + kRowWarps - 1) / kRowWarps : rows;
+  static int resident = 0;  // blocks per SM, of 32 threads
+  if (resident == 0) {
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, quantize_kernel<Src, kWarp, kChunks>) != cudaSuccess) return kErrCuda;
+    resident = kBlockRegs / (32 * ((attr.numRegs + 7) / 8 * 8));
+  }
+  const int per_sm = resident / (threads / 32) < 2048 / threads ? resident / (threads / 32) : 2048 / threads;
+  const long long most = static_cast<long long>(num_sms()) * (per_sm < 1 ? 1 : per_sm);
+  return launch_chained(quantize_kernel<Src, kWarp, kChunks>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(threads), 0, s, src, rows, cols, q,
+                        ldq, scale) == cudaSuccess
              ? kErrOk
              : kErrCuda;
 }
+
+inline bool aligned16(const void* p, long long bytes) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (bytes & 15) == 0; }
 
 template <class Src>
 int quantize(const Src& src, long long rows, int cols, void* q, long long ldq, float* scale, void* stream) {
   if (rows <= 0 || cols <= 0 || q == nullptr || scale == nullptr || (ldq & 7) || ldq < cols || (reinterpret_cast<uintptr_t>(q) & 7)) return kErrBadArg;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int8_t* o = reinterpret_cast<int8_t*>(q);
-  if (cols <= 256) return launch<Src, 32, 1>(src, rows, cols, o, ldq, scale, s);
-  if (cols <= 512) return launch<Src, 32, 2>(src, rows, cols, o, ldq, scale, s);
-  if (cols <= 1024) return launch<Src, 32, 4>(src, rows, cols, o, ldq, scale, s);
-  if (cols <= 2048) return launch<Src, 128, 2>(src, rows, cols, o, ldq, scale, s);
-  if (cols <= 4096) return launch<Src, 256, 2>(src, rows, cols, o, ldq, scale, s);
-  if (cols <= 8192) return launch<Src, 512, 2>(src, rows, cols, o, ldq, scale, s);
-  if (cols <= 16384) return launch<Src, 512, 4>(src, rows, cols, o, ldq, scale, s);
-  if (cols <= 32768) return launch<Src, 1024, 4>(src, rows, cols, o, ldq, scale, s);
-  return launch<Src, 1024, 0>(src, rows, cols, o, ldq, scale, s);
+  constexpr int kChunks = kHeldGroups, kWarpBlock = 32 * kRowWarps;
+  if (cols <= 512) return launch<Src, true, 2>(src, rows, cols, kWarpBlock, o, ldq, scale, s);
+  if (cols <= kMostThreads * 8 * kChunks) {
+    const int units = (cols + 7) / 8, threads = (units + kChunks - 1) / kChunks;
+    return launch<Src, false, kChunks>(src, rows, cols, (threads + 31) / 32 * 32, o, ldq, scale, s);
+  }
+  return launch<Src, false, 0>(src, rows, cols, kMostThreads, o, ldq, scale, s);
 }
 
-// out[row, j] = q[row, j] * scale[row]; 16 elements per thread where the addresses allow, rounded once
-template <typename T>
+// out = q * scale, rounded once, for dense rows `out`.  kWhole: rows are whole groups of eight; else a group lies across the ends of rows.
+template <typename T, bool kWhole>
 __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restrict__ q, long long ldq, const float* __restrict__ scale, long long rows,
                                                          int cols, T* __restrict__ out) {
   chain_wait();
-  const int units = (cols + 7) / 8;
-  const long long total = rows * units;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long row = i / units;
-    const int c = static_cast<int>(i - row * units) * 8, live = min(8, cols - c);
-    const int8_t* p = q + row * ldq + c;
-    const float s = scale[row];
+  const long long total = rows * cols;
+  const unsigned units = cols / 8;
+  const bool narrow = total < (1ll << 32);  // a division of 32 bits is three times as fast
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i * 8 < total; i += gridDim.x * 256ll) {
     float v[8];
-    if (live == 8 && (reinterpret_cast<uintptr_t>(p) & 7) == 0) {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
+    Raw<T> whole;  // (groups of eight of a dense `out` start on 16 bytes)
+    if constexpr (kWhole) {
+      const long long row = narrow ? static_cast<unsigned>(i) / units : i / units;
+      const int8_t* p = q + row * ldq + (i - row * units) * 8;
+      const float s = __ldg(scale + row);
+      if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = static_cast<float>(static_cast<int8_t>(w.x >> (8 * j))) * s;
-        v[4 + j] = static_cast<float>(static_cast<int8_t>(w.y >> (8 * j))) * s;
+        for (int j = 0; j < 4; ++j) {
+          v[j] = static_cast<float>(static_cast<int8_t>(w.x >> (8 * j))) * s;
+          v[4 + j] = static_cast<float>(static_cast<int8_t>(w.y >> (8 * j))) * s;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(__ldg(p + j)) * s;
       }
+      whole.set(v);
+      whole.template store<true>(out + i * 8, 8);
     } else {
+      long long row = narrow ? static_cast<unsigned>(i * 8) / static_cast<unsigned>(cols) : i * 8 / cols;
+      int c = static_cast<int>(i * 8 - row * cols);
+      float s = __ldg(scale + row);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < live ? static_cast<float>(p[j]) * s : 0.f;
+      for (int j = 0; j < 8; ++j) {
+        if (i * 8 + j < total) {
+          v[j] = static_cast<float>(__ldg(q + row * ldq + c)) * s;
+          if (++c == cols && i * 8 + j + 1 < total) {
+            c = 0;
+            s = __ldg(scale + ++row);
+          }
+        }
+      }
+      whole.set(v);
+      const long long left = total - i * 8;
+      if (left >= 8) whole.template store<true>(out + i * 8, 8);
+      else whole.put(out + i * 8, 0, static_cast<int>(left));
     }
-    store8(out + row * cols + c, live, v);
   }
+}
+
+template <typename T>
+int dequantize(const void* q, long long ldq, const float* scale, long long rows, int cols, void* out, cudaStream_t s) {
+  const long long units = (rows * cols + 7) / 8, most = 16ll * num_sms();
+  const dim3 grid(static_cast<unsigned>((units + 255) / 256 < most ? (units + 255) / 256 : most));
+  const int8_t* p = reinterpret_cast<const int8_t*>(q);
+  const cudaError_t e = cols % 8 == 0 ? launch_chained(dequantize_kernel<T, true>, grid, dim3(256), 0, s, p, ldq, scale, rows, cols, reinterpret_cast<T*>(out))
+                                      : launch_chained(dequantize_kernel<T, false>, grid, dim3(256), 0, s, p, ldq, scale, rows, cols, reinterpret_cast<T*>(out));
+  return e == cudaSuccess ? kErrOk : kErrCuda;
 }
 
 }  // namespace int8_rows
@@ -301,8 +536,9 @@ extern "C" int lvb_int8_quantize(const void* x, int f32, long long ldx, long lon
   using namespace lvb;
   using namespace lvb::int8_rows;
   if (x == nullptr) return kErrBadArg;
-  if (f32) return quantize(Plain<float>{reinterpret_cast<const float*>(x), ldx}, rows, cols, q, ldq, scale, stream);
-  return quantize(Plain<__nv_bfloat16>{reinterpret_cast<const __nv_bfloat16*>(x), ldx}, rows, cols, q, ldq, scale, stream);
+  if (f32) return quantize(Plain<float, false>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
+  if (cols % 8 == 0 && aligned16(x, ldx * 2)) return quantize(Plain<__nv_bfloat16, true>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
+  return quantize(Plain<__nv_bfloat16, false>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
 }
 
 // The RMS norm of x (+ residual): weight [cols] (w_f32: fp32, else bf16; may be null) plus w_offset.  With a residual h = x + residual is written, in
@@ -312,13 +548,20 @@ extern "C" int lvb_int8_rms_norm(const void* x, const void* residual, void* h, i
   using namespace lvb;
   using namespace lvb::int8_rows;
   if (x == nullptr || (residual == nullptr) != (h == nullptr)) return kErrBadArg;
-  if (f32)
-    return quantize(Norm<float>{reinterpret_cast<const float*>(x), reinterpret_cast<const float*>(residual), reinterpret_cast<float*>(h), weight, ldx, ldr, ldh,
-                                w_f32, w_offset, eps},
-                    rows, cols, q, ldq, scale, stream);
-  return quantize(Norm<__nv_bfloat16>{reinterpret_cast<const __nv_bfloat16*>(x), reinterpret_cast<const __nv_bfloat16*>(residual),
-                                      reinterpret_cast<__nv_bfloat16*>(h), weight, ldx, ldr, ldh, w_f32, w_offset, eps},
-                  rows, cols, q, ldq, scale, stream);
+  auto run = [&](auto type, auto with, auto aligned) {
+    using T = decltype(type);
+    constexpr bool kResidual = decltype(with)::value;
+    Span<T> r{};
+    if (kResidual) r = Span<T>(residual, ldr, rows, cols);
+    return quantize(Norm<T, kResidual, decltype(aligned)::value>{{x, ldx, rows, cols}, r, reinterpret_cast<T*>(h), weight, ldh, w_f32, w_offset, eps, 1.f / cols}, rows,
+                    cols, q, ldq, scale, stream);
+  };
+  using yes = std::true_type;
+  using no = std::false_type;
+  if (f32) return residual != nullptr ? run(float{}, yes{}, no{}) : run(float{}, no{}, no{});
+  if (cols % 8 == 0 && aligned16(x, ldx * 2) && aligned16(residual, ldr * 2) && aligned16(h, ldh * 2) && aligned16(weight, 0))
+    return residual != nullptr ? run(__nv_bfloat16{}, yes{}, yes{}) : run(__nv_bfloat16{}, no{}, yes{});
+  return residual != nullptr ? run(__nv_bfloat16{}, yes{}, no{}) : run(__nv_bfloat16{}, no{}, no{});
 }
 
 // act(gate) * up; act: 0 silu, 1 gelu (tanh form), 2 gelu, 3 relu, 4 g sigmoid(1.702 g).
@@ -327,23 +570,28 @@ extern "C" int lvb_int8_glu(const void* gate, const void* up, int f32, long long
   using namespace lvb;
   using namespace lvb::int8_rows;
   if (gate == nullptr || up == nullptr || act < 0 || act > 4) return kErrBadArg;
-  if (f32)
-    return quantize(Glu<float>{reinterpret_cast<const float*>(gate), reinterpret_cast<const float*>(up), ldg, ldu, act}, rows, cols, q, ldq, scale, stream);
-  return quantize(Glu<__nv_bfloat16>{reinterpret_cast<const __nv_bfloat16*>(gate), reinterpret_cast<const __nv_bfloat16*>(up), ldg, ldu, act}, rows, cols, q, ldq,
-                  scale, stream);
+  const bool whole = cols % 8 == 0 && aligned16(gate, ldg * 2) && aligned16(up, ldu * 2);
+  auto run = [&](auto type, auto kind, auto aligned) {
+    using T = decltype(type);
+    return quantize(Glu<T, decltype(kind)::value, decltype(aligned)::value>{{gate, ldg, rows, cols}, {up, ldu, rows, cols}}, rows, cols, q, ldq, scale, stream);
+  };
+  auto of = [&](auto kind) {
+    return f32 ? run(float{}, kind, std::false_type{}) : whole ? run(__nv_bfloat16{}, kind, std::true_type{}) : run(__nv_bfloat16{}, kind, std::false_type{});
+  };
+  switch (act) {
+    case kSilu: return of(std::integral_constant<int, kSilu>{});
+    case kGeluTanh: return of(std::integral_constant<int, kGeluTanh>{});
+    case kGelu: return of(std::integral_constant<int, kGelu>{});
+    case kRelu: return of(std::integral_constant<int, kRelu>{});
+    default: return of(std::integral_constant<int, kQuickGelu>{});
+  }
 }
 
 // out [rows, cols] dense, bf16 or fp32 (f32).
 extern "C" int lvb_int8_dequantize(const void* q, long long ldq, const float* scale, long long rows, int cols, void* out, int f32, void* stream) {
   using namespace lvb;
   using namespace lvb::int8_rows;
-  if (q == nullptr || scale == nullptr || out == nullptr || rows <= 0 || cols <= 0 || ldq < cols) return kErrBadArg;
-  const long long units = rows * ((cols + 7) / 8), most = 16ll * num_sms();
-  const unsigned blocks = static_cast<unsigned>((units + 255) / 256 < most ? (units + 255) / 256 : most);
+  if (q == nullptr || scale == nullptr || out == nullptr || rows <= 0 || cols <= 0 || ldq < cols || (reinterpret_cast<uintptr_t>(out) & 15)) return kErrBadArg;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const cudaError_t e = f32 ? launch_chained(dequantize_kernel<float>, blocks, 256, 0, s, reinterpret_cast<const int8_t*>(q), ldq, scale, rows, cols,
-                                             reinterpret_cast<float*>(out))
-                            : launch_chained(dequantize_kernel<__nv_bfloat16>, blocks, 256, 0, s, reinterpret_cast<const int8_t*>(q), ldq, scale, rows, cols,
-                                             reinterpret_cast<__nv_bfloat16*>(out));
-  return e == cudaSuccess ? kErrOk : kErrCuda;
+  return f32 ? dequantize<float>(q, ldq, scale, rows, cols, out, s) : dequantize<__nv_bfloat16>(q, ldq, scale, rows, cols, out, s);
 }

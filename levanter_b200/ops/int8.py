@@ -48,99 +48,113 @@ class Int8Rows(NamedTuple):
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """What the rows stand for, ``values * scale`` rounded once to ``dtype`` (bf16 or fp32)."""
-        _check_rows(self, "rows")
+        v, s = self
+        _check_rows(v, s, "rows")
         if dtype not in _FLOATS:
             raise TypeError(f"rows come back as bf16 or fp32, not {dtype}")
-        v, s = self
-        if not (v.is_cuda and lib.available()):
+        if not _kernels(v):
             return (v.float() * s.unsqueeze(-1)).to(dtype)
-        v2, ld = _rows_of(v, 1)
-        out = torch.empty(v.shape, dtype=dtype, device=v.device)
-        if out.numel():
-            with _on(v):
-                rc = _fn("lvb_int8_dequantize", "plplipi")(v2.data_ptr(), ld, s.contiguous().data_ptr(), v2.shape[0], v2.shape[1], out.data_ptr(), int(dtype == torch.float32),
-                                                           lib.stream_ptr())
-            lib.check_rc(rc, "lvb_int8_dequantize")
+        out = torch.empty(*v.shape, dtype=dtype, device=v.device)
+        cols = v.size(-1)
+        v, ptr, rows, ld = _rows_of(v)
+        if rows:
+            s = _dense(s)
+            _launch("lvb_int8_dequantize", v, ptr, ld, s.data_ptr(), rows, cols, out.data_ptr(), int(dtype is torch.float32))
         return out
 
 
-def _fn(name: str, args: str):
-    """The launcher ``name``: arguments by letter (p pointer, l long long, i int, f float), then the stream."""
-    if name not in _f:
+# ------------------------------------------------------------------------------------------------ calls
+# Arguments of the launchers by letter (p pointer, l long long, i int, f float); a stream follows.
+_ARGS = {"lvb_int8_quantize": "pilliplp", "lvb_int8_rms_norm": "pppilllpiffliplp", "lvb_int8_glu": "ppilliliplp", "lvb_int8_dequantize": "plplipi",
+         "lvb_int8_gemm": "pppppiiilllippliiip"}
+
+
+def _launch(name: str, t: torch.Tensor, *args) -> None:
+    """Launches on the device of ``t`` and its current stream.  (Steps of a few rows take less time on the device than these lines on the host: what
+    follows reads the state itself and makes no objects.)"""
+    f = _f.get(name)
+    if f is None:
         kinds = {"p": lib.c_void_p, "l": lib.c_longlong, "i": lib.c_int, "f": lib.c_float}
-        _f[name] = lib.fn(name, [kinds[a] for a in args] + [lib.c_void_p])
-    return _f[name]
+        f = _f[name] = lib.fn(name, [kinds[a] for a in _ARGS[name]] + [lib.c_void_p])
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        rc = f(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        lib.check_rc(rc, name)
 
 
-class _Here:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
+def _kernels(t: torch.Tensor) -> bool:
+    if not t.is_cuda:
         return False
+    major = lib._major.get(t.get_device())  # known after the first call on a device
+    return lib.available() if major is None else major == 10 and not getattr(lib._tls, "reference", 0)
 
 
-_here = _Here()
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _on(t: torch.Tensor):
-    """The device of ``t`` as the current one, while a kernel is launched there."""
-    return _here if t.device.index == lib._current_device() else torch.cuda.device(t.device)
-
-
-def _check_rows(rows: Int8Rows, what: str) -> None:
-    v, s = rows
-    if v.dtype != torch.int8 or s.dtype != torch.float32:
+def _check_rows(v: torch.Tensor, s: torch.Tensor, what: str) -> None:
+    if v.dtype is not torch.int8 or s.dtype is not torch.float32:
         raise TypeError(f"{what}: int8 values with fp32 scales expected, got {v.dtype} and {s.dtype}")
     if v.dim() == 0 or s.shape != v.shape[:-1]:
         raise ValueError(f"{what}: values {tuple(v.shape)} need one scale per row, got {tuple(s.shape)}")
-    if s.device != v.device:
+    if s.get_device() != v.get_device():
         raise ValueError(f"{what}: values on {v.device}, scales on {s.device}")
 
 
-def _check_floats(what: str, like: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+def _check_floats(what: str, like: torch.Tensor, other: Optional[torch.Tensor] = None) -> None:
     if like.dtype not in _FLOATS:
         raise TypeError(f"{what}: rows in bf16 or fp32 expected, got {like.dtype}")
     if like.dim() == 0 or like.shape[-1] == 0:
         raise ValueError(f"{what}: rows of at least one element expected, got {tuple(like.shape)}")
-    for t in others:
-        if t is not None and (t.dtype != like.dtype or t.shape != like.shape or t.device != like.device):
-            raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} on {t.device} does not go with {tuple(like.shape)} {like.dtype} on {like.device}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (like, *others)):
-        raise RuntimeError(f"{what} has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
+    if other is not None and (other.dtype is not like.dtype or other.shape != like.shape or other.get_device() != like.get_device()):
+        raise ValueError(f"{what}: {tuple(other.shape)} {other.dtype} on {other.device} does not go with {tuple(like.shape)} {like.dtype} on {like.device}")
+    _no_gradient(what, like, other)
 
 
-def _rows_of(t: torch.Tensor, align: int) -> Tuple[torch.Tensor, int]:
-    """``t [..., cols]`` as rows and their stride in elements; copied unless the elements of a row lie side by side, rows do not overlap and start at
-    multiples of ``align`` bytes (a power of two)."""
+def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
+
+
+def _rows_of(t: torch.Tensor, align: int = 1) -> Tuple[torch.Tensor, int, int, int]:
+    """``(t, address, rows, row stride in elements)`` of ``t [..., cols]`` as rows; copied unless the elements of a row lie side by side, rows do not
+    overlap and they start at multiples of ``align`` bytes."""
     cols = t.shape[-1]
-    t2 = t.reshape(-1, cols)
-    ld = t2.stride(0) if t2.shape[0] > 1 else -(-cols // 16) * 16
-    e = t.element_size()
-    if (cols > 1 and t2.stride(1) != 1) or ld < cols or (ld * e) % align or t2.data_ptr() % align:
-        t2 = _room(t2.shape, t.dtype, t.device, align // e or 1).copy_(t2)
-        ld = t2.stride(0) if t2.shape[0] > 1 else -(-cols // 16) * 16
-    return t2, ld
+    if t.is_contiguous():
+        rows, ld, ok = t.numel() // cols, cols, True
+    else:
+        t = t if t.dim() == 2 else t.reshape(-1, cols)  # the caller keeps what a copy is read from
+        rows, ld = t.shape[0], t.stride(0)
+        ok = (cols == 1 or t.stride(1) == 1) and ld >= cols
+    if rows == 1 and ok:
+        ld = -(-cols // 16) * 16
+    ptr = t.data_ptr()
+    if not ok or (align > 1 and (ptr % align or ld * t.element_size() % align)):
+        t = _room(t.shape, t.dtype, t.device, max(1, align // t.element_size())).copy_(t)
+        return t, t.data_ptr(), rows, t.stride(-2) if rows > 1 and t.dim() > 1 else -(-cols // 16) * 16
+    return t, ptr, rows, ld
 
 
 def _room(shape, dtype: torch.dtype, device, multiple: int = 16) -> torch.Tensor:
-    """Empty rows whose stride is a multiple of that many elements."""
+    """An empty tensor whose rows start at multiples of that many elements."""
     cols = shape[-1]
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    wide = torch.empty(rows, -(-cols // multiple) * multiple, dtype=dtype, device=device)
-    return wide[:, :cols].view(shape) if wide.shape[1] == cols else wide[:, :cols].unflatten(0, shape[:-1]) if len(shape) != 2 else wide[:, :cols]
+    if cols % multiple == 0:
+        return torch.empty(*shape, dtype=dtype, device=device)  # (sizes one by one are read faster than as a tuple)
+    return torch.empty((*shape[:-1], -(-cols // multiple) * multiple), dtype=dtype, device=device)[..., :cols]
 
 
 def _empty_rows(shape, device) -> Int8Rows:
-    if len(shape) == 1:
-        return Int8Rows(_room((1, shape[0]), torch.int8, device)[0], torch.empty((), dtype=torch.float32, device=device))
-    return Int8Rows(_room(shape, torch.int8, device), torch.empty(shape[:-1], dtype=torch.float32, device=device))
-
-
-def _kernels(t: torch.Tensor) -> bool:
-    return t.is_cuda and lib.available()
+    values = _room(shape, torch.int8, device)
+    if len(shape) == 2:
+        return Int8Rows(values, torch.empty(shape[0], dtype=torch.float32, device=device))
+    return Int8Rows(values, torch.empty(shape[:-1], dtype=torch.float32, device=device))
 
 
 # ------------------------------------------------------------------------------------------------ rows
@@ -149,12 +163,12 @@ def quantize_reference(y: torch.Tensor, factor: Optional[torch.Tensor] = None) -
     y = y.float()
     top = y.abs().amax(-1, keepdim=True)
     most = top if factor is None else top * factor
-    live = most >= TINY
+    live = (most >= TINY) & (top >= 2.0 ** -120)
     q = torch.where(live & torch.isfinite(top), torch.round(y * 127.0 / top), torch.zeros_like(y))
     scale = torch.where(live, most / 127.0, torch.zeros_like(most))
     ok = torch.isfinite(top) & ~torch.isnan(most)
     scale = torch.where(ok, scale, torch.full_like(scale, float("nan")))
-    values = _empty_rows(y.shape, y.device).values
+    values = _room(y.shape, torch.int8, y.device)
     return Int8Rows(values.copy_(torch.where(ok, q, torch.zeros_like(q))), scale.squeeze(-1))
 
 
@@ -165,21 +179,15 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
 
 
 def _quantize(x: torch.Tensor) -> Int8Rows:
-    x = x.detach()
     if not _kernels(x):
-        return quantize_reference(x)
-    x2, ld = _rows_of(x, 1)
-    out = _empty_rows(x.shape, x.device)
-    if x.numel():
-        with _on(x):
-            rc = _fn("lvb_int8_quantize", "pilliplp")(x2.data_ptr(), int(x.dtype == torch.float32), ld, x2.shape[0], x2.shape[1],
-                                                                               out.values.data_ptr(), _ldq(x.shape[-1]), out.scale.data_ptr(), lib.stream_ptr())
-        lib.check_rc(rc, "lvb_int8_quantize")
+        return quantize_reference(x.detach())
+    shape = x.shape
+    cols = shape[-1]
+    x, ptr, rows, ld = _rows_of(x)
+    out = _empty_rows(shape, x.device)
+    if rows:
+        _launch("lvb_int8_quantize", x, ptr, int(x.dtype is torch.float32), ld, rows, cols, out[0].data_ptr(), -(-cols // 16) * 16, out[1].data_ptr())
     return out
-
-
-def _ldq(cols: int) -> int:
-    return -(-cols // 16) * 16
 
 
 def rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6, *, w_offset: float = 0.0,
@@ -187,49 +195,53 @@ def rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 
     """``(rows, h)``: the RMS norm of ``h = x + residual`` (rounded to the type of ``x``; without a residual ``x`` itself, and the second item is None) times
     ``weight + w_offset``, in 8 bits.  ``x [..., cols]`` and ``residual`` in bf16 or fp32, ``weight [cols]`` in bf16 or fp32 or None."""
     _check_floats("rms_norm_int8", x, residual)
-    cols = x.shape[-1]
-    if weight is not None and (weight.shape != (cols,) or weight.dtype not in _FLOATS or weight.device != x.device):
-        raise ValueError(f"rms_norm_int8: weight [{cols}] in bf16 or fp32 on {x.device} expected, got {tuple(weight.shape)} {weight.dtype} on {weight.device}")
-    x = x.detach()
+    shape = x.shape
+    cols = shape[-1]
+    if weight is not None:
+        if weight.dim() != 1 or weight.shape[0] != cols or weight.dtype not in _FLOATS or weight.get_device() != x.get_device():
+            raise ValueError(f"rms_norm_int8: weight [{cols}] in bf16 or fp32 on {x.device} expected, got {tuple(weight.shape)} {weight.dtype} on {weight.device}")
+        _no_gradient("rms_norm_int8", weight)
     if not _kernels(x):
+        x = x.detach()
         h = x if residual is None else (x.float() + residual.detach().float()).to(x.dtype)
         f = h.float()
         y = f if weight is None else f * (weight.detach().float() + w_offset)
         return quantize_reference(y, torch.rsqrt(f.square().mean(-1, keepdim=True) + eps)), None if residual is None else h
-    x2, ldx = _rows_of(x, 1)
-    h = r2 = None
-    ldr = 0
+    x, ptr, rows, ldx = _rows_of(x)
+    dev = x.device
+    h, rptr, hptr, ldr = None, 0, 0, 0
     if residual is not None:
-        r2, ldr = _rows_of(residual.detach(), 1)
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    w = None if weight is None else weight.detach().contiguous()
-    out = _empty_rows(x.shape, x.device)
-    if x.numel():
-        with _on(x):
-            rc = _fn("lvb_int8_rms_norm", "pppilllpiffliplp")(x2.data_ptr(), lib.ptr(r2), lib.ptr(h), int(x.dtype == torch.float32), ldx, ldr, cols, lib.ptr(w),
-                                                                  int(w is not None and w.dtype == torch.float32), float(w_offset), float(eps), x2.shape[0], cols,
-                                                                  out.values.data_ptr(), _ldq(cols), out.scale.data_ptr(), lib.stream_ptr())
-        lib.check_rc(rc, "lvb_int8_rms_norm")
+        residual, rptr, _, ldr = _rows_of(residual)
+        h = torch.empty(*shape, dtype=x.dtype, device=dev)
+        hptr = h.data_ptr()
+    wptr = w32 = 0
+    if weight is not None:
+        weight = _dense(weight)
+        wptr, w32 = weight.data_ptr(), int(weight.dtype is torch.float32)
+    out = _empty_rows(shape, dev)
+    if rows:
+        _launch("lvb_int8_rms_norm", x, ptr, rptr, hptr, int(x.dtype is torch.float32), ldx, ldr, cols, wptr, w32, w_offset, eps, rows, cols, out[0].data_ptr(),
+                -(-cols // 16) * 16, out[1].data_ptr())
     return out, h
 
 
 def gated_activation_int8(gate: torch.Tensor, up: torch.Tensor, act: GatedActivation) -> Int8Rows:
     """``act(gate) * up`` in 8 bits; ``gate`` and ``up [..., cols]`` in bf16 or fp32 may be the halves of a joint product's rows."""
     _check_floats("gated_activation_int8", gate, up)
-    gate, up = gate.detach(), up.detach()
-    act = ActivationFunctionEnum(act) if isinstance(act, str) and not isinstance(act, ActivationFunctionEnum) else act
+    if isinstance(act, str) and not isinstance(act, ActivationFunctionEnum):
+        act = ActivationFunctionEnum(act)
     if act not in _ACT:  # bounded gates and the like: quantised as they come
-        return _quantize(gated_activation(gate, up, act))
+        return _quantize(gated_activation(gate.detach(), up.detach(), act))
     if not _kernels(gate):
-        return quantize_reference(act.to_fn()(gate.float()) * up.float())
-    (g2, ldg), (u2, ldu) = _rows_of(gate, 1), _rows_of(up, 1)
-    cols = gate.shape[-1]
-    out = _empty_rows(gate.shape, gate.device)
-    if gate.numel():
-        with _on(gate):
-            rc = _fn("lvb_int8_glu", "ppilliliplp")(g2.data_ptr(), u2.data_ptr(), int(gate.dtype == torch.float32), ldg, ldu, _ACT[act], g2.shape[0], cols,
-                                                       out.values.data_ptr(), _ldq(cols), out.scale.data_ptr(), lib.stream_ptr())
-        lib.check_rc(rc, "lvb_int8_glu")
+        return quantize_reference(act.to_fn()(gate.detach().float()) * up.detach().float())
+    shape = gate.shape
+    cols = shape[-1]
+    gate, gptr, rows, ldg = _rows_of(gate)
+    up, uptr, _, ldu = _rows_of(up)
+    out = _empty_rows(shape, gate.device)
+    if rows:
+        _launch("lvb_int8_glu", gate, gptr, uptr, int(gate.dtype is torch.float32), ldg, ldu, _ACT[act], rows, cols, out[0].data_ptr(), -(-cols // 16) * 16,
+                out[1].data_ptr())
     return out
 
 
@@ -246,49 +258,56 @@ def int8_product(rows: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] 
     return _product(rows, weight, bias, residual, out_dtype)
 
 
-def _product(rows, weight, bias=None, residual=None, out_dtype=torch.bfloat16, form: int = 0, splits: int = 0, stages: int = 0) -> torch.Tensor:
-    _check_rows(rows, "int8_product: rows")
-    _check_rows(weight, "int8_product: weight")
-    v, w = rows.values, weight.values
-    K, dev = v.shape[-1], v.device
-    if w.dim() != 2 or w.shape[1] != K or w.device != dev:
-        raise ValueError(f"int8_product: rows {tuple(v.shape)} on {dev} and weight {tuple(w.shape)} on {w.device} do not go together")
+def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dtype=torch.bfloat16, form: int = 0, splits: int = 0, stages: int = 0) -> torch.Tensor:
+    v, sv = rows
+    w, sw = weight
+    _check_rows(v, sv, "int8_product: rows")
+    _check_rows(w, sw, "int8_product: weight")
+    lead, (N, K) = v.shape[:-1], w.shape if w.dim() == 2 else (0, 0)
+    if v.shape[-1] != K or w.get_device() != v.get_device():
+        raise ValueError(f"int8_product: rows {tuple(v.shape)} on {v.device} and weight {tuple(w.shape)} on {w.device} do not go together")
     if not 0 < K <= MAX_COLS:
         raise ValueError(f"int8_product: rows of 1 to {MAX_COLS} elements expected, got {K}")
     if out_dtype not in _FLOATS:
         raise TypeError(f"int8_product: results in bf16 or fp32, not {out_dtype}")
-    N, shape = w.shape[0], (*v.shape[:-1], w.shape[0])
-    for t, want, what in ((bias, (N,), "bias"), (residual, shape, "residual")):
-        if t is not None and (tuple(t.shape) != want or t.dtype not in _FLOATS or t.device != dev):
-            raise ValueError(f"int8_product: {what} {want} in bf16 or fp32 on {dev} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (bias, residual)):
-        raise RuntimeError("int8_product has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
+    shape = (*lead, N)
+    if bias is not None or residual is not None:
+        for t, want, what in ((bias, (N,), "bias"), (residual, shape, "residual")):
+            if t is not None and (t.shape != want or t.dtype not in _FLOATS or t.get_device() != v.get_device()):
+                raise ValueError(f"int8_product: {what} {want} in bf16 or fp32 on {v.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        _no_gradient("int8_product", bias, residual)
     if not _kernels(v):
-        y = torch.matmul(v.double(), w.double().t()).float() * rows.scale.unsqueeze(-1) * weight.scale
+        y = torch.matmul(v.double(), w.double().t()).float() * sv.unsqueeze(-1) * sw
         for t in (bias, residual):
             y = y if t is None else y + t.float()
         return y.to(out_dtype)
-    (a, lda), (b, ldb) = _rows_of(v, 16), _rows_of(w, 16)
-    M = a.shape[0]
-    out = torch.empty(shape, dtype=out_dtype, device=dev)
-    if out.numel() == 0:
+    v, a, M, lda = _rows_of(v, 16)
+    w, b, _, ldb = _rows_of(w, 16)
+    out = torch.empty(*shape, dtype=out_dtype, device=v.device)
+    if M == 0 or N == 0:
         return out
-    flags = F_OUT_F32 if out_dtype == torch.float32 else 0
-    ldr = 0
+    flags = F_OUT_F32 if out_dtype is torch.float32 else 0
+    bptr = rptr = ldr = 0
     if bias is not None:
-        flags |= F_BIAS | (F_BIAS_F32 if bias.dtype == torch.float32 else 0)
-        bias = bias.contiguous()
+        flags |= F_BIAS | (F_BIAS_F32 if bias.dtype is torch.float32 else 0)
+        bias = _dense(bias)
+        bptr = bias.data_ptr()
     if residual is not None:
-        flags |= F_RESIDUAL | (F_RESIDUAL_F32 if residual.dtype == torch.float32 else 0)
-        residual, ldr = _rows_of(residual, 1)
-        ldr = max(ldr, N)
-    sa, sb = rows.scale.contiguous(), weight.scale.contiguous()
-    with _on(v):
-        rc = _fn("lvb_int8_gemm", "pppppiiilllippliiip")(a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), out.data_ptr(), M, N, K, lda, ldb, N, flags,
-                                                                 lib.ptr(bias), lib.ptr(residual), ldr, form, splits, stages, lib.status_buffer().data_ptr(),
-                                                                 lib.stream_ptr())
-    lib.check_rc(rc, "lvb_int8_gemm")
+        flags |= F_RESIDUAL | (F_RESIDUAL_F32 if residual.dtype is torch.float32 else 0)
+        residual, rptr, _, ldr = _rows_of(residual)
+    sv, sw = _dense(sv), _dense(sw)
+    _launch("lvb_int8_gemm", v, a, b, sv.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K, lda, ldb, N, flags, bptr, rptr, ldr, form, splits, stages,
+            _status(v))
     return out
+
+
+def _status(t: torch.Tensor) -> int:
+    """Address of the status word on the device of ``t``."""
+    buf = lib._status.get(t.get_device())
+    if buf is None:
+        with torch.cuda.device(t.device):
+            buf = lib.status_buffer()
+    return buf.data_ptr()
 
 
 # ------------------------------------------------------------------------------------------------ training
