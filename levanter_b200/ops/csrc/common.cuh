@@ -580,6 +580,18 @@ inline int make_tmap_2d_u8(CUtensorMap* out, const void* ptr, uint64_t rows, uin
   return r == CUDA_SUCCESS ? kErrOk : kErrTensorMap;
 }
 
+// The limit of dynamic shared memory is set once per kernel and device.
+template <auto kKernel>
+inline int allow_shared(int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
+  if (dev < 64 && done[dev]) return kErrOk;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return kErrCuda;
+  if (dev < 64) done[dev] = true;
+  return kErrOk;
+}
+
 inline int num_sms() {
   static int n = 0;
   if (n == 0) {

@@ -19,18 +19,6 @@ constexpr int BK = 128;      // bytes of K per stage: one 128-byte swizzled line
 constexpr int kUmmaK = 32;   // of which one matrix instruction takes 32
 constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA and tensor memory, warps 2-5 epilogue
 
-// The limit of dynamic shared memory is set once per kernel and device.
-template <auto kKernel>
-inline int allow_shared(int bytes) {
-  static bool done[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return kErrCuda;
-  if (dev < 64 && done[dev]) return kErrOk;
-  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return kErrCuda;
-  if (dev < 64) done[dev] = true;
-  return kErrOk;
-}
-
 enum Flags : int { kOutF32 = 1, kBias = 2, kBiasF32 = 4, kResidual = 8, kResidualF32 = 16 };
 
 struct Params {

@@ -10,7 +10,9 @@
 // What bounds it: memory.  One pass reads the inputs and writes 1 byte per element (and h, 2 or 4).  The threads of a row keep it in registers as
 // fp32 between the reduction and the write: a warp per row up to 1024 columns, up to 1024 threads per row beyond that, and above 32768
 // columns the row is read twice.
+#include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 
@@ -86,16 +88,7 @@ template <typename T>
 struct Raw {  // eight elements as they lie in memory
   static constexpr int kWords = 2 * sizeof(T);
   uint32_t u[kWords];
-  template <bool kAligned>
   __device__ __forceinline__ void load(const T* p, int live, const char* lo, const char* hi) {
-    if constexpr (kAligned) {
-#pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const uint4 w = live > 0 ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
-        u[4 * i] = w.x; u[4 * i + 1] = w.y; u[4 * i + 2] = w.z; u[4 * i + 3] = w.w;
-      }
-      return;
-    }
     const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
     const char* base = reinterpret_cast<const char*>(p) - off;
     if (live >= 8 && off == 0) {
@@ -154,15 +147,7 @@ struct Raw {  // eight elements as they lie in memory
   }
   // All lanes of a warp, each with the eight elements behind those of the lane before it (`live` of them exist, none where it is not positive).  Where they do not
   // start on 16 bytes, a lane writes the aligned words up to its last whole ones, the first of them with the end of what the lane before it holds.
-  template <bool kAligned>
   __device__ __forceinline__ void store(T* p, int live) const {
-    if constexpr (kAligned) {
-      if (live > 0) {
-#pragma unroll
-        for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
-      }
-      return;
-    }
     const int lane = threadIdx.x & 31;
     const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
     if (off == 0) {
@@ -193,20 +178,18 @@ struct Raw {  // eight elements as they lie in memory
 };
 
 // ---- where a row comes from: load() starts the reads of eight of its elements, get() gives them and adds what the row's factor needs to `ss`.  All
-// lanes of a warp call get(); `live` of the elements exist (none where it is not positive), the others are zero.  kAligned: rows, and the groups of eight
-// in them, start on 16 bytes and are whole.
-template <typename T, bool kAligned>
+// lanes of a warp call get(); `live` of the elements exist (none where it is not positive), the others are zero.
+template <typename T>
 struct Plain {
   Span<T> x;
-  using Type = T;
   using In = Raw<T>;
   static constexpr bool kSum = false;
-  __device__ __forceinline__ void load(In& in, long long row, int c, int live) const { in.template load<kAligned>(x.p + row * x.ld + c, live, x.lo, x.hi); }
+  __device__ __forceinline__ void load(In& in, long long row, int c, int live) const { in.load(x.p + row * x.ld + c, live, x.lo, x.hi); }
   __device__ __forceinline__ void get(const In& in, long long, int, int, float (&y)[8], F32x2&) const { in.get(y); }
   __device__ __forceinline__ float factor(float) const { return 1.f; }
 };
 
-template <typename T, bool kResidual, bool kAligned>
+template <typename T, bool kResidual>
 struct Norm {
   Span<T> x, r;
   T* h;  // written where there is a residual
@@ -217,16 +200,15 @@ struct Norm {
   struct In {
     Raw<T> a, b;  // (without a residual the second is never loaded and takes no register)
   };
-  using Type = T;
   static constexpr bool kSum = true;
   __device__ __forceinline__ void load(In& in, long long row, int c, int live) const {
-    in.a.template load<kAligned>(x.p + row * x.ld + c, live, x.lo, x.hi);
-    if constexpr (kResidual) in.b.template load<kAligned>(r.p + row * r.ld + c, live, r.lo, r.hi);
+    in.a.load(x.p + row * x.ld + c, live, x.lo, x.hi);
+    if constexpr (kResidual) in.b.load(r.p + row * r.ld + c, live, r.lo, r.hi);
   }
   template <typename W>
   __device__ __forceinline__ void weigh(const W* p, int live, float (&y)[8]) const {
     Raw<W> raw;
-    raw.template load<kAligned>(p, live, nullptr, nullptr);
+    raw.load(p, live, nullptr, nullptr);
     float f[8];
     raw.get(f);
     if (w_offset != 0.f) {
@@ -246,7 +228,7 @@ struct Norm {
       Raw<T> sum;
       sum.set(y);
       sum.get(y);  // the sum in the rows' type is what goes on, here too
-      sum.template store<kAligned>(h + row * ldh + c, live);
+      sum.store(h + row * ldh + c, live);
     }
 #pragma unroll
     for (int j = 0; j < 8; j += 2) ss = f2_fma(f2(y[j], y[j + 1]), f2(y[j], y[j + 1]), ss);
@@ -258,17 +240,16 @@ struct Norm {
   __device__ __forceinline__ float factor(float ss) const { return rsqrtf(ss * per_col + eps); }
 };
 
-template <typename T, int kAct, bool kAligned>
+template <typename T, int kAct>
 struct Glu {
   Span<T> g, u;
   struct In {
     Raw<T> a, b;
   };
-  using Type = T;
   static constexpr bool kSum = false;
   __device__ __forceinline__ void load(In& in, long long row, int c, int live) const {
-    in.a.template load<kAligned>(g.p + row * g.ld + c, live, g.lo, g.hi);
-    in.b.template load<kAligned>(u.p + row * u.ld + c, live, u.lo, u.hi);
+    in.a.load(g.p + row * g.ld + c, live, g.lo, g.hi);
+    in.b.load(u.p + row * u.ld + c, live, u.lo, u.hi);
   }
   __device__ __forceinline__ void get(const In& in, long long, int, int, float (&y)[8], F32x2&) const {
     float b[8];
@@ -276,6 +257,99 @@ struct Glu {
     in.b.get(b);
 #pragma unroll
     for (int j = 0; j < 8; j += 2) f2_split(f2_mul(activation2<kAct>(f2(y[j], y[j + 1])), f2(b[j], b[j + 1])), y[j], y[j + 1]);
+  }
+  __device__ __forceinline__ float factor(float) const { return 1.f; }
+};
+
+// ---- the same for rows of whole groups of 16 bf16 elements that start on 32 bytes: load() and get() of the group at element `at`, column `c`.  The rows of all
+// inputs (and of h) have one stride.
+struct Raw16 {
+  uint32_t u[8];
+  __device__ __forceinline__ void load(const void* p) {
+    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+                 : "l"(p));
+  }
+  __device__ __forceinline__ void store(void* p) const {
+    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]),
+                 "r"(u[7]), "l"(p)
+                 : "memory");
+  }
+  __device__ __forceinline__ F32x2 pair(int j) const { return f2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xFFFF0000u)); }
+};
+struct Plain16 {
+  const __nv_bfloat16* x;
+  struct In {
+    Raw16 x;
+  };
+  static constexpr bool kSum = false;
+  __device__ __forceinline__ void load(In& in, long long at) const { in.x.load(x + at); }
+  __device__ __forceinline__ void get(const In& in, long long, int, float (&y)[16], F32x2&) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f2_split(in.x.pair(j), y[2 * j], y[2 * j + 1]);
+  }
+  __device__ __forceinline__ float factor(float) const { return 1.f; }
+};
+template <bool kResidual, bool kW32>
+struct Norm16 {
+  const __nv_bfloat16 *x, *r;
+  __nv_bfloat16* h;
+  const void* w;
+  float w_offset, eps, per_col;
+  struct In {
+    Raw16 x, r;
+  };
+  static constexpr bool kSum = true;
+  __device__ __forceinline__ void load(In& in, long long at) const {
+    in.x.load(x + at);
+    if constexpr (kResidual) in.r.load(r + at);
+  }
+  __device__ __forceinline__ void get(const In& in, long long at, int c, float (&y)[16], F32x2& ss) const {
+    Raw16 sum = in.x;
+    if constexpr (kResidual) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // the sum in the rows' type is what goes on, here too
+        float a, b;
+        f2_split(f2_add(in.x.pair(j), in.r.pair(j)), a, b);
+        sum.u[j] = pack_bf16x2(a, b);
+      }
+      sum.store(h + at);
+    }
+    Raw16 w0, w1;
+    if (w != nullptr) {  // from the L1, row after row
+      w0.load(kW32 ? static_cast<const void*>(static_cast<const float*>(w) + c) : static_cast<const void*>(static_cast<const __nv_bfloat16*>(w) + c));
+      if constexpr (kW32) w1.load(static_cast<const float*>(w) + c + 8);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      F32x2 v = sum.pair(j);
+      ss = f2_fma(v, v, ss);
+      if (w != nullptr) {
+        F32x2 f;
+        if constexpr (kW32) f = f2(__uint_as_float(j < 4 ? w0.u[2 * j % 8] : w1.u[2 * j % 8]), __uint_as_float(j < 4 ? w0.u[(2 * j + 1) % 8] : w1.u[(2 * j + 1) % 8]));
+        else f = w0.pair(j);
+        if (w_offset != 0.f) f = f2_add(f, f2(w_offset, w_offset));
+        v = f2_mul(v, f);
+      }
+      f2_split(v, y[2 * j], y[2 * j + 1]);
+    }
+  }
+  __device__ __forceinline__ float factor(float ss) const { return rsqrtf(ss * per_col + eps); }
+};
+template <int kAct>
+struct Glu16 {
+  const __nv_bfloat16 *g, *u;
+  struct In {
+    Raw16 g, u;
+  };
+  static constexpr bool kSum = false;
+  __device__ __forceinline__ void load(In& in, long long at) const {
+    in.g.load(g + at);
+    in.u.load(u + at);
+  }
+  __device__ __forceinline__ void get(const In& in, long long, int, float (&y)[16], F32x2&) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f2_split(f2_mul(activation2<kAct>(in.g.pair(j)), in.u.pair(j)), y[2 * j], y[2 * j + 1]);
   }
   __device__ __forceinline__ float factor(float) const { return 1.f; }
 };
@@ -288,7 +362,7 @@ __device__ __forceinline__ float largest_of(float a, float b, float c) {
 }
 
 // Eight whole numbers as bytes.  Adding 1.5 * 2^23 rounds to the nearest whole number, ties to even, and leaves it in the low bits.
-__device__ __forceinline__ uint2 whole8(const float (&y)[8], float top, float inv) {
+__device__ __forceinline__ uint2 whole8(const float* y, float top, float inv) {
   constexpr float kMagic = 12582912.f;
   uint32_t b[8];
   float far = 0.f;  // how far the furthest lies from its whole number
@@ -296,7 +370,7 @@ __device__ __forceinline__ uint2 whole8(const float (&y)[8], float top, float in
   for (int j = 0; j < 8; j += 2) {
     const F32x2 v = f2(y[j], y[j + 1]), k = f2(inv, inv);
     const F32x2 m = f2_fma(v, k, f2(kMagic, kMagic));
-    const F32x2 q = f2_add(f2(kMagic, kMagic), f2_mul(m, f2(-1.f, -1.f)));
+    const F32x2 q = f2_fma(m, f2(-1.f, -1.f), f2(kMagic, kMagic));
     float d0, d1, m0, m1;
     f2_split(f2_fma(v, k, q), d0, d1);
     f2_split(m, m0, m1);
@@ -319,27 +393,74 @@ __device__ __forceinline__ uint2 whole8(const float (&y)[8], float top, float in
 }
 
 constexpr int kRowWarps = 4;  // of a block whose warps have a row each
-constexpr int kBlockRegs = 65536;
 
 constexpr int kHeldGroups = 2;   // groups of eight per thread of a block that has a row
 constexpr int kMostThreads = 1024;
 
-// kWarp: a row per warp, else a row per block.  kChunks: groups of eight elements per thread, held in registers; 0: any number of them, each made twice.
-// A block goes through rows far apart and starts the reads of its next row before it reduces and writes the one it has.  q has room for whole groups of
-// eight up to the end of its row stride.
+// What the threads of a row agree on: its largest magnitude (as bits, which order infinities and NaN last) and its factor.
+struct RowScale {
+  float most, inv, scale;
+  bool live;
+  __device__ __forceinline__ RowScale(uint32_t top, float f) {
+    most = __uint_as_float(top);
+    const bool finite = top < 0x7F800000u && f == f;
+    live = finite && most * f >= kTiny && most >= kLeast;
+    // (the quick quotient is good for divisors up to 2^126; 1e30 keeps the quotient a normal number, too)
+    inv = !live ? 0.f : most < 1e30f ? __fdividef(127.f, most) : 127.f / most;
+    scale = most * f;
+    if (!live) scale = finite ? 0.f : __uint_as_float(0x7FC00000u);
+  }
+  __device__ __forceinline__ void put(int8_t* out, const float (&v)[8]) const {
+    *reinterpret_cast<uint2*>(out) = live ? whole8(v, most, inv) : make_uint2(0, 0);
+  }
+};
+__device__ __forceinline__ void note(float& largest, const float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) largest = largest_of(largest, v[j], v[j + 1]);
+}
+// The maximum and sum over a block, through `tops` and `sums` [32], in which the numbers of warps that do not exist are 0.
+template <bool kSum>
+__device__ __forceinline__ void reduce_block(uint32_t& top, float& ss, uint32_t* tops, float* sums) {
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    tops[warp] = top;
+    if constexpr (kSum) sums[warp] = ss;
+  }
+  __syncthreads();
+  top = 0;
+  ss = 0.f;
+  for (int i = 0; i < warps; i += 4) {
+    const uint4 v = reinterpret_cast<const uint4*>(tops)[i / 4];
+    top = max(max(top, max(v.x, v.y)), max(v.z, v.w));
+    if constexpr (kSum) {
+      const float4 a = reinterpret_cast<const float4*>(sums)[i / 4];
+      ss += (a.x + a.y) + (a.z + a.w);
+    }
+  }
+}
+template <bool kSum>
+__device__ __forceinline__ float warp_ss(F32x2 ss2) {
+  if constexpr (!kSum) return 0.f;
+  float a, b;
+  f2_split(ss2, a, b);
+  return warp_sum(a + b);
+}
+
+// Few rows, and rows that lie anywhere.  kWarp: a row per warp, else a row per block.  kChunks: groups of eight elements per thread, held in registers; 0:
+// any number of them, each made twice.  A block goes through rows far apart and starts the reads of its next row before it reduces and writes the one it
+// has.  q has room for whole groups of eight up to the end of its row stride.
 template <class Src, bool kWarp, int kChunks>
-__global__ void __launch_bounds__(kWarp ? 32 * kRowWarps : kMostThreads) quantize_kernel(Src src, long long rows, int cols, int8_t* __restrict__ q,
-                                                                                               long long ldq, float* __restrict__ scale) {
-  __shared__ uint32_t s_top[2][32];
-  __shared__ float s_ss[2][32];
+__global__ void __launch_bounds__(kWarp ? 32 * kRowWarps : kMostThreads) quantize_kernel(Src src, long long rows, int cols, int8_t* __restrict__ q, long long ldq,
+                                                                                        float* __restrict__ scale) {
+  __shared__ __align__(16) uint32_t s_top[2][32];
+  __shared__ __align__(16) float s_ss[2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = kWarp ? lane : static_cast<int>(threadIdx.x);
   const int group = kWarp ? 32 : static_cast<int>(blockDim.x);
-  const int warps = group >> 5;
   const long long step = kWarp ? static_cast<long long>(gridDim.x) * kRowWarps : gridDim.x;
   long long row = kWarp ? static_cast<long long>(blockIdx.x) * kRowWarps + warp : blockIdx.x;
   if constexpr (!kWarp) {
-    if (threadIdx.x < 32) {  // the partial results of warps that do not exist
+    if (threadIdx.x < 32) {
       s_top[0][lane] = s_top[1][lane] = 0;
       s_ss[0][lane] = s_ss[1][lane] = 0.f;
     }
@@ -361,139 +482,184 @@ __global__ void __launch_bounds__(kWarp ? 32 * kRowWarps : kMostThreads) quantiz
     float y[kHeld][8];
     F32x2 ss2 = f2(0.f, 0.f);
     float largest = 0.f;
-    auto note = [&](const float (&v)[8]) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) largest = largest_of(largest, v[j], v[j + 1]);
-    };
     if constexpr (kChunks > 0) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int c = (t + i * group) * 8;
         src.get(in[i], row, c, cols - c, y[i], ss2);
-        note(y[i]);
+        note(largest, y[i]);
       }
       if (row + step < rows) load(row + step);
     } else {
       for (int c = t * 8; c < limit; c += group * 8) {
         src.load(in[0], row, c, cols - c);
         src.get(in[0], row, c, cols - c, y[0], ss2);
-        note(y[0]);
+        note(largest, y[0]);
       }
     }
-    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));  // magnitudes order as their bits, infinities and NaN last
-    float ss = 0.f;
-    if constexpr (Src::kSum) {
-      float a, b;
-      f2_split(ss2, a, b);
-      ss = warp_sum(a + b);
-    }
-    if constexpr (!kWarp) {
-      if (lane == 0) {
-        s_top[odd][warp] = top;
-        s_ss[odd][warp] = ss;
-      }
-      __syncthreads();  // (one per row: what this row reads is written again two rows on, behind the next row's)
-      const uint4* tops = reinterpret_cast<const uint4*>(s_top[odd]);
-      const float4* sums = reinterpret_cast<const float4*>(s_ss[odd]);
-      top = 0;
-      ss = 0.f;
-      for (int i = 0; i < warps; i += 4) {
-        const uint4 v = tops[i / 4];
-        top = max(max(top, max(v.x, v.y)), max(v.z, v.w));
-        if constexpr (Src::kSum) {
-          const float4 a = sums[i / 4];
-          ss += (a.x + a.y) + (a.z + a.w);
-        }
-      }
-    }
-    const float f = src.factor(ss);
-    const float most = __uint_as_float(top);
-    const bool finite = top < 0x7F800000u && f == f;
-    const bool live = finite && most * f >= kTiny && most >= kLeast;
-    // (the quick quotient is good for divisors up to 2^126; 1e30 keeps the quotient a normal number, too)
-    const float inv = !live ? 0.f : most < 1e30f ? __fdividef(127.f, most) : 127.f / most;
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+    float ss = warp_ss<Src::kSum>(ss2);
+    // (one barrier per row: what this row reads is written again two rows on, behind the next row's)
+    if constexpr (!kWarp) reduce_block<Src::kSum>(top, ss, s_top[odd], s_ss[odd]);
+    const RowScale r(top, src.factor(ss));
     int8_t* out = q + row * ldq;
-    auto put = [&](int c, const float (&v)[8]) { *reinterpret_cast<uint2*>(out + c) = live ? whole8(v, most, inv) : make_uint2(0, 0); };
     if constexpr (kChunks > 0) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int c = (t + i * group) * 8;
-        if (c < cols) put(c, y[i]);
+        if (c < cols) r.put(out + c, y[i]);
       }
     } else {
       for (int c = t * 8; c < limit; c += group * 8) {
         F32x2 again = f2(0.f, 0.f);
         src.load(in[0], row, c, cols - c);
         src.get(in[0], row, c, cols - c, y[0], again);
-        if (c < cols) put(c, y[0]);
+        if (c < cols) r.put(out + c, y[0]);
       }
     }
-    if (t == 0) scale[row] = live ? most * f / 127.f : finite ? 0.f : __uint_as_float(0x7FC00000u);
+    if (t == 0) scale[row] = r.scale / 127.f;
   }
+}
+
+// Aligned rows of whole groups of 16 elements, a thread has one: 32 bytes of each input in one load.
+template <class Src>
+__global__ void __launch_bounds__(kMostThreads) rows16_kernel(Src src, long long ld, int rows, int cols, int8_t* __restrict__ q, long long ldq,
+                                                              float* __restrict__ scale) {
+  __shared__ uint32_t s_top[2][32];
+  __shared__ float s_ss[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = threadIdx.x * 16;
+  const bool mine = c < cols;
+  if (threadIdx.x < 32) {  // the partial results of warps that do not exist
+    s_top[0][lane] = s_top[1][lane] = 0;
+    s_ss[0][lane] = s_ss[1][lane] = 0.f;
+  }
+  __syncthreads();
+  chain_wait();
+  const int step = gridDim.x;
+  int row = blockIdx.x;
+  long long at = row * ld + c;
+  typename Src::In in;
+  if (mine) src.load(in, at);
+  for (int odd = 0; row < rows; row += step, odd ^= 1) {
+    float y[16] = {};
+    F32x2 ss2 = f2(0.f, 0.f);
+    float largest = 0.f;
+    if (mine) {
+      src.get(in, at, c, y, ss2);
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) largest = largest_of(largest, y[j], y[j + 1]);
+      at += step * ld;
+      if (row + step < rows) src.load(in, at);
+    }
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+    float ss = warp_ss<Src::kSum>(ss2);
+    if (lane == 0) {
+      s_top[odd][warp] = top;
+      if constexpr (Src::kSum) s_ss[odd][warp] = ss;
+    }
+    __syncthreads();  // (one per row: what this row reads is written again two rows on, behind the next row's)
+    top = __reduce_max_sync(0xffffffffu, s_top[odd][lane]);
+    if constexpr (Src::kSum) ss = warp_sum(s_ss[odd][lane]);
+    const RowScale r(top, src.factor(ss));
+    if (mine) {
+      uint2 a = make_uint2(0, 0), b = a;
+      if (r.live) {
+        a = whole8(y, r.most, r.inv);
+        b = whole8(y + 8, r.most, r.inv);
+      }
+      *reinterpret_cast<uint4*>(q + row * ldq + c) = make_uint4(a.x, a.y, b.x, b.y);
+    }
+    if (threadIdx.x == 0) scale[row] = r.scale / 127.f;
+  }
+}
+
+template <auto kKernel>
+int resident_blocks(int threads, int shared) {  // per SM
+  static int regs = 0;
+  if (regs == 0) {
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kKernel) != cudaSuccess) return 1;
+    regs = (attr.numRegs + 7) / 8 * 8;
+  }
+  int n = 65536 / (regs * threads);
+  if (n > 2048 / threads) n = 2048 / threads;
+  if (n > 228 * 1024 / (shared + 2048)) n = 228 * 1024 / (shared + 2048);
+  return n < 1 ? 1 : n > 32 ? 32 : n;
 }
 
 template <class Src, bool kWarp, int kChunks>
 int launch(const Src& src, long long rows, int cols, int threads, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
   const long long blocks = kWarp ? (rows + kRowWarps - 1) / kRowWarps : rows;
-  static int resident = 0;  // blocks per SM, of 32 threads
-  if (resident == 0) {
-    cudaFuncAttributes attr;
-    if (cudaFuncGetAttributes(&attr, quantize_kernel<Src, kWarp, kChunks>) != cudaSuccess) return kErrCuda;
-    resident = kBlockRegs / (32 * ((attr.numRegs + 7) / 8 * 8));
-  }
-  const int per_sm = resident / (threads / 32) < 2048 / threads ? resident / (threads / 32) : 2048 / threads;
-  const long long most = static_cast<long long>(num_sms()) * (per_sm < 1 ? 1 : per_sm);
+  const long long most = static_cast<long long>(num_sms()) * resident_blocks<quantize_kernel<Src, kWarp, kChunks>>(threads, 0);
   return launch_chained(quantize_kernel<Src, kWarp, kChunks>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(threads), 0, s, src, rows, cols, q,
                         ldq, scale) == cudaSuccess
              ? kErrOk
              : kErrCuda;
 }
 
-inline bool aligned16(const void* p, long long bytes) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (bytes & 15) == 0; }
+template <class Src>
+int quantize16(const Src& src, long long ld, long long rows, int cols, void* q, long long ldq, float* scale, void* stream) {
+  if (rows <= 0 || q == nullptr || scale == nullptr || (ldq & 15) || ldq < cols || (reinterpret_cast<uintptr_t>(q) & 15)) return kErrBadArg;
+  const int threads = (cols / 16 + 31) / 32 * 32;
+  const long long most = static_cast<long long>(num_sms()) * resident_blocks<rows16_kernel<Src>>(threads, 0);
+  return launch_chained(rows16_kernel<Src>, dim3(static_cast<unsigned>(rows < most ? rows : most)), dim3(threads), 0, reinterpret_cast<cudaStream_t>(stream), src, ld,
+                        static_cast<int>(rows), cols, reinterpret_cast<int8_t*>(q), ldq, scale) == cudaSuccess
+             ? kErrOk
+             : kErrCuda;
+}
+
+// Whether rows are of whole groups of 16 elements, few enough for a block and more than a warp takes, start on 32 bytes and have one stride.
+inline bool rows16(long long rows, int cols, long long ld, std::initializer_list<std::pair<const void*, long long>> inputs) {
+  if (cols % 16 != 0 || cols > 16 * kMostThreads || cols <= 512 || rows > 0x3FFFFFFF || (ld & 15)) return false;
+  for (const auto& i : inputs)
+    if (i.first != nullptr && ((reinterpret_cast<uintptr_t>(i.first) & 31) || i.second != ld)) return false;
+  return true;
+}
 
 template <class Src>
 int quantize(const Src& src, long long rows, int cols, void* q, long long ldq, float* scale, void* stream) {
   if (rows <= 0 || cols <= 0 || q == nullptr || scale == nullptr || (ldq & 7) || ldq < cols || (reinterpret_cast<uintptr_t>(q) & 7)) return kErrBadArg;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int8_t* o = reinterpret_cast<int8_t*>(q);
-  constexpr int kChunks = kHeldGroups, kWarpBlock = 32 * kRowWarps;
-  if (cols <= 512) return launch<Src, true, 2>(src, rows, cols, kWarpBlock, o, ldq, scale, s);
-  if (cols <= kMostThreads * 8 * kChunks) {
-    const int units = (cols + 7) / 8, threads = (units + kChunks - 1) / kChunks;
-    return launch<Src, false, kChunks>(src, rows, cols, (threads + 31) / 32 * 32, o, ldq, scale, s);
-  }
-  return launch<Src, false, 0>(src, rows, cols, kMostThreads, o, ldq, scale, s);
+  if (cols <= 512) return launch<Src, true, 2>(src, rows, cols, 32 * kRowWarps, o, ldq, scale, s);
+  if (cols > kMostThreads * 8 * kHeldGroups) return launch<Src, false, 0>(src, rows, cols, kMostThreads, o, ldq, scale, s);
+  const int threads = ((cols + 7) / 8 + 32 * kHeldGroups - 1) / (32 * kHeldGroups) * 32;
+  return launch<Src, false, kHeldGroups>(src, rows, cols, threads, o, ldq, scale, s);
 }
 
-// out = q * scale, rounded once, for dense rows `out`.  kWhole: rows are whole groups of eight; else a group lies across the ends of rows.
-template <typename T, bool kWhole>
+// out = q * scale, rounded once, for dense rows `out`.  kGroup elements per thread: 16 of aligned rows of whole groups of 16, else 8, and those may lie
+// across the ends of rows.
+template <typename T, int kGroup>
 __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restrict__ q, long long ldq, const float* __restrict__ scale, long long rows,
                                                          int cols, T* __restrict__ out) {
   chain_wait();
   const long long total = rows * cols;
-  const unsigned units = cols / 8;
+  const unsigned units = cols / kGroup;
   const bool narrow = total < (1ll << 32);  // a division of 32 bits is three times as fast
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i * 8 < total; i += gridDim.x * 256ll) {
-    float v[8];
-    Raw<T> whole;  // (groups of eight of a dense `out` start on 16 bytes)
-    if constexpr (kWhole) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i * kGroup < total; i += gridDim.x * 256ll) {
+    if constexpr (kGroup == 16) {
       const long long row = narrow ? static_cast<unsigned>(i) / units : i / units;
-      const int8_t* p = q + row * ldq + (i - row * units) * 8;
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + row * ldq + (i - row * units) * 16));
       const float s = __ldg(scale + row);
-      if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      Raw16 o[sizeof(T) / 2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] = static_cast<float>(static_cast<int8_t>(w.x >> (8 * j))) * s;
-          v[4 + j] = static_cast<float>(static_cast<int8_t>(w.y >> (8 * j))) * s;
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t p = u[j / 2] >> (16 * (j & 1));
+        const float a = static_cast<float>(static_cast<int8_t>(p)) * s, b = static_cast<float>(static_cast<int8_t>(p >> 8)) * s;
+        if constexpr (sizeof(T) == 2) {
+          o[0].u[j] = pack_bf16x2(a, b);
+        } else {
+          o[j / 4 % (sizeof(T) / 2)].u[2 * j % 8] = __float_as_uint(a);
+          o[j / 4 % (sizeof(T) / 2)].u[(2 * j + 1) % 8] = __float_as_uint(b);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(__ldg(p + j)) * s;
       }
-      whole.set(v);
-      whole.template store<true>(out + i * 8, 8);
+#pragma unroll
+      for (int k = 0; k < sizeof(T) / 2; ++k) o[k].store(out + i * 16 + k * 8);
     } else {
+      float v[8];
+      Raw<T> group;  // (groups of eight of a dense `out` start on 16 bytes)
       long long row = narrow ? static_cast<unsigned>(i * 8) / static_cast<unsigned>(cols) : i * 8 / cols;
       int c = static_cast<int>(i * 8 - row * cols);
       float s = __ldg(scale + row);
@@ -507,21 +673,22 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restric
           }
         }
       }
-      whole.set(v);
+      group.set(v);
       const long long left = total - i * 8;
-      if (left >= 8) whole.template store<true>(out + i * 8, 8);
-      else whole.put(out + i * 8, 0, static_cast<int>(left));
+      if (left >= 8) group.store(out + i * 8, 8);
+      else group.put(out + i * 8, 0, static_cast<int>(left));
     }
   }
 }
 
 template <typename T>
 int dequantize(const void* q, long long ldq, const float* scale, long long rows, int cols, void* out, cudaStream_t s) {
-  const long long units = (rows * cols + 7) / 8, most = 16ll * num_sms();
+  const bool whole = cols % 16 == 0 && (ldq & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0;
+  const long long units = whole ? rows * (cols / 16) : (rows * cols + 7) / 8, most = 8ll * num_sms();
   const dim3 grid(static_cast<unsigned>((units + 255) / 256 < most ? (units + 255) / 256 : most));
   const int8_t* p = reinterpret_cast<const int8_t*>(q);
-  const cudaError_t e = cols % 8 == 0 ? launch_chained(dequantize_kernel<T, true>, grid, dim3(256), 0, s, p, ldq, scale, rows, cols, reinterpret_cast<T*>(out))
-                                      : launch_chained(dequantize_kernel<T, false>, grid, dim3(256), 0, s, p, ldq, scale, rows, cols, reinterpret_cast<T*>(out));
+  const cudaError_t e = whole ? launch_chained(dequantize_kernel<T, 16>, grid, dim3(256), 0, s, p, ldq, scale, rows, cols, reinterpret_cast<T*>(out))
+                              : launch_chained(dequantize_kernel<T, 8>, grid, dim3(256), 0, s, p, ldq, scale, rows, cols, reinterpret_cast<T*>(out));
   return e == cudaSuccess ? kErrOk : kErrCuda;
 }
 
@@ -536,9 +703,9 @@ extern "C" int lvb_int8_quantize(const void* x, int f32, long long ldx, long lon
   using namespace lvb;
   using namespace lvb::int8_rows;
   if (x == nullptr) return kErrBadArg;
-  if (f32) return quantize(Plain<float, false>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
-  if (cols % 8 == 0 && aligned16(x, ldx * 2)) return quantize(Plain<__nv_bfloat16, true>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
-  return quantize(Plain<__nv_bfloat16, false>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
+  if (f32) return quantize(Plain<float>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
+  if (rows16(rows, cols, ldx, {{x, ldx}})) return quantize16(Plain16{static_cast<const __nv_bfloat16*>(x)}, ldx, rows, cols, q, ldq, scale, stream);
+  return quantize(Plain<__nv_bfloat16>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
 }
 
 // The RMS norm of x (+ residual): weight [cols] (w_f32: fp32, else bf16; may be null) plus w_offset.  With a residual h = x + residual is written, in
@@ -547,21 +714,26 @@ extern "C" int lvb_int8_rms_norm(const void* x, const void* residual, void* h, i
                                  int w_f32, float w_offset, float eps, long long rows, int cols, void* q, long long ldq, float* scale, void* stream) {
   using namespace lvb;
   using namespace lvb::int8_rows;
-  if (x == nullptr || (residual == nullptr) != (h == nullptr)) return kErrBadArg;
-  auto run = [&](auto type, auto with, auto aligned) {
-    using T = decltype(type);
-    constexpr bool kResidual = decltype(with)::value;
-    Span<T> r{};
-    if (kResidual) r = Span<T>(residual, ldr, rows, cols);
-    return quantize(Norm<T, kResidual, decltype(aligned)::value>{{x, ldx, rows, cols}, r, reinterpret_cast<T*>(h), weight, ldh, w_f32, w_offset, eps, 1.f / cols}, rows,
-                    cols, q, ldq, scale, stream);
+  using bf16 = __nv_bfloat16;
+  if (x == nullptr || cols <= 0 || (residual == nullptr) != (h == nullptr)) return kErrBadArg;
+  const float per_col = 1.f / static_cast<float>(cols);
+  auto run = [&](auto with, auto wide) {
+    constexpr bool kResidual = decltype(with)::value, kWide = decltype(wide)::value;
+    if (!f32 && rows16(rows, cols, ldx, {{x, ldx}, {residual, ldr}, {h, ldh}, {weight, ldx}}))
+      return quantize16(Norm16<kResidual, kWide>{static_cast<const bf16*>(x), static_cast<const bf16*>(residual), static_cast<bf16*>(h), weight, w_offset, eps, per_col},
+                        ldx, rows, cols, q, ldq, scale, stream);
+    auto general = [&](auto type) {
+      using T = decltype(type);
+      Span<T> r{};
+      if (kResidual) r = Span<T>(residual, ldr, rows, cols);
+      return quantize(Norm<T, kResidual>{{x, ldx, rows, cols}, r, static_cast<T*>(h), weight, ldh, w_f32, w_offset, eps, per_col}, rows, cols, q, ldq, scale, stream);
+    };
+    return f32 ? general(float{}) : general(bf16{});
   };
   using yes = std::true_type;
   using no = std::false_type;
-  if (f32) return residual != nullptr ? run(float{}, yes{}, no{}) : run(float{}, no{}, no{});
-  if (cols % 8 == 0 && aligned16(x, ldx * 2) && aligned16(residual, ldr * 2) && aligned16(h, ldh * 2) && aligned16(weight, 0))
-    return residual != nullptr ? run(__nv_bfloat16{}, yes{}, yes{}) : run(__nv_bfloat16{}, no{}, yes{});
-  return residual != nullptr ? run(__nv_bfloat16{}, yes{}, no{}) : run(__nv_bfloat16{}, no{}, no{});
+  if (residual != nullptr) return w_f32 ? run(yes{}, yes{}) : run(yes{}, no{});
+  return w_f32 ? run(no{}, yes{}) : run(no{}, no{});
 }
 
 // act(gate) * up; act: 0 silu, 1 gelu (tanh form), 2 gelu, 3 relu, 4 g sigmoid(1.702 g).
@@ -569,21 +741,21 @@ extern "C" int lvb_int8_glu(const void* gate, const void* up, int f32, long long
                             long long ldq, float* scale, void* stream) {
   using namespace lvb;
   using namespace lvb::int8_rows;
+  using bf16 = __nv_bfloat16;
   if (gate == nullptr || up == nullptr || act < 0 || act > 4) return kErrBadArg;
-  const bool whole = cols % 8 == 0 && aligned16(gate, ldg * 2) && aligned16(up, ldu * 2);
-  auto run = [&](auto type, auto kind, auto aligned) {
-    using T = decltype(type);
-    return quantize(Glu<T, decltype(kind)::value, decltype(aligned)::value>{{gate, ldg, rows, cols}, {up, ldu, rows, cols}}, rows, cols, q, ldq, scale, stream);
-  };
-  auto of = [&](auto kind) {
-    return f32 ? run(float{}, kind, std::false_type{}) : whole ? run(__nv_bfloat16{}, kind, std::true_type{}) : run(__nv_bfloat16{}, kind, std::false_type{});
+  auto run = [&](auto kind) {
+    constexpr int kAct = decltype(kind)::value;
+    if (f32) return quantize(Glu<float, kAct>{{gate, ldg, rows, cols}, {up, ldu, rows, cols}}, rows, cols, q, ldq, scale, stream);
+    if (rows16(rows, cols, ldg, {{gate, ldg}, {up, ldu}}))
+      return quantize16(Glu16<kAct>{static_cast<const bf16*>(gate), static_cast<const bf16*>(up)}, ldg, rows, cols, q, ldq, scale, stream);
+    return quantize(Glu<bf16, kAct>{{gate, ldg, rows, cols}, {up, ldu, rows, cols}}, rows, cols, q, ldq, scale, stream);
   };
   switch (act) {
-    case kSilu: return of(std::integral_constant<int, kSilu>{});
-    case kGeluTanh: return of(std::integral_constant<int, kGeluTanh>{});
-    case kGelu: return of(std::integral_constant<int, kGelu>{});
-    case kRelu: return of(std::integral_constant<int, kRelu>{});
-    default: return of(std::integral_constant<int, kQuickGelu>{});
+    case kSilu: return run(std::integral_constant<int, kSilu>{});
+    case kGeluTanh: return run(std::integral_constant<int, kGeluTanh>{});
+    case kGelu: return run(std::integral_constant<int, kGelu>{});
+    case kRelu: return run(std::integral_constant<int, kRelu>{});
+    default: return run(std::integral_constant<int, kQuickGelu>{});
   }
 }
 
