@@ -191,13 +191,23 @@ int launch_few(const void* A, const void* B, long long lda, long long ldb, const
 // that finishes them, a share of the rows each, so that every CTA reads, adds and writes as much as the others.
 constexpr int kMaxStages = 12;
 
-// Rows that each of `splits` CTAs finishes of `live` ones, and how far apart (in numbers) its channels lie in its buffer.
+// Rows that each of `splits` CTAs finishes of `live` ones, and how far apart (in numbers) the channels of such a share lie: four rows are written at a time, and
+// an odd multiple of 16 bytes lets neighbouring channels meet in no bank.
 __host__ __device__ inline int exchange_share(int live, int splits) { return ((live + splits - 1) / splits + 3) / 4 * 4; }
 __host__ __device__ inline int exchange_pitch(int share) { return 4 * (share / 4 | 1); }
 
+// A copy from this CTA's shared memory to that of CTA `to` of the cluster, completion on its barrier; both are given by their place here.
+__device__ __forceinline__ void bulk_copy_to(const void* dst_here, const void* src, uint32_t bytes, uint64_t* bar_here, int to) {
+  uint32_t dst, bar;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(dst_here)), "r"(to));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(bar_here)), "r"(to));
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(smem_u32(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 template <int TN>
 __global__ void __launch_bounds__(kThreads, 1)
-stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Params p, int stages, int kb_per_split) {
+stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Params p, int stages, int kb_per_split, int ring_bytes) {
   constexpr int kWBytes = 128 * BK;
   constexpr int kXBytes = TN * BK;
   constexpr int kStage = kWBytes + kXBytes;
@@ -207,7 +217,8 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem);
   uint64_t* empty_bar = full_bar + kMaxStages;
   uint64_t* tfull_bar = empty_bar + kMaxStages;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull_bar + 1);
+  uint64_t* parts_bar = tfull_bar + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(parts_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   float* s_scale = reinterpret_cast<float*>(smem + 1024);  // the rows' scales
   uint8_t* ring = smem + 2048;
@@ -222,6 +233,9 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
   const int kb0 = rank * kb_per_split;
   const int n_kb = min(k_blocks, kb0 + kb_per_split) - kb0;  // at least one (the launcher sees to it)
 
+  const int live = min(TN, p.M - m0);
+  const int share = exchange_share(live, splits), pitch = exchange_pitch(share);
+  const uint32_t part_bytes = 128u * pitch * 4u;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int s = 0; s < stages; ++s) {
@@ -229,7 +243,9 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
       mbar_init(&empty_bar[s], 1);
     }
     mbar_init(tfull_bar, 1);
+    mbar_init(parts_bar, 1);
     mbar_fence_init();
+    if (splits > 1) mbar_expect_tx(parts_bar, (splits - 1) * part_bytes);
     tma_prefetch_desc(&tmW);
     tma_prefetch_desc(&tmX);
   }
@@ -241,6 +257,7 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (waited for ahead of the exchange) the barriers are there
   if (warp == 0 && blockIdx.y == 0 && lane < min(stages, n_kb)) tma_prefetch_2d(&tmW, (kb0 + lane) * BK, n0);  // weights: into the L2 while the kernel before ends
   chain_wait();
 
@@ -280,7 +297,6 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
   __syncwarp();
   // ---- the epilogue's operands, while the sums are made
   const int quad = warp & 3;
-  const int live = min(TN, p.M - m0);
   const int n = n0 + quad * 32 + lane;
   const bool in = n < p.N;
   float sb = 0.f, bias = 0.f;
@@ -314,39 +330,50 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
         finish_column<kLoad>(p, m0 + c, live - c, n, in, r, s_scale + c, sb, bias);
       }
   } else {
-    // Rows [i share, (i + 1) share) of the tile are finished by CTA i: its buffer is [source CTA][channel][row], where the ring was.  Four rows travel
-    // together; the pitch of a channel is an odd multiple of 16 bytes, so that neighbouring lanes meet in no bank.
-    const int share = exchange_share(live, splits), pitch = exchange_pitch(share);
-    const uint32_t mine = smem_u32(ring);
-    const uint32_t slot = static_cast<uint32_t>((rank * 128 + quad * 32 + lane) * pitch * 4);
-    cluster_sync_all();  // every CTA of the cluster is done with its ring
-    if (warp >= 2 && all)
-      for (int c = 0; c < live; c += kLoad) {
-        int r[kLoad];
-        sums(c, r);
+    // Rows [i share, (i + 1) share) of the tile are finished by CTA i.  A CTA writes its sums of every share, [channel][row], where its ring was, and sends
+    // each to its CTA with one copy; it adds what it has itself to what the others send, which has a place of its own behind the ring.
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    uint8_t* sent = ring;
+    uint8_t* got = ring + ring_bytes;
+    if (warp >= 2) {
+      if (all) {
+        const int at = (quad * 32 + lane) * pitch;
+        for (int c = 0; c < live; c += kLoad) {
+          int r[kLoad];
+          sums(c, r);
+          int to = c / share, i = c - to * share;
 #pragma unroll
-        for (int j = 0; j < kLoad; j += 4) {
-          if (c + j < live) {
-            const int to = (c + j) / share;
-            uint32_t remote;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(mine + slot + (c + j - to * share) * 4), "r"(to));
-            asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "r"(r[j]), "r"(r[j + 1]), "r"(r[j + 2]), "r"(r[j + 3]) : "memory");
+          for (int j = 0; j < kLoad; j += 4) {
+            if (c + j < live) *reinterpret_cast<int4*>(reinterpret_cast<int*>(sent + to * part_bytes) + at + i) = make_int4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            i += 4;
+            if (i == share) {
+              i = 0;
+              ++to;
+            }
           }
         }
       }
-    cluster_sync_all();  // all parts have arrived
-    if (warp >= 2 && all && !*abort_flag) {
-      const int first = rank * share, count = min(share, live - first);
-      const int* part = reinterpret_cast<const int*>(ring) + (quad * 32 + lane) * pitch;
-      for (int i = 0; i < count; i += 4) {
-        int sum[4] = {0, 0, 0, 0};
-        for (int s = 0; s < splits; ++s) {
-          const int4 v = *reinterpret_cast<const int4*>(part + s * 128 * pitch + i);
-          sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+      fence_proxy_async_smem();
+      named_bar_sync(1, 128);
+      if (warp == 2 && lane < splits && lane != rank && all)
+        bulk_copy_to(got + (rank < lane ? rank : rank - 1) * part_bytes, sent + lane * part_bytes, part_bytes, parts_bar, lane);
+      const bool complete = __all_sync(0xffffffffu, mbar_wait(parts_bar, 0, abort_flag, p.status, 400, rank));
+      if (all && complete) {
+        const int first = rank * share, count = min(share, live - first);
+        const int* own = reinterpret_cast<const int*>(sent + rank * part_bytes) + (quad * 32 + lane) * pitch;
+        const int* other = reinterpret_cast<const int*>(got) + (quad * 32 + lane) * pitch;
+        for (int i = 0; i < count; i += 4) {
+          const int4 a = *reinterpret_cast<const int4*>(own + i);
+          int sum[4] = {a.x, a.y, a.z, a.w};
+          for (int s = 0; s < splits - 1; ++s) {
+            const int4 v = *reinterpret_cast<const int4*>(other + s * 128 * pitch + i);
+            sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+          }
+          finish_column<4>(p, m0 + first + i, count - i, n, in, sum, s_scale + first + i, sb, bias);
         }
-        finish_column<4>(p, m0 + first + i, count - i, n, in, sum, s_scale + first + i, sb, bias);
       }
     }
+    cluster_sync_all();  // nobody leaves while its copies are read or written
   }
   tc_fence_before();
   __syncthreads();
@@ -363,20 +390,25 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
   if (splits < 1) splits = 1;
   if (splits > 8) splits = 8;
   if (splits > k_blocks) splits = k_blocks;
-  const int per = (k_blocks + splits - 1) / splits;
-  splits = (k_blocks + per - 1) / per;  // no empty share
-  // the ring also holds the exchanged sums
-  const int exchange = splits > 1 ? splits * 128 * 4 * exchange_pitch(exchange_share(p.M < TN ? p.M : TN, splits)) : 0;
   if (stages > kMaxStages) stages = kMaxStages;
-  if (stages > 220 * 1024 / kStage) stages = 220 * 1024 / kStage;
-  if (stages > per) stages = per;
-  if (stages < 1) stages = 1;
+  int per, part, ring;
+  while (true) {  // as many splits as the shared memory has room for
+    per = (k_blocks + splits - 1) / splits;
+    splits = (k_blocks + per - 1) / per;  // no empty share
+    if (stages > per) stages = per;
+    if (stages < 1) stages = 1;
+    part = splits > 1 ? 128 * 4 * exchange_pitch(exchange_share(p.M < TN ? p.M : TN, splits)) : 0;
+    while (stages > 1 && stages * kStage + (splits - 1) * part > 220 * 1024) --stages;
+    ring = stages * kStage > splits * part ? stages * kStage : (splits * part + 1023) / 1024 * 1024;  // it also holds the sums that are sent
+    if (ring + (splits - 1) * part <= 220 * 1024) break;
+    --splits;  // (one split needs the ring alone)
+  }
   // CTAs whose tensor memory does not fit beside that of others on their SM wait for it, and CTAs of clusters wait for one another: that could close a
   // circle.  A share of shared memory that is at least the share of tensor memory keeps out what would not fit; 34 KB keeps out the pairs of
   // the kernels with 256 x 256 tiles, which take all columns and all but 30 KB.
   constexpr int kCols = TN < 32 ? 32 : TN;
   constexpr int kLeast = kCols * 464 > 34 * 1024 ? kCols * 464 : 34 * 1024;
-  int bytes = stages * kStage > exchange ? stages * kStage : exchange;
+  int bytes = ring + (splits - 1) * part;
   if (bytes < kLeast) bytes = kLeast;
   CUtensorMap tmW, tmX;
   int rc = make_tmap_2d_u8(&tmW, B, p.N, p.K, ldb, 128);
@@ -399,14 +431,14 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, stream_kernel<TN>, tmW, tmX, p, stages, per) == cudaSuccess ? kErrOk : kErrCuda;
+  return cudaLaunchKernelEx(&cfg, stream_kernel<TN>, tmW, tmX, p, stages, per, ring) == cudaSuccess ? kErrOk : kErrCuda;
 }
 
 // ================================================================ many rows
 constexpr int BN = 256, BMP = 256, BMC = 128;
 constexpr int kPairStage = (BMC + BN / 2) * BK;  // per CTA
 constexpr int kPairStages = 6;
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 2 * BN * 4 + (2 * kPairStages + 4) * 8 + 16;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 4 * BN * 4 + (2 * kPairStages + 4) * 8 + 16;
 
 __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& mb, int& nb) {
   constexpr int GM = 4;  // four row tiles stay in the L2 while the raster sweeps N
@@ -420,7 +452,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* s_scale = reinterpret_cast<float*>(smem + kPairStages * kPairStage);  // the columns' scales, of one tile and the next
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_scale + 2 * BN);
+  float* s_bias = s_scale + 2 * BN;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_scale + 4 * BN);
   uint64_t* empty_bar = full_bar + kPairStages;
   uint64_t* tfull_bar = empty_bar + kPairStages;
   uint64_t* tempty_bar = tfull_bar + 2;
@@ -519,7 +552,9 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
       for (int j = 0; j < BN; j += 128) {
         const int at = j + static_cast<int>(threadIdx.x) - 64;
-        sb[at] = nb * BN + at < p.N ? __ldg(p.scale_b + nb * BN + at) : 0.f;
+        const bool there = nb * BN + at < p.N;
+        sb[at] = there ? __ldg(p.scale_b + nb * BN + at) : 0.f;
+        if (p.flags & kBias) s_bias[buf * BN + at] = there ? bias_at(p, nb * BN + at) : 0.f;
       }
       named_bar_sync(1, 128);
       if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&tfull_bar[buf], tphase, abort_flag, p.status, 300, buf));
@@ -546,8 +581,10 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         }
         if (p.flags & kBias) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < cols) v[j] += bias_at(p, n0 + j);
+          for (int q = 0; q < 8; ++q) {
+            const float4 f = *reinterpret_cast<const float4*>(s_bias + buf * BN + c + 4 * q);
+            v[4 * q] += f.x; v[4 * q + 1] += f.y; v[4 * q + 2] += f.z; v[4 * q + 3] += f.w;
+          }
         }
         if (p.flags & kResidual) {
           if (p.flags & kResidualF32) {
@@ -654,6 +691,40 @@ int launch_pair(const void* A, const void* B, long long lda, long long ldb, cons
   return launch_chained(pair_kernel, dim3(grid), dim3(kThreads), kPairSmem, s, tmA, tmB, p) == cudaSuccess ? kErrOk : kErrCuda;
 }
 
+// Which form (us, weights out of the cache).  few / stream: 1 row, 768 x 768 2.0 / 3.2, 2304 x 768 2.6 / 3.3, 2048 x 2048 4.4 / 3.7, 4096 x 4096 7.8 / 5.3; 16 rows, 2304 x 768
+// 3.3 / 3.6.  stream / pair, where the stream's tiles of 128 x 256 are one wave: 512 rows, 2304 x 768 6.7 / 9.6, 6144 x 4096 15.9 / 17.2; 1000 rows, 4096 x 4096
+// 15.3 / 16.6; more than a wave: 777 rows, 6144 x 4096 26.2 / 26.2, 28672 x 4096 116 / 83, 1500 rows, 4096 x 4096 28 / 26; up to 128 rows, 28672 x 4096 24 / 30.
+inline int choose_form(int M, int N, int K) {
+  if (M <= 16 && K <= 1024 && N <= 4096) return 1;
+  if (M <= 128) return 2;
+  return static_cast<long long>((N + 127) / 128) * ((M + 255) / 256) <= num_sms() ? 2 : 3;
+}
+// Splits of K and ring stages of the stream form, where they are 0.  A CTA gets 16 KB of weights per 0.28 us wherever they come from, so fewer than some 110 CTAs do
+// not keep the memory busy, and all that run should run at once; a split costs a start, the exchange of its sums (which grows with the rows) and the rows
+// of activations once more.  us for 1, 2, 4, 8 splits: 4096 x 4096, 1 row 10.8, 7.8, 5.3, 6.4, 64 rows 11.6, 10.4, 8.2, 20, 128 rows 12.3, 13.0, 10.9; 6144 x 4096, 16
+// rows 11.2, 8.7, 6.9, 7.9; 8192 x 2048, 16 rows 7.4, 5.7, 6.3, 10.3; 512 x 8192, 1 row 19.5, 11.4, 7.0, 5.0; 28672 x 4096, 1 row 20.7, 25, 25, 32.
+inline void choose_splits(int M, int N, int K, int& splits, int& stages) {
+  const int tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  const int tiles = (N + 127) / 128 * ((M + tn - 1) / tn), k_blocks = (K + BK - 1) / BK, sms = num_sms();
+  if (splits == 0) {
+    splits = 1;
+    if (tn <= 64) {
+      if (3 * tiles <= sms) splits = 4;  // 48 tiles
+      else if (2 * tiles <= sms && tn <= 32) splits = 2;
+      if (16 * tiles <= sms && k_blocks >= 32) splits = 8;
+      while (splits > 1 && k_blocks < 4 * splits) splits /= 2;
+    } else if (tn == 128) {
+      if (4 * tiles <= sms && k_blocks >= 32) splits = 4;
+    } else if (2 * tiles <= sms && k_blocks >= 64) {
+      splits = 2;
+    }
+  }
+  if (stages == 0) {
+    const int per_sm = (tiles * splits + sms - 1) / sms;
+    stages = (per_sm <= 1 ? 216 : per_sm == 2 ? 110 : 72) * 1024 / ((128 + tn) * BK);
+  }
+}
+
 }  // namespace int8_gemm
 }  // namespace lvb
 
@@ -672,15 +743,11 @@ extern "C" int lvb_int8_gemm(const void* A, const void* B, const float* scale_a,
   if (((flags & kBias) && bias == nullptr) || ((flags & kResidual) && (residual == nullptr || ldr < N))) return kErrBadArg;
   Params p{C, scale_a, scale_b, bias, residual, M, N, K, ldc, ldr, flags, status};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (form == 0) form = M <= 16 ? 1 : M <= 256 ? 2 : 3;
+  if (form == 0) form = choose_form(M, N, K);
   if (form == 1) return M <= 16 ? launch_few(A, B, lda, ldb, p, s) : kErrBadArg;
   if (form == 3) return launch_pair(A, B, lda, ldb, p, s);
   if (form != 2) return kErrBadArg;
-  if (splits == 0) {
-    const int tiles = (N + 127) / 128;
-    splits = num_sms() / tiles;
-  }
-  if (stages == 0) stages = kMaxStages;
+  choose_splits(M, N, K, splits, stages);
   if (M <= 16) return launch_stream<16>(A, B, lda, ldb, p, splits, stages, s);
   if (M <= 32) return launch_stream<32>(A, B, lda, ldb, p, splits, stages, s);
   if (M <= 64) return launch_stream<64>(A, B, lda, ldb, p, splits, stages, s);

@@ -277,13 +277,22 @@ struct Raw16 {
   }
   __device__ __forceinline__ F32x2 pair(int j) const { return f2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xFFFF0000u)); }
 };
-struct Plain16 {
+constexpr int kMostParts = 5;
+struct Plain16 {  // rows of up to five matrices, one behind the other: those from row end[i - 1] on lie `off[i]` elements from where x would have them
   const __nv_bfloat16* x;
+  int end[kMostParts - 1];
+  long long off[kMostParts];
   struct In {
     Raw16 x;
   };
   static constexpr bool kSum = false;
-  __device__ __forceinline__ void load(In& in, long long at) const { in.x.load(x + at); }
+  __device__ __forceinline__ void load(In& in, long long at, int row) const {
+    long long o = off[0];
+#pragma unroll
+    for (int i = 0; i < kMostParts - 1; ++i)
+      if (row >= end[i]) o = off[i + 1];
+    in.x.load(x + at + o);
+  }
   __device__ __forceinline__ void get(const In& in, long long, int, float (&y)[16], F32x2&) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f2_split(in.x.pair(j), y[2 * j], y[2 * j + 1]);
@@ -300,7 +309,7 @@ struct Norm16 {
     Raw16 x, r;
   };
   static constexpr bool kSum = true;
-  __device__ __forceinline__ void load(In& in, long long at) const {
+  __device__ __forceinline__ void load(In& in, long long at, int) const {
     in.x.load(x + at);
     if constexpr (kResidual) in.r.load(r + at);
   }
@@ -343,7 +352,7 @@ struct Glu16 {
     Raw16 g, u;
   };
   static constexpr bool kSum = false;
-  __device__ __forceinline__ void load(In& in, long long at) const {
+  __device__ __forceinline__ void load(In& in, long long at, int) const {
     in.g.load(g + at);
     in.u.load(u + at);
   }
@@ -540,7 +549,7 @@ __global__ void __launch_bounds__(kMostThreads) rows16_kernel(Src src, long long
   int row = blockIdx.x;
   long long at = row * ld + c;
   typename Src::In in;
-  if (mine) src.load(in, at);
+  if (mine) src.load(in, at, row);
   for (int odd = 0; row < rows; row += step, odd ^= 1) {
     float y[16] = {};
     F32x2 ss2 = f2(0.f, 0.f);
@@ -550,7 +559,7 @@ __global__ void __launch_bounds__(kMostThreads) rows16_kernel(Src src, long long
 #pragma unroll
       for (int j = 0; j < 16; j += 2) largest = largest_of(largest, y[j], y[j + 1]);
       at += step * ld;
-      if (row + step < rows) src.load(in, at);
+      if (row + step < rows) src.load(in, at, row + step);
     }
     uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
     float ss = warp_ss<Src::kSum>(ss2);
@@ -704,8 +713,33 @@ extern "C" int lvb_int8_quantize(const void* x, int f32, long long ldx, long lon
   using namespace lvb::int8_rows;
   if (x == nullptr) return kErrBadArg;
   if (f32) return quantize(Plain<float>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
-  if (rows16(rows, cols, ldx, {{x, ldx}})) return quantize16(Plain16{static_cast<const __nv_bfloat16*>(x)}, ldx, rows, cols, q, ldq, scale, stream);
+  if (rows16(rows, cols, ldx, {{x, ldx}})) {
+    Plain16 src{static_cast<const __nv_bfloat16*>(x), {}, {}};
+    for (int i = 0; i < kMostParts - 1; ++i) src.end[i] = 0x7FFFFFFF;
+    return quantize16(src, ldx, rows, cols, q, ldq, scale, stream);
+  }
   return quantize(Plain<__nv_bfloat16>{{x, ldx, rows, cols}}, rows, cols, q, ldq, scale, stream);
+}
+
+// The rows of up to five dense bf16 matrices with the same columns (a multiple of 16 from 528 to 16384; 32-byte aligned), one matrix behind the other:
+// xi [ni, cols], those past the last null with no rows.
+extern "C" int lvb_int8_quantize_parts(const void* x0, const void* x1, const void* x2, const void* x3, const void* x4, int n0, int n1, int n2, int n3, int n4,
+                                       int cols, void* q, float* scale, void* stream) {
+  using namespace lvb;
+  using namespace lvb::int8_rows;
+  const void* x[kMostParts] = {x0, x1, x2, x3, x4};
+  const int n[kMostParts] = {n0, n1, n2, n3, n4};
+  Plain16 src{static_cast<const __nv_bfloat16*>(x0), {}, {}};
+  long long rows = 0;
+  for (int i = 0; i < kMostParts; ++i) {
+    if (n[i] < 0 || (n[i] > 0 && x[i] == nullptr)) return kErrBadArg;
+    src.off[i] = n[i] > 0 ? (reinterpret_cast<intptr_t>(x[i]) - reinterpret_cast<intptr_t>(x0)) / 2 - rows * cols : 0;
+    rows += n[i];
+    if (rows > 0x3FFFFFFF) return kErrTooLarge;
+    if (i < kMostParts - 1) src.end[i] = static_cast<int>(rows);
+  }
+  if (n0 <= 0 || !rows16(rows, cols, cols, {{x0, cols}, {x1, cols}, {x2, cols}, {x3, cols}, {x4, cols}})) return kErrBadArg;
+  return quantize16(src, cols, rows, cols, q, cols, scale, stream);
 }
 
 // The RMS norm of x (+ residual): weight [cols] (w_f32: fp32, else bf16; may be null) plus w_offset.  With a residual h = x + residual is written, in

@@ -66,7 +66,7 @@ class Int8Rows(NamedTuple):
 # ------------------------------------------------------------------------------------------------ calls
 # Arguments of the launchers by letter (p pointer, l long long, i int, f float); a stream follows.
 _ARGS = {"lvb_int8_quantize": "pilliplp", "lvb_int8_rms_norm": "pppilllpiffliplp", "lvb_int8_glu": "ppilliliplp", "lvb_int8_dequantize": "plplipi",
-         "lvb_int8_gemm": "pppppiiilllippliiip"}
+         "lvb_int8_gemm": "pppppiiilllippliiip", "lvb_int8_quantize_parts": "pppppiiiiiipp"}
 
 
 def _launch(name: str, t: torch.Tensor, *args) -> None:
@@ -316,18 +316,54 @@ def _straight_through(x: torch.Tensor) -> torch.Tensor:
     return x + (quantize_reference(x.detach()).dequantize(torch.float32).to(x.dtype) - x).detach()
 
 
+def _quantize_parts(parts: List[torch.Tensor]) -> List[Int8Rows]:
+    """The rows of each of the parts, which have the same columns; one launch for up to five aligned ones, as parts of one buffer."""
+    cols = parts[0].shape[-1]
+    if not (1 < len(parts) <= 5 and cols % 16 == 0 and 512 < cols <= 16384 and all(p.is_contiguous() and p.data_ptr() % 32 == 0 for p in parts)):
+        return [_quantize(p) for p in parts]
+    counts = [p.numel() // cols for p in parts]
+    dev = parts[0].device
+    values = torch.empty(sum(counts), cols, dtype=torch.int8, device=dev)
+    scale = torch.empty(values.shape[0], dtype=torch.float32, device=dev)
+    pad = (0,) * (5 - len(parts))
+    _launch("lvb_int8_quantize_parts", values, *[p.data_ptr() for p in parts], *pad, *counts, *pad, cols, values.data_ptr(), scale.data_ptr())
+    return [Int8Rows(v.view(p.shape), s.view(p.shape[:-1])) for p, v, s in zip(parts, values.split(counts), scale.split(counts))]
+
+
+def _joint(rows: Sequence[Int8Rows]) -> Optional[Int8Rows]:
+    """Matrices that lie one behind the other in one buffer as one, or None."""
+    v0, s0 = rows[0]
+    at, scales, n = v0.data_ptr(), s0.data_ptr(), 0
+    if v0.stride(-1) != 1 or not all(v.is_contiguous() for v, _ in rows):
+        return None
+    for v, s in rows:
+        if v.data_ptr() != at + n * v0.shape[-1] or s.data_ptr() != scales + 4 * n or v.untyped_storage().data_ptr() != v0.untyped_storage().data_ptr():
+            return None
+        n += s.numel()
+    return Int8Rows(v0.as_strided((n, v0.shape[-1]), (v0.shape[-1], 1)), s0.as_strided((n,), (1,)))
+
+
+# Up to so many rows the host's part bounds a layer: the projections are one product, whose columns are their results, and their output gradients are
+# laid side by side for one product each way.  Above it their results are tensors of their own, as their readers expect them, and the input gradient
+# is summed in fp32.
+MANY_ROWS = 2048
+
+
 class _Int8ManyFn(torch.autograd.Function):
     """Projections of the same rows.  Kept for the backward pass: the rows and the weights in 8 bits, 1 byte per activation instead of 2, once for all projections.
 
     ``dx = sum dy w'`` and ``dw = dy^T x'`` are bf16 products of what the whole numbers stand for, rounded to bf16 (2^-9 of each value, as any operand
-    of a bf16 layer); output gradients are not quantised, their rows span too many magnitudes for one scale."""
+    of a bf16 layer); output gradients are not quantised, their rows span too many magnitudes for one scale.  The sum over several projections is rounded once."""
 
     @staticmethod
     def forward(ctx, x, count, *tensors):
         weights, biases = tensors[:count], tensors[count:]
-        rows = _quantize(x)
-        ws = [_quantize(w) for w in weights]
-        ys = tuple(_product(rows, w, b, out_dtype=x.dtype) for w, b in zip(ws, biases))
+        rows, *ws = _quantize_parts([x, *weights])
+        joint = _joint(ws) if count > 1 and rows.scale.numel() <= MANY_ROWS and not any(b is not None for b in biases) else None
+        if joint is not None:
+            ys = _product(rows, joint, out_dtype=x.dtype).split([w.shape[0] for w in weights], dim=-1)
+        else:
+            ys = tuple(_product(rows, w, b, out_dtype=x.dtype) for w, b in zip(ws, biases))
         ctx.save_for_backward(rows.values, rows.scale, *[t for w in ws for t in w])
         ctx.refs, ctx.bias_dtypes = weights, [None if b is None else b.dtype for b in biases]
         ctx.x_shape = x.shape
@@ -339,26 +375,47 @@ class _Int8ManyFn(torch.autograd.Function):
         from .gemm import _weight_grad, col_sum, gemm
 
         values, scale, *flat = ctx.saved_tensors
-        n = len(ctx.refs)
-        need_w = [dy is not None and need for dy, need in zip(dys, ctx.needs_input_grad[2:2 + n])]
-        x2 = None
-        if any(need_w):
-            x2 = Int8Rows(values, scale).dequantize().reshape(-1, values.shape[-1])
+        n, cols = len(ctx.refs), values.shape[-1]
+        live = [i for i, dy in enumerate(dys) if dy is not None]
+        need_x = ctx.needs_input_grad[0]
+        need_w = [i for i in live if ctx.needs_input_grad[2 + i]]
+        need_b = [i for i in live if ctx.bias_dtypes[i] is not None and ctx.needs_input_grad[2 + n + i]]
         dx, dws, dbs = None, [None] * n, [None] * n
-        for i, dy in enumerate(dys):
-            if dy is None:
-                continue
-            dy2 = dy.reshape(-1, dy.shape[-1])
-            if dy2.dtype != torch.bfloat16:
-                dy2 = dy2.to(torch.bfloat16)
-            if ctx.needs_input_grad[0]:
-                w = Int8Rows(flat[2 * i], flat[2 * i + 1]).dequantize()
-                dx = gemm(dy2, w, b_mn=True, out=dx, accumulate=dx is not None)
-            if need_w[i]:
-                dws[i] = _weight_grad(ctx.refs[i], dy2, x2)
-            if ctx.bias_dtypes[i] is not None and ctx.needs_input_grad[2 + n + i]:
-                dbs[i] = col_sum(dy2, ctx.bias_dtypes[i])
-        return (None if dx is None else dx.view(ctx.x_shape), None, *dws, *dbs)
+        if not live:
+            return (None, None, *dws, *dbs)
+        d2 = {i: dys[i].reshape(-1, dys[i].shape[-1]) for i in live}
+        d2 = {i: d if d.dtype == torch.bfloat16 else d.to(torch.bfloat16) for i, d in d2.items()}
+        rows, ws = Int8Rows(values, scale), [Int8Rows(flat[2 * i], flat[2 * i + 1]) for i in live]
+        wanted = ([rows] if need_w else []) + (ws if need_x else [])
+        whole = _joint(wanted) if len(wanted) > 1 else None
+        if whole is not None:
+            counts = [r.scale.numel() for r in wanted]
+            back = list(whole.dequantize().split(counts))
+        else:
+            back = [r.dequantize().reshape(-1, cols) for r in wanted]
+        x2 = back.pop(0) if need_w else None
+        sizes = [d2[i].shape[1] for i in live]
+        side = None
+        if len(live) > 1 and scale.numel() <= MANY_ROWS:
+            side = torch.cat([d2[i] for i in live], dim=1)
+        if need_x:
+            if side is not None:
+                w = back[0].as_strided((sum(sizes), cols), (cols, 1)) if whole is not None else torch.cat(back)
+                dx = gemm(side, w, b_mn=True)
+            else:
+                for i, w in zip(live, back):
+                    dx = gemm(d2[i], w, b_mn=True, out=dx, accumulate=dx is not None, out_dtype=torch.bfloat16 if len(live) == 1 else torch.float32)
+            dx = dx.to(torch.bfloat16).view(ctx.x_shape)
+        plain = all(getattr(ctx.refs[i], "main_grad", None) is None and getattr(ctx.refs[i], "grad_sink", None) is None and ctx.refs[i].dtype == torch.bfloat16 for i in live)
+        if side is not None and need_w == live and plain:
+            for i, dw in zip(live, gemm(side, x2, a_mn=True, b_mn=True).split(sizes)):
+                dws[i] = dw
+        else:
+            for i in need_w:
+                dws[i] = _weight_grad(ctx.refs[i], d2[i], x2)
+        for i in need_b:
+            dbs[i] = col_sum(d2[i], ctx.bias_dtypes[i])
+        return (dx, None, *dws, *dbs)
 
 
 def int8_linear_many(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: Optional[Sequence[Optional[torch.Tensor]]] = None) -> Tuple[torch.Tensor, ...]:
@@ -379,8 +436,8 @@ def int8_linear_many(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: O
 
     if _kernels(x) and x.dtype == torch.bfloat16 and x.numel() and all(w.dtype == torch.bfloat16 and _tma_shapes_ok(w) and w.shape[0] > 0 for w in weights):
         if lib.plain_call():
-            rows = _quantize(x)
-            return tuple(_product(rows, _quantize(w), b) for w, b in zip(weights, biases))
+            rows, *ws = _quantize_parts([x, *weights])
+            return tuple(_product(rows, w, b) for w, b in zip(ws, biases))
         return _Int8ManyFn.apply(x, len(weights), *weights, *biases)
     x8 = _straight_through(x)
     return tuple(F.linear(x8, _straight_through(w).to(x.dtype), None if b is None else b.to(x.dtype)) for w, b in zip(weights, biases))

@@ -232,3 +232,105 @@ def test_nan_rows_stay_where_they_are():
     w = I.quantize_rows(rand(40, 256, seed=2))
     y = I.int8_product(I.quantize_rows(x), w)
     assert y[3].isnan().all() and int(y.isnan().sum()) == 40
+
+
+# ------------------------------------------------------------------------------------------------ layers in training
+def held(x):
+    q, s = whole(x)
+    return q * s[..., None]
+
+
+@pytest.mark.parametrize("shape,outs,bias", [((1, 64), [8], False), ((5, 7, 768), [256, 1000, 8], False), ((3, 200), [16, 24], True), ((2100, 1024), [512, 528], False),
+                                             ((999, 768), [2304], True), ((2, 3, 1040), [64, 8, 16, 24], False), ((130, 544), [16, 8, 8, 8, 8, 16], False)])
+def test_linear_many_and_its_gradients(shape, outs, bias):
+    x = rand(*shape, seed=1).requires_grad_()
+    ws = [rand(n, shape[-1], seed=2 + n, std=0.05).requires_grad_() for n in outs]
+    bs = [rand(n, seed=3 + n).requires_grad_() for n in outs] if bias else None
+    ys = I.int8_linear_many(x, ws, bs)
+    dys = [rand(*y.shape, seed=7 + i) for i, y in enumerate(ys)]
+    grads = torch.autograd.grad(ys, [x, *ws, *(bs or [])], dys)
+    lib.check_status()
+    xd, wd, gd = held(x.detach()), [held(w.detach()) for w in ws], [g.double() for g in dys]
+    dx = torch.zeros_like(xd)
+    size = torch.zeros_like(xd)
+    for i, (y, w, g) in enumerate(zip(ys, wd, gd)):
+        want = xd @ w.t() + (bs[i].double() if bias else 0.0)
+        assert y.shape == want.shape and bool(((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -21 * (xd.abs() @ w.abs().t() + 1)).all())
+        dx += g @ w
+        size += g.abs() @ w.abs()
+        dw, mag = g.flatten(0, -2).t() @ xd.flatten(0, -2), g.flatten(0, -2).abs().t() @ xd.flatten(0, -2).abs()
+        # operands rounded to bf16 (2^-8 of every product at most), sums in fp32, one rounding of the result
+        assert bool(((grads[1 + i].double() - dw).abs() <= 2.0 ** -8 * dw.abs() + 1.01 * 2.0 ** -8 * mag).all())
+        if bias:
+            db = g.flatten(0, -2).sum(0)
+            assert bool(((grads[1 + len(outs) + i].double() - db).abs() <= 2.0 ** -8 * db.abs() + 2.0 ** -18 * g.flatten(0, -2).abs().sum(0)).all())
+    assert bool(((grads[0].double() - dx).abs() <= 2.0 ** -8 * dx.abs() + 1.01 * 2.0 ** -8 * size).all())
+    # and not only at worst: roundings of either sign average out
+    assert (grads[0].double() - dx).norm() <= 2.0 ** -8 * dx.norm()
+
+
+def test_gradient_against_differences():
+    """The loss is linear in what the rows stand for, so the difference between two inputs whose rows are exact is the gradient times their difference."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randint(-63, 64, (6, 64), generator=g, device="cuda").float()
+    q[:, 0] = 127  # the scale of every row is 2^-6, before and after
+    x = (q * 2.0 ** -6).to(BF)
+    w = (torch.randint(-63, 64, (32, 64), generator=g, device="cuda").float() * 2.0 ** -6).to(BF)
+    w[:, 0] = 127 * 2.0 ** -6
+    c = torch.randint(-4, 5, (6, 32), generator=g, device="cuda").to(BF)
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    gx, gw = torch.autograd.grad((I.int8_linear(xr, wr).float() * c.float()).sum(), [xr, wr])
+    with torch.no_grad():
+        rows, wrows = I.quantize_rows(x), I.quantize_rows(w)
+        f = lambda a, b: (I.int8_product(I.quantize_rows(a), I.quantize_rows(b), out_dtype=F32).double() * c.double()).sum()  # noqa: E731
+        assert torch.equal(rows.dequantize(), x) and torch.equal(wrows.dequantize(), w)
+        for i, j in ((0, 5), (3, 63), (5, 17)):
+            step = torch.zeros_like(x)
+            step[i, j] = 2.0 ** -6
+            assert abs((f(x + step, w) - f(x, w)).item() - gx[i, j].double().item() * 2.0 ** -6) <= 2.0 ** -8 * abs(gx[i, j].item()) * 2.0 ** -6
+        for i, j in ((0, 5), (31, 63), (7, 17)):
+            step = torch.zeros_like(w)
+            step[i, j] = 2.0 ** -6
+            assert abs((f(x, w + step) - f(x, w)).item() - gw[i, j].double().item() * 2.0 ** -6) <= 2.0 ** -8 * abs(gw[i, j].item()) * 2.0 ** -6
+
+
+def test_what_is_kept_is_in_8_bits():
+    x, w = rand(4000, 4096).requires_grad_(), rand(1024, 4096, seed=2).requires_grad_()
+    I.int8_linear(x, w)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = I.int8_linear(x, w)
+    kept = torch.cuda.memory_allocated() - before - y.numel() * 2
+    assert kept <= 1.05 * (x.numel() + w.numel())
+    del y
+
+
+def test_gradients_of_some():
+    x, ws = rand(64, 1024).requires_grad_(), [rand(32, 1024, seed=2 + i).requires_grad_() for i in range(3)]
+    y0, y1, y2 = I.int8_linear_many(x, ws)
+    gx, g1 = torch.autograd.grad(y1.sum(), [x, ws[1]], retain_graph=True)
+    want = torch.autograd.grad(I.int8_linear(x, ws[1]).sum(), [x, ws[1]])
+    assert torch.equal(gx, want[0]) and torch.equal(g1, want[1])
+    assert torch.autograd.grad(y0.sum(), [ws[1]], retain_graph=True, allow_unused=True)[0] is None
+    frozen = [w.detach() for w in ws]
+    (gx,) = torch.autograd.grad(sum(y.float().sum() for y in I.int8_linear_many(x, frozen)), [x])
+    assert gx.shape == x.shape
+    ys = I.int8_linear_many(x.detach(), ws)
+    assert all(g.shape == w.shape for g, w in zip(torch.autograd.grad(sum(y.float().sum() for y in ys), ws), ws))
+
+
+def test_main_grad_receives_the_weight_gradient():
+    x, w = rand(64, 512).requires_grad_(), rand(32, 512, seed=2).requires_grad_()
+    want = torch.autograd.grad(I.int8_linear(x, w).sum(), [w])[0]
+    w.main_grad = torch.ones(32, 512, device="cuda")
+    I.int8_linear(x, w).sum().backward()
+    assert w.grad is None and bool(((w.main_grad - 1 - want.float()).abs() <= 2.0 ** -8 * want.float().abs() + 2.0 ** -22).all())
+
+
+def test_sizes_without_a_kernel_take_the_library():
+    x, w = rand(6, 100).requires_grad_(), rand(13, 100, seed=2).requires_grad_()
+    y = I.int8_linear(x, w)
+    want = held(x.detach()) @ held(w.detach()).t()
+    assert bool(((y.double() - want).abs() <= 2.0 ** -6 * (held(x.detach()).abs() @ held(w.detach()).abs().t())).all())
+    y.sum().backward()
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape
