@@ -693,11 +693,11 @@ int launch_pair(const void* A, const void* B, long long lda, long long ldb, cons
 
 // Which form (us, weights out of the cache).  few / stream: 1 row, 768 x 768 2.0 / 3.2, 2304 x 768 2.6 / 3.3, 2048 x 2048 4.4 / 3.7, 4096 x 4096 7.8 / 5.3; 16 rows, 2304 x 768
 // 3.3 / 3.6.  stream / pair, where the stream's tiles of 128 x 256 are one wave: 512 rows, 2304 x 768 6.7 / 9.6, 6144 x 4096 15.9 / 17.2; 1000 rows, 4096 x 4096
-// 15.3 / 16.6; more than a wave: 777 rows, 6144 x 4096 26.2 / 26.2, 28672 x 4096 116 / 83, 1500 rows, 4096 x 4096 28 / 26; up to 128 rows, 28672 x 4096 24 / 30.
+// 15.3 / 16.6, 4096 x 14336 46 / 42; more than a wave: 777 rows, 6144 x 4096 26.2 / 26.2, 28672 x 4096 116 / 83, 1500 rows, 4096 x 4096 28 / 26; up to 128 rows, 28672 x 4096 24 / 30.
 inline int choose_form(int M, int N, int K) {
   if (M <= 16 && K <= 1024 && N <= 4096) return 1;
   if (M <= 128) return 2;
-  return static_cast<long long>((N + 127) / 128) * ((M + 255) / 256) <= num_sms() ? 2 : 3;
+  return K <= 4096 && static_cast<long long>((N + 127) / 128) * ((M + 255) / 256) <= num_sms() ? 2 : 3;
 }
 // Splits of K and ring stages of the stream form, where they are 0.  A CTA gets 16 KB of weights per 0.28 us wherever they come from, so fewer than some 110 CTAs do
 // not keep the memory busy, and all that run should run at once; a split costs a start, the exchange of its sums (which grows with the rows) and the rows

@@ -316,105 +316,120 @@ def _straight_through(x: torch.Tensor) -> torch.Tensor:
     return x + (quantize_reference(x.detach()).dequantize(torch.float32).to(x.dtype) - x).detach()
 
 
-def _quantize_parts(parts: List[torch.Tensor]) -> List[Int8Rows]:
-    """The rows of each of the parts, which have the same columns; one launch for up to five aligned ones, as parts of one buffer."""
-    cols = parts[0].shape[-1]
-    if not (1 < len(parts) <= 5 and cols % 16 == 0 and 512 < cols <= 16384 and all(p.is_contiguous() and p.data_ptr() % 32 == 0 for p in parts)):
-        return [_quantize(p) for p in parts]
-    counts = [p.numel() // cols for p in parts]
-    dev = parts[0].device
-    values = torch.empty(sum(counts), cols, dtype=torch.int8, device=dev)
-    scale = torch.empty(values.shape[0], dtype=torch.float32, device=dev)
-    pad = (0,) * (5 - len(parts))
-    _launch("lvb_int8_quantize_parts", values, *[p.data_ptr() for p in parts], *pad, *counts, *pad, cols, values.data_ptr(), scale.data_ptr())
-    return [Int8Rows(v.view(p.shape), s.view(p.shape[:-1])) for p, v, s in zip(parts, values.split(counts), scale.split(counts))]
-
-
-def _joint(rows: Sequence[Int8Rows]) -> Optional[Int8Rows]:
-    """Matrices that lie one behind the other in one buffer as one, or None."""
-    v0, s0 = rows[0]
-    at, scales, n = v0.data_ptr(), s0.data_ptr(), 0
-    if v0.stride(-1) != 1 or not all(v.is_contiguous() for v, _ in rows):
-        return None
-    for v, s in rows:
-        if v.data_ptr() != at + n * v0.shape[-1] or s.data_ptr() != scales + 4 * n or v.untyped_storage().data_ptr() != v0.untyped_storage().data_ptr():
-            return None
-        n += s.numel()
-    return Int8Rows(v0.as_strided((n, v0.shape[-1]), (v0.shape[-1], 1)), s0.as_strided((n,), (1,)))
-
-
-# Up to so many rows the host's part bounds a layer: the projections are one product, whose columns are their results, and their output gradients are
-# laid side by side for one product each way.  Above it their results are tensors of their own, as their readers expect them, and the input gradient
-# is summed in fp32.
+# Up to so many rows the host's part bounds a layer: the projections of a layer without biases are one product, whose columns are their results, and so are
+# their gradients.  Above it their results are tensors of their own, as their readers expect them.
 MANY_ROWS = 2048
+
+
+def _hold(x: torch.Tensor, weights: Sequence[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, int]:
+    """``(values, scale, stride)``: the 8-bit rows of ``x`` and of the weights, one behind the other, and the bytes from one to the next."""
+    cols = x.shape[-1]
+    ld = -(-cols // 16) * 16
+    parts = [x, *weights]
+    counts = [x.numel() // cols, *[w.shape[0] for w in weights]]
+    total = sum(counts)
+    values = torch.empty(total, ld, dtype=torch.int8, device=x.device)
+    scale = torch.empty(total, dtype=torch.float32, device=x.device)
+    q, s = values.data_ptr(), scale.data_ptr()
+    if len(parts) <= 5 and ld == cols and 512 < cols <= 16384 and all(p.is_contiguous() and p.data_ptr() % 32 == 0 for p in parts):
+        pad = (0,) * (5 - len(parts))
+        _launch("lvb_int8_quantize_parts", x, *[p.data_ptr() for p in parts], *pad, *counts, *pad, cols, q, s)
+    else:
+        for part, n in zip(parts, counts):
+            part, ptr, _, stride = _rows_of(part)
+            _launch("lvb_int8_quantize", part, ptr, 0, stride, n, cols, q, ld, s)
+            q, s = q + n * ld, s + 4 * n
+    return values, scale, ld
+
+
+def _held_products(x: torch.Tensor, values: torch.Tensor, scale: torch.Tensor, ld: int, weights, biases) -> Tuple[torch.Tensor, ...]:
+    """The products of what :func:`_hold` gives for ``x`` and the weights."""
+    lead, cols, rows = x.shape[:-1], x.shape[-1], x.numel() // x.shape[-1]
+    q, s, status = values.data_ptr(), scale.data_ptr(), _status(x)
+
+    def product(first: int, outs: int, bias):
+        y = torch.empty(*lead, outs, dtype=torch.bfloat16, device=x.device)
+        flags = 0
+        if bias is not None:
+            flags, bias = F_BIAS | (F_BIAS_F32 if bias.dtype is torch.float32 else 0), _dense(bias)
+        _launch("lvb_int8_gemm", y, q, q + first * ld, s, s + 4 * first, y.data_ptr(), rows, outs, cols, ld, ld, outs, flags, lib.ptr(bias), 0, 0, 0, 0, 0, status)
+        return y
+
+    if len(weights) > 1 and rows <= MANY_ROWS and all(b is None for b in biases):
+        sizes = [w.shape[0] for w in weights]
+        return product(rows, sum(sizes), None).split(sizes, dim=-1)
+    ys, first = [], rows
+    for w, b in zip(weights, biases):
+        ys.append(product(first, w.shape[0], b))
+        first += w.shape[0]
+    return tuple(ys)
 
 
 class _Int8ManyFn(torch.autograd.Function):
     """Projections of the same rows.  Kept for the backward pass: the rows and the weights in 8 bits, 1 byte per activation instead of 2, once for all projections.
 
     ``dx = sum dy w'`` and ``dw = dy^T x'`` are bf16 products of what the whole numbers stand for, rounded to bf16 (2^-9 of each value, as any operand
-    of a bf16 layer); output gradients are not quantised, their rows span too many magnitudes for one scale.  The sum over several projections is rounded once."""
+    of a bf16 layer); output gradients are not quantised, their rows span too many magnitudes for one scale.  The sum over several projections is rounded
+    once: of few rows their output gradients are laid side by side for one product each way, of many rows it is formed in fp32 (8192 rows of 4096 by two of
+    11008, us in a row of such steps: side by side 1375 to 1414, in fp32 1268 to 1313, rounding what the second product adds to 1158 to 1239)."""
 
     @staticmethod
     def forward(ctx, x, count, *tensors):
         weights, biases = tensors[:count], tensors[count:]
-        rows, *ws = _quantize_parts([x, *weights])
-        joint = _joint(ws) if count > 1 and rows.scale.numel() <= MANY_ROWS and not any(b is not None for b in biases) else None
-        if joint is not None:
-            ys = _product(rows, joint, out_dtype=x.dtype).split([w.shape[0] for w in weights], dim=-1)
-        else:
-            ys = tuple(_product(rows, w, b, out_dtype=x.dtype) for w, b in zip(ws, biases))
-        ctx.save_for_backward(rows.values, rows.scale, *[t for w in ws for t in w])
+        values, scale, ld = _hold(x, weights)
+        ctx.save_for_backward(values, scale)
         ctx.refs, ctx.bias_dtypes = weights, [None if b is None else b.dtype for b in biases]
-        ctx.x_shape = x.shape
+        ctx.x_shape, ctx.ld = x.shape, ld
         ctx.set_materialize_grads(False)  # a product that nothing uses has no gradient, and its weight none
-        return ys
+        return _held_products(x, values, scale, ld, weights, biases)
 
     @staticmethod
     def backward(ctx, *dys):
         from .gemm import _weight_grad, col_sum, gemm
 
-        values, scale, *flat = ctx.saved_tensors
-        n, cols = len(ctx.refs), values.shape[-1]
-        live = [i for i, dy in enumerate(dys) if dy is not None]
-        need_x = ctx.needs_input_grad[0]
-        need_w = [i for i in live if ctx.needs_input_grad[2 + i]]
-        need_b = [i for i in live if ctx.bias_dtypes[i] is not None and ctx.needs_input_grad[2 + n + i]]
-        dx, dws, dbs = None, [None] * n, [None] * n
+        values, scale = ctx.saved_tensors
+        refs, shape, ld = ctx.refs, ctx.x_shape, ctx.ld
+        n, cols = len(refs), shape[-1]
+        total, rows = values.shape[0], values.shape[0] - sum(w.shape[0] for w in refs)
+        need = ctx.needs_input_grad
+        live = [i for i in range(n) if dys[i] is not None]
+        dws, dbs = [None] * n, [None] * n
         if not live:
             return (None, None, *dws, *dbs)
-        d2 = {i: dys[i].reshape(-1, dys[i].shape[-1]) for i in live}
-        d2 = {i: d if d.dtype == torch.bfloat16 else d.to(torch.bfloat16) for i, d in d2.items()}
-        rows, ws = Int8Rows(values, scale), [Int8Rows(flat[2 * i], flat[2 * i + 1]) for i in live]
-        wanted = ([rows] if need_w else []) + (ws if need_x else [])
-        whole = _joint(wanted) if len(wanted) > 1 else None
-        if whole is not None:
-            counts = [r.scale.numel() for r in wanted]
-            back = list(whole.dequantize().split(counts))
-        else:
-            back = [r.dequantize().reshape(-1, cols) for r in wanted]
-        x2 = back.pop(0) if need_w else None
-        sizes = [d2[i].shape[1] for i in live]
-        side = None
-        if len(live) > 1 and scale.numel() <= MANY_ROWS:
-            side = torch.cat([d2[i] for i in live], dim=1)
-        if need_x:
+        d2 = [dys[i].reshape(rows, refs[i].shape[0]) for i in live]
+        d2 = [d if d.dtype is torch.bfloat16 else d.to(torch.bfloat16) for d in d2]
+        need_w = [i for i in live if need[2 + i]]
+        # what the rows in question stand for, in one launch: x, the weights or both
+        first, last = 0 if need_w else rows, total if need[0] else rows
+        back = torch.empty(last - first, cols, dtype=torch.bfloat16, device=values.device) if last > first else None
+        if back is not None:
+            _launch("lvb_int8_dequantize", values, values.data_ptr() + first * ld, ld, scale.data_ptr() + 4 * first, last - first, cols, back.data_ptr(), 0)
+        side = d2[0] if len(live) == 1 else torch.cat(d2, dim=1) if rows <= MANY_ROWS else None
+        dx = None
+        if need[0]:
+            w = back[rows - first:]
+            if len(live) < n or side is None:
+                ws = [p for i, p in enumerate(w.split([r.shape[0] for r in refs])) if i in live]
             if side is not None:
-                w = back[0].as_strided((sum(sizes), cols), (cols, 1)) if whole is not None else torch.cat(back)
-                dx = gemm(side, w, b_mn=True)
+                dx = gemm(side, w if len(live) == n else torch.cat(ws), b_mn=True)
             else:
-                for i, w in zip(live, back):
-                    dx = gemm(d2[i], w, b_mn=True, out=dx, accumulate=dx is not None, out_dtype=torch.bfloat16 if len(live) == 1 else torch.float32)
-            dx = dx.to(torch.bfloat16).view(ctx.x_shape)
-        plain = all(getattr(ctx.refs[i], "main_grad", None) is None and getattr(ctx.refs[i], "grad_sink", None) is None and ctx.refs[i].dtype == torch.bfloat16 for i in live)
-        if side is not None and need_w == live and plain:
-            for i, dw in zip(live, gemm(side, x2, a_mn=True, b_mn=True).split(sizes)):
-                dws[i] = dw
-        else:
-            for i in need_w:
-                dws[i] = _weight_grad(ctx.refs[i], d2[i], x2)
-        for i in need_b:
-            dbs[i] = col_sum(d2[i], ctx.bias_dtypes[i])
+                for d, w in zip(d2, ws):
+                    dx = gemm(d, w, b_mn=True, out=dx, accumulate=dx is not None, out_dtype=torch.float32)
+                dx = dx.to(torch.bfloat16)
+            dx = dx.view(shape)
+        if need_w:
+            x2 = back[:rows]
+            own = all(getattr(refs[i], "main_grad", None) is None and getattr(refs[i], "grad_sink", None) is None and refs[i].dtype is torch.bfloat16 for i in live)
+            if len(live) > 1 and side is not None and need_w == live and own:
+                for i, dw in zip(live, gemm(side, x2, a_mn=True, b_mn=True).split([refs[i].shape[0] for i in live])):
+                    dws[i] = dw
+            else:
+                for i, d in zip(live, d2):
+                    if need[2 + i]:
+                        dws[i] = _weight_grad(refs[i], d, x2)
+        for i, d in zip(live, d2):
+            if ctx.bias_dtypes[i] is not None and need[2 + n + i]:
+                dbs[i] = col_sum(d, ctx.bias_dtypes[i])
         return (dx, None, *dws, *dbs)
 
 
@@ -436,8 +451,7 @@ def int8_linear_many(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: O
 
     if _kernels(x) and x.dtype == torch.bfloat16 and x.numel() and all(w.dtype == torch.bfloat16 and _tma_shapes_ok(w) and w.shape[0] > 0 for w in weights):
         if lib.plain_call():
-            rows, *ws = _quantize_parts([x, *weights])
-            return tuple(_product(rows, w, b) for w, b in zip(ws, biases))
+            return _held_products(x, *_hold(x, weights), weights, biases)
         return _Int8ManyFn.apply(x, len(weights), *weights, *biases)
     x8 = _straight_through(x)
     return tuple(F.linear(x8, _straight_through(w).to(x.dtype), None if b is None else b.to(x.dtype)) for w, b in zip(weights, biases))
