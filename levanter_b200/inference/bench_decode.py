@@ -120,6 +120,7 @@ def main(argv=None):
     ap.add_argument("--tp", type=int, default=1, help="tensor-parallel ranks (launch with torchrun, one rank per GPU)")
     ap.add_argument("--prompt-min", type=int, default=0, help="with --prompt-max: prompt lengths uniform in [min, max]")
     ap.add_argument("--prompt-max", type=int, default=0)
+    ap.add_argument("--int8", action="store_true", help="hold the weights of attention and MLP layers in 8 bits")
     ap.add_argument("--quiet", action="store_true", help="return the result without printing it")
     a = ap.parse_args(argv)
     return run(a)
@@ -129,6 +130,7 @@ def run(a):
     import os
 
     from ..data.passthrough_tokenizer import PassthroughTokenizer
+    from ..quantization import QuantizationConfig
     from .engine import InferenceEngine, InferenceEngineConfig, Request
     from .jit_scheduler import SeqDecodingParams
 
@@ -168,7 +170,8 @@ def run(a):
     pages_per_seq = -(-total_len // a.page_size) + 1
     ecfg = InferenceEngineConfig(max_pages=a.seqs * pages_per_seq + 8, max_seqs=a.seqs, page_size=a.page_size, max_pages_per_seq=pages_per_seq,
                                  compute_dtype=dtype, max_seqs_in_prefill=min(a.seqs, 16), max_prefill_size=16 * prompt_max,
-                                 max_rounds=a.max_rounds, use_cuda_graph=a.cuda_graph)
+                                 max_rounds=a.max_rounds, use_cuda_graph=a.cuda_graph,
+                                 quantization=QuantizationConfig(int8=True) if getattr(a, "int8", False) else None)
     engine = InferenceEngine.from_model_with_config(model, PassthroughTokenizer(vocab), ecfg)
     rng = np.random.default_rng(0)
 
@@ -225,7 +228,7 @@ def run(a):
     out = {"metric": f"decode tokens/s (engine.generate, {a.tp} GPU{'s, tensor parallel' if a.tp > 1 else ''})", "model": a.model, "seqs": a.seqs,
            "prompt_len": a.prompt_len if not a.prompt_max else [prompt_min, prompt_max], "tp": a.tp,
            "kernel_all_reduces": None if tp is None else tp.kernel_all_reduces,
-           "new_tokens": a.new_tokens, "page_size": a.page_size, "cuda_graph": bool(a.cuda_graph), "max_rounds": a.max_rounds, "dtype": str(dtype),
+           "new_tokens": a.new_tokens, "page_size": a.page_size, "cuda_graph": bool(a.cuda_graph), "max_rounds": a.max_rounds, "dtype": str(dtype), "int8_weights": bool(getattr(a, "int8", False)),
            "prefill_tokens_per_s": round(best["prefill_tokens"] / max(best["prefill_seconds"], 1e-9), 1),
            "decode_tokens_per_s": round(best["decode_tokens"] / max(best["decode_seconds"], 1e-9), 1),
            "end_to_end_generated_tokens_per_s": round(best["generated"] / best["wall_s"], 1),

@@ -26,6 +26,7 @@ import torch
 
 from ..layers.attention import KvPageCache
 from ..layers.sampler import Sampler
+from ..quantization import QuantizationConfig, quantize_for_serving
 from .jit_scheduler import DecodeState, SeqDecodingParams, _DecodeOutputs
 from .page_table import PageBatchInfo, PageTable
 from .utils import INVALID, is_valid
@@ -70,6 +71,7 @@ class InferenceEngineConfig:
     seed: int = 0
     enable_logprobs: bool = False
     use_cuda_graph: bool = False  # capture the decode call (fixed shapes) and replay it
+    quantization: Optional[QuantizationConfig] = None  # {int8: true}: attention and MLP weights in 8 bits, their inputs quantised token by token
 
     @property
     def imputed_max_pages(self) -> int:
@@ -192,6 +194,8 @@ class InferenceEngine:
 
     @classmethod
     def from_model_with_config(cls, model, tokenizer, config: InferenceEngineConfig) -> "InferenceEngine":
+        if config.quantization is not None:
+            model = quantize_for_serving(model, config.quantization)
         table = PageTable.init(config.imputed_max_pages, config.max_seqs, config.page_size, config.max_pages_per_seq)
         try:
             device = next(model.parameters()).device

@@ -376,6 +376,8 @@ def dot_product_attention_with_sink(q, k, v, sink: torch.Tensor, mask=None, bias
 
 # --------------------------------------------------------------------------------------------- module
 from ..nn import FusedRows, Linear, RmsNorm, linear_many, plain  # noqa: E402  (after function definitions to keep the file readable)
+from ..ops.int8 import Int8Rows, Int8ServingLinear, as_int8_rows, int8_product  # noqa: E402
+from ..ops.int8 import Int8Rows, Int8ServingLinear, as_int8_rows, int8_product
 
 
 @dataclass(frozen=True)
@@ -490,8 +492,13 @@ class Attention(nn.Module):
         rows = sum(m.weight.shape[0] for m in self._projections())
         pad = -rows % 8  # whole groups of 8 columns keep the slices of the joint product aligned
         self._rows, self._bias_rows = FusedRows(pad), FusedRows(pad + (self.local_heads if c.head_gate else 0))
+        self._scale_rows = FusedRows(pad)
 
     difference_names = ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2")
+
+    def row_readers(self):
+        """The projections that read this layer's input rows."""
+        return self._projections()
 
     def _projections(self):
         return [self.q_proj, self.k_proj, self.v_proj] + ([self.g_proj] if self.config.output_gate or self.config.head_gate else [])
@@ -501,7 +508,8 @@ class Attention(nn.Module):
         c = self.config
         D = c.head_size
         lead = x.shape[:-1]
-        self._rows.hold([m.weight for m in (self.q_proj, self.k_proj, self.v_proj) if type(m) is Linear])
+        self._rows.hold([m.weight for m in (self.q_proj, self.k_proj, self.v_proj) if type(m) in (Linear, Int8ServingLinear)])
+        self._scale_rows.hold([m.weight_scale for m in (self.q_proj, self.k_proj, self.v_proj) if type(m) is Int8ServingLinear])
         q, k, v = linear_many(x, self.q_proj, self.k_proj, self.v_proj)
         q, k, v = q.view(*lead, c.maps * self.local_heads, D), k.view(*lead, c.maps * self.local_kv, D), v.view(*lead, self.local_kv, c.v_head_size)
         if self.q_norm is not None:
@@ -634,6 +642,8 @@ class Attention(nn.Module):
                 from ..ops.gemm import linear_residual
 
                 return linear_residual(out, self.o_proj.weight, self.o_proj.bias, residual), kv_cache
+            if plain(self.o_proj, Int8ServingLinear):
+                return self.o_proj(out, residual=residual), kv_cache
             return self.o_proj(out) + residual, kv_cache
         return self.o_proj(out), kv_cache
 
@@ -658,8 +668,11 @@ class Attention(nn.Module):
     def lay_out_for_serving(self) -> None:
         """Lays the projections' weights side by side where serving steps of a few rows read them as one matrix.  Done with the cache, before a step
         or a CUDA graph knows where they lie; what was taken from the parameters before (a ``state_dict``) keeps the values and no longer follows them."""
-        if self.q_norm is None and self._plain_pages() and self._prepared_heads() and all(type(m) is Linear and m.weight.is_cuda for m in self._projections()):
-            self._fused_projection(build=True)
+        if self.q_norm is None and self._plain_pages() and self._prepared_heads():
+            if all(type(m) is Linear and m.weight.is_cuda for m in self._projections()):
+                self._fused_projection(build=True)
+            elif all(type(m) is Int8ServingLinear for m in self._projections()):
+                self._fused_int8(build=True)
 
     def _project_and_prepare(self, x, kv_cache: "KvPageCache", batch_info, pos_ids):
         """``q, k, v`` rows as attention reads them (for a few rows slices of the joint product's rows), keys and values written to the pages."""
@@ -669,10 +682,11 @@ class Attention(nn.Module):
 
         D = self.config.head_size
         nq, nk = self.local_heads * D, self.local_kv * D
-        fused = self._fused_projection() if (x.shape[0] <= DECODE_ROWS and self.q_norm is None and not self.training
-                                             and all(plain(m, Linear) for m in self._projections())) else None
-        if fused is not None:
-            y = project(x, fused[0], bias=fused[1])
+        few = x.shape[0] <= DECODE_ROWS and self.q_norm is None and not self.training
+        fused = self._fused_projection() if few and all(plain(m, Linear) for m in self._projections()) else None
+        held = self._fused_int8() if few and all(plain(m, Int8ServingLinear) for m in self._projections()) else None
+        if fused is not None or held is not None:
+            y = project(x, fused[0], bias=fused[1]) if held is None else int8_product(as_int8_rows(x), held[0], held[1])
             q, k, v = y[:, :nq].unflatten(1, (-1, D)), y[:, nq:nq + nk].unflatten(1, (-1, D)), y[:, nq + nk:nq + 2 * nk].unflatten(1, (-1, D))
         else:
             q, k, v = self._compute_qkv(x, pos_ids, rotate=False)
@@ -695,6 +709,16 @@ class Attention(nn.Module):
         w = self._rows.get([m.weight for m in mods], build)
         b = self._bias_rows.get([m.bias for m in with_bias], build) if w is not None and biased[0] else None
         return None if w is None or (biased[0] and b is None) else (w, b)
+
+    def _fused_int8(self, build: bool = False):
+        """:meth:`_fused_projection` of projections whose weights are held in 8 bits: ``(rows of the joint weight, bias or None)``, or None."""
+        mods = self._projections()
+        biased = [m.bias is not None for m in mods]
+        if any(biased) != all(biased) or mods[0].in_features % 16 != 0:
+            return None
+        w, s = self._rows.get([m.weight for m in mods], build), self._scale_rows.get([m.weight_scale for m in mods], build)
+        b = self._bias_rows.get([m.bias for m in mods], build) if biased[0] else None
+        return None if w is None or s is None or (biased[0] and b is None) else (Int8Rows(w, s), b)
 
     def _paged_heads(self, x, kv_cache: "KvPageCache", batch_info, pos_ids, v_first: Optional[torch.Tensor] = None):
         """``(heads, v_first)``: the (gated) concatenated heads ``[T, heads * v_head_size]`` of packed tokens, for the forms of attention

@@ -21,9 +21,10 @@ from ..compat.hf_checkpoints import HFCheckpointConverter, HFCompatConfig
 from ..layers.attention import DECODE_ROWS, Attention, AttentionBackend, AttentionConfig, AttentionMask, KvPageCache
 from ..layers.normalization import LayerNormConfigBase, RmsNormConfig
 from ..layers.rotary import rope_config_from_hf, rope_to_hf_dict, DefaultRotaryEmbeddingsConfig, RotaryEmbeddingsConfig
-from ..nn import Embedding, FusedRows, Linear, fork_norm, linear_many, plain
+from ..nn import Embedding, FusedRows, Linear, fork_norm, linear_many, norm_for, plain
 from ..ops.gemm import linear_residual
 from ..ops.glu import ClampedGlu, GatedActivation, gated_activation
+from ..ops.int8 import Int8Rows, Int8ServingLinear, as_int8_rows, gated_activation_int8, int8_product
 from ..ops.residual_stream import add_linear, glu_of_rows, project
 from ..utils.activation import ActivationFunctionEnum
 from ..utils.flop_utils import lm_flops_per_token
@@ -162,11 +163,18 @@ class LlamaMlp(nn.Module):
         self.up_proj = Linear(hidden, local, bias=use_bias, init_std=init_std, parallel=("column", tp))
         self.down_proj = Linear(local, hidden, bias=use_bias, init_std=init_std, parallel=("row", tp))
         self.act = activation if isinstance(activation, (ActivationFunctionEnum, ClampedGlu)) else ActivationFunctionEnum(activation)
-        self._rows = FusedRows()
+        self._rows, self._scales = FusedRows(), FusedRows()
+
+    def row_readers(self):
+        """The projections that read this layer's input rows."""
+        return self.gate_proj, self.up_proj
 
     def lay_out_for_serving(self) -> None:
         """Lays gate and up side by side for serving steps of a few rows, as the attention layer does with its projections."""
         mods = (self.gate_proj, self.up_proj)
+        if all(type(m) is Int8ServingLinear and m.bias is None and m.in_features % 16 == 0 for m in mods):
+            self._rows.get([m.weight for m in mods])
+            self._scales.get([m.weight_scale for m in mods])
         if all(type(m) is Linear and m.bias is None and m.weight.is_cuda and m.weight.dtype == torch.bfloat16 for m in mods):
             self._rows.get([m.weight for m in mods])
 
@@ -195,7 +203,22 @@ class LlamaMlp(nn.Module):
             return add_linear(stream, h, self.down_proj.weight)
         return stream + self.down_proj(h).float()
 
+    def _int8(self, x, residual: Optional[torch.Tensor]) -> torch.Tensor:
+        """The MLP on weights held in 8 bits: every row is quantised where it is made, gate and up are one product where they lie side by side."""
+        mods = (self.gate_proj, self.up_proj)
+        rows, shared = as_int8_rows(x), all(m.bias is None for m in mods)
+        weight = self._rows.get([m.weight for m in mods], build=False) if shared else None
+        scale = self._scales.get([m.weight_scale for m in mods], build=False) if shared else None
+        if weight is not None and scale is not None:
+            y, ff = int8_product(rows, Int8Rows(weight, scale), out_dtype=x.dtype), self.gate_proj.out_features
+            gate, up = y[..., :ff], y[..., ff:]
+        else:
+            gate, up = self.gate_proj(rows), self.up_proj(rows)
+        return self.down_proj(gated_activation_int8(gate, up, self.act), residual=residual)
+
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if all(plain(m, Int8ServingLinear) for m in (self.gate_proj, self.up_proj, self.down_proj)):
+            return self._int8(x, residual)
         if self.tp is not None and self.tp.size > 1:
             x = self.tp.copy_to_region(x)
         if x.dim() == 2 and x.shape[0] <= DECODE_ROWS and not torch.is_grad_enabled() and x.dtype == self.gate_proj.weight.dtype == torch.bfloat16:
@@ -260,19 +283,19 @@ class LlamaDecoderLayer(nn.Module):
         return self.mlp(h, residual=x)
 
     def decode(self, x, kv_cache: KvPageCache, batch_info, pos_ids):
-        h = self.input_layernorm(x)
+        h, x = norm_for(self.input_layernorm, x, self.self_attn.row_readers())
         tp_on = self.tp is not None and self.tp.size > 1
         if not tp_on and self.post_attn_layernorm is None:
             # both residual adds ride in the epilogues of the output and down projections
             x, kv_cache = self.self_attn.paged_decode(h, kv_cache, batch_info, pos_ids, residual=x)
+            attn_out = None
         else:
             attn_out, kv_cache = self.self_attn.paged_decode(h, kv_cache, batch_info, pos_ids)
             if tp_on:
                 attn_out = self.tp.all_reduce(attn_out)
             if self.post_attn_layernorm is not None:
                 attn_out = self.post_attn_layernorm(attn_out)
-            x = x + attn_out
-        h = self.post_attention_layernorm(x)
+        h, x = norm_for(self.post_attention_layernorm, x, self.mlp.row_readers() if isinstance(self.mlp, LlamaMlp) else (), residual=attn_out)
         if self.post_mlp_layernorm is None:
             return self.mlp(h, residual=x), kv_cache
         return x + self.post_mlp_layernorm(self.mlp(h)), kv_cache

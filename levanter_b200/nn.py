@@ -269,13 +269,31 @@ def fork_norm(norm: nn.Module, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Ten
 def linear_many(x: torch.Tensor, *projections: nn.Module):
     """The projections of the same rows, one by one; in training their input gradients are summed in the epilogues of their products."""
     from .ops.gemm import linear_many as many
+    from .ops.int8 import Int8Linear, Int8ServingLinear, as_int8_rows, int8_linear_many
 
-    if x.requires_grad and torch.is_grad_enabled() and all(plain(m, Linear) and m.bias is None and getattr(m.weight, "grad_sink", None) is None
+    if all(plain(m, Int8ServingLinear) for m in projections):
+        x = as_int8_rows(x)  # once for all of them
+    elif all(plain(m, Int8Linear) for m in projections):
+        return int8_linear_many(x, [m.operand(x.dtype) for m in projections], [m.bias for m in projections])
+    elif x.requires_grad and torch.is_grad_enabled() and all(plain(m, Linear) and m.bias is None and getattr(m.weight, "grad_sink", None) is None
                                                           for m in projections):
         got = many(x, [m.weight for m in projections])
         if got is not None:
             return got
     return tuple(m(x) for m in projections)
+
+
+def norm_for(norm: nn.Module, x: torch.Tensor, projections: Sequence[nn.Module] = (), residual: Optional[torch.Tensor] = None):
+    """``(norm(h), h)`` of ``h = x + residual`` (no residual: of ``x``) for the projections that read it: as 8-bit rows where all of them hold their weights in
+    8 bits, made in the norm's own pass with the residual's addition."""
+    from .ops.int8 import Int8ServingLinear, rms_norm_int8
+
+    if x.dtype == torch.bfloat16 and not torch.is_grad_enabled() and plain(norm, RmsNorm) and norm.bias is None and len(projections) > 0 and all(
+            plain(m, Int8ServingLinear) for m in projections):
+        rows, h = rms_norm_int8(x, norm.weight, norm.eps, residual=residual)
+        return rows, x if h is None else h
+    h = x if residual is None else x + residual
+    return norm(h), h
 
 
 class Dropout(nn.Module):

@@ -46,6 +46,14 @@ class Int8Rows(NamedTuple):
     def device(self) -> torch.device:
         return self.values.device
 
+    # what a layer asks of the rows that it is given, whichever they are: a serving step's rows are bf16 ones
+    dtype = property(lambda self: torch.bfloat16)
+    is_cuda = property(lambda self: self.values.is_cuda)
+    requires_grad = property(lambda self: False)
+
+    def dim(self) -> int:
+        return self.values.dim()
+
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """What the rows stand for, ``values * scale`` rounded once to ``dtype`` (bf16 or fp32)."""
         v, s = self
@@ -460,3 +468,77 @@ def int8_linear_many(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: O
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`int8_linear_many` of one projection."""
     return int8_linear_many(x, [weight], [bias])[0]
+
+
+# ------------------------------------------------------------------------------------------------ modules
+class Int8Linear(nn.Module):
+    """Drop-in for :class:`levanter_b200.nn.Linear` that trains on :func:`int8_linear`: it owns the same ``weight`` and ``bias`` parameters; master weights,
+    optimizer state and checkpoints are unchanged."""
+
+    def __init__(self, weight: nn.Parameter, bias: Optional[nn.Parameter]):
+        super().__init__()
+        self.weight, self.bias = weight, bias
+        self.in_features, self.out_features = weight.shape[1], weight.shape[0]
+
+    @staticmethod
+    def from_linear(linear: nn.Module) -> "Int8Linear":
+        return Int8Linear(linear.weight, getattr(linear, "bias", None))
+
+    def operand(self, dtype: torch.dtype) -> torch.Tensor:
+        """The weight in ``dtype``; a converted one passes its gradient on to the buffer that the weight names."""
+        w = self.weight
+        if w.dtype == dtype:
+            return w
+        w = w.to(dtype)
+        for name in ("main_grad", "grad_sink"):
+            if hasattr(self.weight, name):
+                setattr(w, name, getattr(self.weight, name))
+        return w
+
+    def forward(self, x: torch.Tensor, *, skip_bias: bool = False) -> torch.Tensor:
+        return int8_linear(x, self.operand(x.dtype), None if skip_bias else self.bias)
+
+    def extra_repr(self):
+        return f"in={self.in_features}, out={self.out_features}, bias={self.bias is not None}, int8"
+
+
+class Int8ServingLinear(nn.Module):
+    """A projection that serves: its weights are held in 8 bits (buffers ``weight`` int8 ``[out, in]`` and ``weight_scale`` fp32 ``[out]``) and have no gradient.
+    It takes rows in bf16 or fp32, or :class:`Int8Rows` that several projections share, and adds a ``residual`` in its product's epilogue."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor]):
+        super().__init__()
+        if weight.dim() != 2 or weight.dtype not in _FLOATS or not 0 < weight.shape[1] <= MAX_COLS:
+            raise ValueError(f"a weight [out, in] in bf16 or fp32 with up to {MAX_COLS} columns expected, got {tuple(weight.shape)} {weight.dtype}")
+        self.out_features, self.in_features = weight.shape
+        self.dtype = weight.dtype
+        rows = _quantize(weight.detach())
+        self.register_buffer("weight", rows.values)
+        self.register_buffer("weight_scale", rows.scale)
+        self.register_buffer("bias", None if bias is None else bias.detach())
+
+    @staticmethod
+    def from_linear(linear: nn.Module) -> "Int8ServingLinear":
+        return Int8ServingLinear(linear.weight, getattr(linear, "bias", None))
+
+    @property
+    def rows(self) -> Int8Rows:
+        return Int8Rows(self.weight, self.weight_scale)
+
+    def _apply(self, fn, recurse=True):
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:  # a model's conversion to another type leaves the scales as they are
+            self.weight_scale = scale.to(self.weight.device)
+        return self
+
+    def forward(self, x: Union[torch.Tensor, Int8Rows], *, skip_bias: bool = False, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        out = self.dtype if isinstance(x, Int8Rows) else x.dtype
+        return int8_product(as_int8_rows(x), self.rows, None if skip_bias else self.bias, residual, out_dtype=out)
+
+    def extra_repr(self):
+        return f"in={self.in_features}, out={self.out_features}, bias={self.bias is not None}, int8 weights"
+
+
+def as_int8_rows(x: Union[torch.Tensor, Int8Rows]) -> Int8Rows:
+    return x if isinstance(x, Int8Rows) else quantize_rows(x)

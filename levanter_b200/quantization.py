@@ -6,8 +6,11 @@ e5m2 for output gradients.  ``scaling: tensor`` (default) uses one scale per ten
 maxima (delayed scaling, as in the reference); ``scaling: block`` uses one power-of-two scale per 32 values along the
 contraction dimension, applied by the tensor core (``tcgen05.mma kind::mxf8f6f4.block_scale``).  ``block_size`` is accepted
 for configs that name it; the hardware's block is 32 whatever it says.
-``quantize_linear_layers`` swaps matching ``Linear`` modules for ``Fp8Linear``;
-master weights, optimizer state and checkpoints are unchanged."""
+``int8: true`` selects 8-bit integer products for the forward pass (``ops/int8.py``): one scale per token and per output channel, taken from the values
+themselves, gradients from bf16 products, activations kept for the backward pass in 8 bits.
+``quantize_linear_layers`` swaps matching ``Linear`` modules for ``Fp8Linear`` or ``Int8Linear``;
+master weights, optimizer state and checkpoints are unchanged.
+``quantize_for_serving`` replaces the projections of attention and MLP layers by ones that hold their weights in 8 bits (``int8: true``)."""
 from __future__ import annotations
 
 import re
@@ -43,18 +46,47 @@ class QuantizationConfig:
 
 
 def quantize_linear_layers(model: nn.Module, config: QuantizationConfig) -> nn.Module:
-    """Replace targeted ``Linear`` modules by their fp8 counterparts (in place; returns the model)."""
+    """Replace targeted ``Linear`` modules by their fp8 or int8 counterparts (in place; returns the model)."""
     if not (config.fp8 or config.int8):
         return model
-    if config.int8:
-        raise NotImplementedError("int8 training is not supported; use fp8")
     from .nn import Linear
     from .ops.fp8 import Fp8Linear
+    from .ops.int8 import Int8Linear
 
     for name, mod in list(model.named_modules()):
         for child_name, child in list(mod.named_children()):
             full = f"{name}.{child_name}" if name else child_name
             if type(child) is Linear and config.matches(full) and "lm_head" not in full:
+                if config.int8:
+                    setattr(mod, child_name, Int8Linear.from_linear(child))
+                    continue
                 setattr(mod, child_name, Fp8Linear.from_linear(child, block=config.block_size, amax_history_length=config.amax_history_length,
                                                                      block_scaled=config.scaling == "block"))
+    return model
+
+
+def quantize_for_serving(model: nn.Module, config: QuantizationConfig) -> nn.Module:
+    """Hold the weights of the targeted projections of attention and MLP layers in 8 bits, one scale per output channel (in place; returns the model).  The
+    model serves from then on: those weights are not parameters any more.  A model that is quantised already comes back as it is."""
+    if config.fp8:
+        raise ValueError("serving holds weights in 8-bit integers: use QuantizationConfig(int8=True)")
+    if not config.int8:
+        return model
+    from .layers.attention import Attention
+    from .models.llama import LlamaMlp
+    from .nn import Linear
+    from .ops.int8 import Int8Linear, Int8ServingLinear
+
+    held = 0
+    for name, mod in list(model.named_modules()):
+        if not isinstance(mod, (Attention, LlamaMlp)):
+            continue
+        if mod.tp is not None and mod.tp.size > 1:
+            raise ValueError(f"{name}: int8 serving weights are not split over tensor-parallel ranks")
+        for child_name, child in list(mod.named_children()):
+            if type(child) in (Linear, Int8Linear) and config.matches(f"{name}.{child_name}"):
+                setattr(mod, child_name, Int8ServingLinear.from_linear(child))
+            held += type(getattr(mod, child_name)) is Int8ServingLinear
+    if held == 0:
+        raise ValueError("no projection of an attention or MLP layer matches the quantization targets")
     return model

@@ -1,0 +1,218 @@
+"""8-bit integer layers on the CPU: the definition of the rows, refusals, training through the layers, serving through the engine."""
+import copy
+
+import pytest
+import torch
+
+from levanter_b200.nn import Linear, RmsNorm, linear_many, norm_for
+from levanter_b200.ops import int8 as I
+from levanter_b200.quantization import QuantizationConfig, quantize_for_serving, quantize_linear_layers
+from levanter_b200.utils.activation import ActivationFunctionEnum as Act
+
+BF = torch.bfloat16
+
+
+def llama(**kw):
+    from levanter_b200.models.llama import LlamaConfig
+
+    cfg = dict(seq_len=64, hidden_dim=64, intermediate_dim=128, num_layers=2, num_heads=4, num_kv_heads=2, gradient_checkpointing=False)
+    return LlamaConfig(**{**cfg, **kw})
+
+
+def test_rows_and_back():
+    torch.manual_seed(0)
+    x = torch.randn(5, 3, 70) * torch.logspace(-3, 3, 3)[:, None]
+    rows = I.quantize_rows(x)
+    assert rows.shape == x.shape and rows.scale.shape == (5, 3) and rows.values.stride(1) % 16 == 0
+    top = x.abs().amax(-1, keepdim=True)
+    assert ((rows.dequantize(torch.float32) - x).abs() <= top / 254 * (1 + 1e-5)).all()
+    assert (rows.values.abs().amax(-1) == 127).all()
+
+
+def test_ties_go_to_the_even_number():
+    x = torch.tensor([[127.0, 63.5, 0.5, 1.5, 2.5, -0.5, -1.5, -126.5], [1.0, 0.5, -0.5, 0, 0, 0, 0, 0]])
+    assert I.quantize_rows(x).values.tolist() == [[127, 64, 0, 2, 2, 0, -2, -126], [127, 64, -64, 0, 0, 0, 0, 0]]
+
+
+def test_special_rows():
+    x = torch.zeros(5, 8)
+    x[1, 2] = 1e-31
+    x[2, 3] = float("nan")
+    x[3, 4] = -float("inf")
+    x[4, 5] = 2.0
+    rows = I.quantize_rows(x)
+    assert rows.scale[:2].tolist() == [0, 0] and rows.scale[2:4].isnan().all() and not rows.values[:4].any() and rows.values[4, 5] == 127
+
+
+def test_norm_with_its_residual_and_gated_activation():
+    torch.manual_seed(1)
+    x, r, w = torch.randn(6, 48).to(BF), torch.randn(6, 48).to(BF), (1 + 0.1 * torch.randn(48)).to(BF)
+    rows, h = I.rms_norm_int8(x, w, 1e-5, residual=r)
+    assert torch.equal(h, (x.float() + r.float()).to(BF))
+    y = h.float() * torch.rsqrt(h.float().square().mean(-1, keepdim=True) + 1e-5) * w.float()
+    assert ((rows.dequantize(torch.float32) - y).abs() <= y.abs().amax(-1, keepdim=True) / 254 * (1 + 1e-5)).all()
+    assert I.rms_norm_int8(x, None)[1] is None
+    y = torch.nn.functional.silu(x.float()) * r.float()
+    assert ((I.gated_activation_int8(x, r, "silu").dequantize(torch.float32) - y).abs() <= y.abs().amax(-1, keepdim=True) / 254 * (1 + 1e-5)).all()
+
+
+def test_product_is_exact_in_whole_numbers():
+    torch.manual_seed(2)
+    a = I.Int8Rows(torch.randint(-128, 128, (4, 300), dtype=torch.int8), torch.ones(4))
+    b = I.Int8Rows(torch.randint(-128, 128, (7, 300), dtype=torch.int8), torch.ones(7))
+    bias, res = torch.randn(7), torch.randn(4, 7)
+    want = (a.values.long() @ b.values.long().t()).float()
+    assert torch.equal(I.int8_product(a, b, out_dtype=torch.float32), want)
+    assert torch.equal(I.int8_product(a, b, bias, res, out_dtype=torch.float32), want + bias + res)
+
+
+@pytest.mark.parametrize("call, error", [
+    (lambda x, w: I.quantize_rows(x.half()), TypeError),
+    (lambda x, w: I.quantize_rows(x.int()), TypeError),
+    (lambda x, w: I.quantize_rows(torch.tensor(1.0)), ValueError),
+    (lambda x, w: I.quantize_rows(torch.zeros(3, 0)), ValueError),
+    (lambda x, w: I.quantize_rows(x.clone().requires_grad_()), RuntimeError),
+    (lambda x, w: I.quantize_rows(x).dequantize(torch.float16), TypeError),
+    (lambda x, w: I.rms_norm_int8(x, torch.ones(7)), ValueError),
+    (lambda x, w: I.rms_norm_int8(x, torch.ones(1, 16)), ValueError),
+    (lambda x, w: I.rms_norm_int8(x, torch.ones(16).half()), ValueError),
+    (lambda x, w: I.rms_norm_int8(x, torch.ones(16), residual=x[:2]), ValueError),
+    (lambda x, w: I.rms_norm_int8(x, torch.ones(16), residual=x.to(BF)), ValueError),
+    (lambda x, w: I.rms_norm_int8(x, torch.ones(16, requires_grad=True)), RuntimeError),
+    (lambda x, w: I.gated_activation_int8(x, x[:, :8], Act.silu), ValueError),
+    (lambda x, w: I.gated_activation_int8(x, x.to(BF), Act.silu), ValueError),
+    (lambda x, w: I.gated_activation_int8(x, x, "no such thing"), ValueError),
+    (lambda x, w: I.int8_product(I.Int8Rows(x, torch.ones(4)), w), TypeError),
+    (lambda x, w: I.int8_product(I.Int8Rows(w.values, w.scale.double()), w), TypeError),
+    (lambda x, w: I.int8_product(I.Int8Rows(w.values, w.scale[:3]), w), ValueError),
+    (lambda x, w: I.int8_product(I.Int8Rows(w.values[:, :8], w.scale), w), ValueError),
+    (lambda x, w: I.int8_product(w, I.Int8Rows(w.values[0], w.scale[0])), ValueError),
+    (lambda x, w: I.int8_product(w, w, bias=torch.ones(5)), ValueError),
+    (lambda x, w: I.int8_product(w, w, bias=torch.ones(4).half()), ValueError),
+    (lambda x, w: I.int8_product(w, w, residual=torch.ones(4, 5)), ValueError),
+    (lambda x, w: I.int8_product(w, w, residual=torch.ones(4, 4, requires_grad=True)), RuntimeError),
+    (lambda x, w: I.int8_product(w, w, out_dtype=torch.float16), TypeError),
+    (lambda x, w: I.int8_product(I.Int8Rows(torch.zeros(1, I.MAX_COLS + 1, dtype=torch.int8), torch.ones(1)),
+                                 I.Int8Rows(torch.zeros(1, I.MAX_COLS + 1, dtype=torch.int8), torch.ones(1))), ValueError),
+    (lambda x, w: I.int8_linear_many(x, []), ValueError),
+    (lambda x, w: I.int8_linear_many(x, [torch.ones(3, 16)], []), ValueError),
+    (lambda x, w: I.int8_linear(x, torch.ones(3, 17)), ValueError),
+    (lambda x, w: I.int8_linear(x, torch.ones(3, 16), torch.ones(4)), ValueError),
+    (lambda x, w: I.int8_linear(x.double(), torch.ones(3, 16)), TypeError),
+    (lambda x, w: I.Int8ServingLinear(torch.ones(3, 16).half(), None), ValueError),
+    (lambda x, w: quantize_for_serving(Linear(8, 8), QuantizationConfig(int8=True)), ValueError),
+    (lambda x, w: quantize_for_serving(Linear(8, 8), QuantizationConfig(fp8=True)), ValueError),
+])
+def test_refusals(call, error):
+    torch.manual_seed(3)
+    with pytest.raises(error):
+        call(torch.randn(4, 16), I.quantize_rows(torch.randn(4, 16)))
+
+
+def test_gradients_are_those_of_the_product_of_what_is_held():
+    torch.manual_seed(4)
+    x, w, b = torch.randn(2, 5, 24), torch.randn(7, 24), torch.randn(7)
+    x, w, b = (t.requires_grad_() for t in (x, w, b))
+    dy = torch.randn(2, 5, 7)
+    y = I.int8_linear(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], dy)
+    xh, wh = (I.quantize_rows(t.detach()).dequantize(torch.float32) for t in (x, w))
+    torch.testing.assert_close(y, xh @ wh.t() + b, atol=2e-5, rtol=1e-5)
+    torch.testing.assert_close(gx, dy @ wh, atol=2e-5, rtol=1e-5)
+    torch.testing.assert_close(gw, dy.flatten(0, 1).t() @ xh.flatten(0, 1), atol=2e-5, rtol=1e-5)
+    torch.testing.assert_close(gb, dy.sum((0, 1)), atol=2e-5, rtol=1e-5)
+
+
+def test_quantize_linear_layers_trains_in_int8_under_the_same_names():
+    from levanter_b200.models.lm_model import LmExample, compute_next_token_loss
+
+    model = llama().build(100, seed=0)
+    names = [n for n, _ in model.named_parameters()]
+    plain = copy.deepcopy(model)
+    quantize_linear_layers(model, QuantizationConfig(int8=True))
+    assert [n for n, _ in model.named_parameters()] == names
+    assert sum(isinstance(m, I.Int8Linear) for m in model.modules()) == 2 * 7 and type(model.lm_head) is Linear
+    ex = LmExample.causal(torch.randint(0, 100, (2, 64), dtype=torch.int32))
+    loss, want = compute_next_token_loss(model, ex), compute_next_token_loss(plain, ex)
+    assert abs(loss.item() - want.item()) < 0.02
+    loss.backward()
+    want.backward()
+    for (n, p), q in zip(model.named_parameters(), plain.parameters()):
+        assert (p.grad - q.grad).norm() <= 0.2 * q.grad.norm() + 1e-6, n
+
+
+def test_targets_choose_the_layers():
+    model = quantize_linear_layers(llama().build(100, seed=0), QuantizationConfig(int8=True, targets="mlp"))
+    assert isinstance(model.transformer.layers[0].mlp.gate_proj, I.Int8Linear) and type(model.transformer.layers[0].self_attn.q_proj) is Linear
+    model = quantize_for_serving(llama().build(100, seed=0), QuantizationConfig(int8=True, targets=["down_proj"]))
+    assert sum(isinstance(m, I.Int8ServingLinear) for m in model.modules()) == 2
+
+
+def test_one_quantisation_for_all_readers(monkeypatch):
+    calls = []
+    monkeypatch.setattr(I, "_quantize", lambda x, real=I._quantize: calls.append(1) or real(x))
+    mods = [I.Int8ServingLinear(torch.randn(n, 32), torch.randn(n) if n == 8 else None) for n in (8, 16, 4)]
+    calls.clear()
+    x = torch.randn(3, 32)
+    with torch.no_grad():
+        ys = linear_many(x, *mods)
+    assert len(calls) == 1
+    for m, y in zip(mods, ys):
+        assert torch.equal(y, m(x))
+
+
+def test_norm_for_makes_rows_only_for_readers_of_rows():
+    norm, x, r = RmsNorm(32).to(BF), torch.randn(3, 32).to(BF), torch.randn(3, 32).to(BF)
+    mods = [I.Int8ServingLinear(torch.randn(8, 32).to(BF), None) for _ in range(2)]
+    with torch.no_grad():
+        rows, h = norm_for(norm, x, mods, residual=r)
+        assert isinstance(rows, I.Int8Rows) and torch.equal(h, x + r)
+        assert isinstance(norm_for(norm, x, mods)[0], I.Int8Rows) and norm_for(norm, x, mods)[1] is x
+        for others in ([], mods[:1] + [Linear(32, 8)]):
+            y, h = norm_for(norm, x, others, residual=r)
+            assert torch.equal(y, norm(x + r)) and torch.equal(h, x + r)
+        mods[0].register_forward_hook(lambda *a: None)  # a hook has to see a tensor
+        assert isinstance(norm_for(norm, x, mods)[0], torch.Tensor)
+    assert isinstance(norm_for(norm, x, mods[1:])[0], torch.Tensor)  # gradients are recorded
+
+
+def test_serving_weights_survive_moves_and_state_dicts():
+    m = I.Int8ServingLinear(torch.randn(8, 20), torch.randn(8))
+    x = torch.randn(3, 20)
+    with torch.no_grad():
+        y = m(x)
+    scale = m.weight_scale.clone()
+    m.to(BF)
+    assert m.weight.dtype == torch.int8 and torch.equal(m.weight_scale, scale) and m.bias.dtype == BF
+    other = I.Int8ServingLinear(torch.zeros(8, 20), torch.zeros(8))
+    other.load_state_dict({k: v.float() if k == "bias" else v for k, v in m.state_dict().items()})
+    with torch.no_grad():
+        assert (other(x) - y).abs().max() <= 2.0 ** -8 * 4
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(hybrid_norm=True), dict(use_bias=True), dict(head_dim=24)])
+def test_engine_serves_weights_held_in_8_bits(kw):
+    """The engine's tokens are those that the quantised model gives without a cache."""
+    from levanter_b200.data.passthrough_tokenizer import PassthroughTokenizer
+    from levanter_b200.inference.engine import InferenceEngine, InferenceEngineConfig, Request
+    from levanter_b200.inference.jit_scheduler import SeqDecodingParams
+    from levanter_b200.layers.attention import AttentionMask
+
+    model = llama(**kw).build(100, seed=0).eval()
+    bytes_before = sum(p.nbytes for p in model.parameters())
+    cfg = InferenceEngineConfig(max_pages=32, max_seqs=4, page_size=8, max_pages_per_seq=8, compute_dtype=torch.float32, quantization=QuantizationConfig(int8=True))
+    with torch.no_grad():
+        engine = InferenceEngine.from_model_with_config(model, PassthroughTokenizer(100), cfg)
+        assert sum(isinstance(m, I.Int8ServingLinear) for m in model.modules()) == 2 * 7
+        assert sum(p.nbytes for p in model.parameters()) < 0.5 * bytes_before
+        prompts = [[3, 14, 15, 92], [65, 35, 8, 9, 79, 32, 38]]
+        reqs = [Request(prompt_tokens=p, request_id=i, decode_params=SeqDecodingParams(len(p) + 6, None, 0.0, i), n_generations=1) for i, p in enumerate(prompts)]
+        got = engine.generate(reqs).tokens
+        for p, out in zip(prompts, got):
+            seq = list(p)
+            for t in out:
+                logits = model(torch.tensor([seq], dtype=torch.int32), AttentionMask.causal())
+                logits = getattr(logits, "array", logits)[0, -1].float()
+                assert logits[t] >= logits.max() - 0.02  # (a cache of other widths sums in another order)
+                seq.append(int(t))
+    assert quantize_for_serving(model, cfg.quantization) is model

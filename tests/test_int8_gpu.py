@@ -334,3 +334,190 @@ def test_sizes_without_a_kernel_take_the_library():
     assert bool(((y.double() - want).abs() <= 2.0 ** -6 * (held(x.detach()).abs() @ held(w.detach()).abs().t())).all())
     y.sum().backward()
     assert x.grad.shape == x.shape and w.grad.shape == w.shape
+
+
+# ------------------------------------------------------------------------------------------------ together
+def half_layer(x, r, w, gu, down, act=Act.silu):
+    rows, h = I.rms_norm_int8(x, w, 1e-5, residual=r)
+    y = I.int8_product(rows, gu)
+    ff = y.shape[-1] // 2
+    return I.int8_product(I.gated_activation_int8(y[..., :ff], y[..., ff:], act), down, residual=h)
+
+
+def half_layer_operands(rows, cols, ff, seed=0):
+    return (rand(rows, cols, seed=seed), rand(rows, cols, seed=seed + 1, std=0.5), (1 + rand(cols, seed=seed + 2, std=0.1)).to(BF),
+            I.quantize_rows(rand(2 * ff, cols, seed=seed + 3, std=0.05)), I.quantize_rows(rand(cols, ff, seed=seed + 4, std=0.05)))
+
+
+@pytest.mark.parametrize("rows,cols,ff", [(1, 256, 512), (7, 1024, 768), (64, 520, 1000), (300, 1024, 2048)])
+def test_feed_forward_half(rows, cols, ff):
+    x, r, w, gu, down = half_layer_operands(rows, cols, ff)
+    got = half_layer(x, r, w, gu, down)
+    h = (x.float() + r.float()).to(BF).double()
+    q, s = whole(h * w.double(), (h.square().mean(-1, keepdim=True) + 1e-5).rsqrt())
+    y = ((q * s[:, None]) @ (gu.values.double() * gu.scale.double()[:, None]).t()).to(BF).double()
+    g, u = y.chunk(2, -1)
+    mid = torch.nn.functional.silu(g) * u
+    want = held(mid) @ (down.values.double() * down.scale.double()[:, None]).t() + h
+    # One bf16 rounding of y may fall the other way and move a row's scale by 2^-8, and with it every rounding of that row to 8 bits: then two
+    # quantisations of the same row differ, each by up to half a step of max |mid| / 127 per element, of random signs.
+    step = mid.abs().amax(-1, keepdim=True) / 127
+    noise = step.squeeze(-1) / 6 ** 0.5 * (down.dequantize(F32).double().square().sum(-1).max() ** 0.5)
+    assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 6 * noise[:, None] + 2.0 ** -8 * mid.abs().amax(-1, keepdim=True)).all())
+    # and in the mean such rows are few
+    assert (got.double() - want).norm() <= 2.0 ** -7 * want.norm()
+
+
+def test_captured_and_replayed():
+    """Two graphs of the same sizes, replayed in turn on new inputs: no workspace is shared between them."""
+    sets = [half_layer_operands(33, 1024, 768, seed=10 * i) for i in range(2)]
+    graphs, outs = [], []
+    for ops in sets:
+        half_layer(*ops)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(half_layer(*ops))
+        graphs.append(g)
+    for turn in range(3):
+        for i, ops in enumerate(sets):
+            ops[0].copy_(rand(33, 1024, seed=100 * turn + i))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for out, ops in zip(outs, sets):
+            assert torch.equal(out, half_layer(*ops))
+
+
+def test_on_other_streams_and_from_two_threads():
+    import threading
+
+    sets = [half_layer_operands(n, 1024, 768, seed=n) for n in (5, 200)]
+    want = [half_layer(*ops) for ops in sets]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = half_layer(*sets[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    lib.check_status()
+
+
+def test_inputs_are_left_as_they_are_and_results_are_new():
+    x, r, w, gu, down = half_layer_operands(9, 512, 256)
+    before = [t.clone() for t in (x, r, w, gu.values, gu.scale, down.values, down.scale)]
+    a = half_layer(x, r, w, gu, down)
+    b = half_layer(x, r, w, gu, down)
+    assert torch.equal(a, b) and a.data_ptr() != b.data_ptr()
+    assert all(torch.equal(t, u) for t, u in zip((x, r, w, gu.values, gu.scale, down.values, down.scale), before))
+    assert torch.equal(half_layer(x, x, w, gu, down), half_layer(x, x.clone(), w, gu, down))  # the same rows twice
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes of rows: the last ones are as right as the first."""
+    rows, cols = 1100000, 4096
+    x = torch.zeros(rows, cols, dtype=BF, device="cuda")
+    tail = rand(3, cols)
+    x[-3:] = tail
+    got = I.quantize_rows(x)
+    assert torch.equal(got.values[-3:], I.quantize_rows(tail).values) and not got.values[:1000].any() and not got.scale[:-3].any()
+    back = got.dequantize()
+    assert torch.equal(back[-3:], I.quantize_rows(tail).dequantize()) and not back[-5].any()
+    del x, back
+    y = I.int8_product(got, I.quantize_rows(rand(8, cols, seed=5)), out_dtype=F32)
+    assert torch.equal(y[-3:], I.int8_product(I.quantize_rows(tail), I.quantize_rows(rand(8, cols, seed=5)), out_dtype=F32)) and not y[:-3].any()
+
+
+# ------------------------------------------------------------------------------------------------ models
+def serving_llama(**kw):
+    from levanter_b200.models.llama import LlamaConfig
+    from levanter_b200.quantization import QuantizationConfig, quantize_for_serving
+
+    cfg = dict(seq_len=256, hidden_dim=256, intermediate_dim=512, num_layers=2, num_heads=4, num_kv_heads=2, gradient_checkpointing=False)
+    model = LlamaConfig(**{**cfg, **kw}).build(512, seed=0, device="cuda", dtype=BF).eval()
+    return quantize_for_serving(model, QuantizationConfig(int8=True))
+
+
+def engine_of(model, graph=False):
+    from levanter_b200.data.passthrough_tokenizer import PassthroughTokenizer
+    from levanter_b200.inference.engine import InferenceEngine, InferenceEngineConfig
+    from levanter_b200.quantization import QuantizationConfig
+
+    return InferenceEngine.from_model_with_config(model, PassthroughTokenizer(512), InferenceEngineConfig(
+        max_pages=64, max_seqs=4, page_size=16, max_pages_per_seq=16, use_cuda_graph=graph, quantization=QuantizationConfig(int8=True)))
+
+
+def requests():
+    from levanter_b200.inference.engine import Request
+    from levanter_b200.inference.jit_scheduler import SeqDecodingParams
+
+    return [Request(prompt_tokens=list(range(5 + i, 40 + 3 * i)), request_id=i, decode_params=SeqDecodingParams(35 + 2 * i + 20, None, 0.0, i), n_generations=1)
+            for i in range(3)]
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(use_bias=True), dict(hybrid_norm=True)])
+def test_llama_serves_what_it_computes_without_a_cache(kw):
+    from levanter_b200.layers.attention import AttentionMask
+
+    model = serving_llama(**kw)
+    with torch.no_grad():
+        engine = engine_of(model)
+        out = engine.generate(requests()).tokens
+        for r, tokens in zip(requests(), out):
+            seq = torch.tensor([list(r.prompt_tokens) + [int(t) for t in tokens]], dtype=torch.int32, device="cuda")
+            logits = torch.nn.functional.linear(model.activations(seq, AttentionMask.causal()), model.get_lm_head())[0].float()
+            n = len(r.prompt_tokens)
+            for i, t in enumerate(tokens):
+                row = logits[n - 1 + i]
+                # the two ways differ by the attention kernels' roundings, which can move every rounding to 8 bits behind them: two layers of
+                # four quantisers with steps of some 4 / 127 of a standard deviation, 0.9 % each, 5 % in all at most
+                assert row[int(t)] >= row.max() - 2 * 0.05 * row.norm() / row.numel() ** 0.5 * 4
+
+
+def test_engine_with_graphs_gives_the_same_tokens():
+    with torch.no_grad():
+        plain = engine_of(serving_llama()).generate(requests()).tokens
+        graph = engine_of(serving_llama(), graph=True).generate(requests()).tokens
+    assert [list(map(int, t)) for t in plain] == [list(map(int, t)) for t in graph]
+
+
+def test_joint_projections_give_what_each_gives():
+    model = serving_llama()
+    layer = model.transformer.layers[0]
+    x = rand(5, 256)
+    with torch.no_grad():
+        apart = [m(x) for m in (layer.self_attn.q_proj, layer.self_attn.k_proj, layer.self_attn.v_proj)]
+        h = layer.mlp(x, residual=x)
+        model.initial_cache(8, 16)
+        joint = layer.self_attn._fused_int8()
+        assert joint is not None
+        y = I.int8_product(I.quantize_rows(x), *joint)
+        assert torch.equal(y[:, :512], torch.cat(apart, 1)) and torch.equal(layer.mlp(x, residual=x), h)
+        assert layer.mlp._rows.get([layer.mlp.gate_proj.weight, layer.mlp.up_proj.weight], build=False) is not None
+
+
+def test_training_step_of_a_model_in_int8():
+    from levanter_b200.models.llama import LlamaConfig
+    from levanter_b200.models.lm_model import LmExample, compute_next_token_loss
+    from levanter_b200.quantization import QuantizationConfig, quantize_linear_layers
+
+    cfg = LlamaConfig(seq_len=128, hidden_dim=256, intermediate_dim=512, num_layers=2, num_heads=4, num_kv_heads=2, gradient_checkpointing=False)
+    plain, model = (cfg.build(512, seed=0, device="cuda", dtype=BF) for _ in range(2))
+    quantize_linear_layers(model, QuantizationConfig(int8=True))
+    ex = LmExample.causal(torch.randint(0, 512, (2, 128), device="cuda", dtype=torch.int32))
+    for m in (plain, model):
+        compute_next_token_loss(m, ex).backward()
+    for (n, p), q in zip(model.named_parameters(), plain.named_parameters()):
+        q = q[1]
+        # eight quantisers of 0.9 % on the way through two layers and back, and as much again from the weights
+        assert (p.grad.float() - q.grad.float()).norm() <= 0.15 * q.grad.float().norm() + 1e-6, n
+    lib.check_status()
