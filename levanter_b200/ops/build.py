@@ -14,8 +14,10 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
+from typing import Optional
 
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIBDIR = Path(__file__).resolve().parent / "_lib"
@@ -88,11 +90,36 @@ def is_current(serving: bool = False) -> bool:
     return lib_path(serving).exists() and stamp.exists() and stamp.read_text().strip() == _digest(_sources(serving))
 
 
+LAUNCHER = "_lvb_launcher.so"
+
+
+def build_launcher(force: bool = False) -> Optional[Path]:
+    """Compile ``csrc/host/launcher.c``, a Python module that calls the library's launchers (:func:`levanter_b200.ops.lib.quick`).  None where Python's own
+    headers are not installed; the launchers are then called through ``ctypes``."""
+    src, out = CSRC / "host" / "launcher.c", LIBDIR / LAUNCHER
+    include = sysconfig.get_paths()["include"]
+    gcc = shutil.which("gcc") or shutil.which("cc")
+    if not (Path(include) / "Python.h").exists() or gcc is None:
+        return out if out.exists() else None
+    stamp, digest = LIBDIR / "launcher.stamp", hashlib.sha256(src.read_bytes()).hexdigest()
+    if not force and out.exists() and stamp.exists() and stamp.read_text().strip() == digest:
+        return out
+    LIBDIR.mkdir(parents=True, exist_ok=True)
+    part = out.with_suffix(f".{os.getpid()}.part")
+    r = subprocess.run([gcc, "-O2", "-shared", "-fPIC", "-I", include, str(src), "-o", str(part)], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{gcc} failed for {src.name}:\n{r.stderr}")
+    os.replace(part, out)
+    stamp.write_text(digest)
+    return out
+
+
 def build(force: bool = False, verbose: bool = False, serving: bool = False) -> Path:
     """Compile every ``csrc/*.cu`` (``serving``: the serving subset) and link the shared object.  Returns its path."""
     srcs = _sources(serving)
     if not srcs:
         raise RuntimeError(f"no CUDA sources in {CSRC}")
+    build_launcher(force)
     if not force and is_current(serving):
         return lib_path(serving)
     LIBDIR.mkdir(parents=True, exist_ok=True)

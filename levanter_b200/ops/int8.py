@@ -82,16 +82,20 @@ def _launch(name: str, t: torch.Tensor, *args) -> None:
     follows reads the state itself and makes no objects.)"""
     f = _f.get(name)
     if f is None:
-        kinds = {"p": lib.c_void_p, "l": lib.c_longlong, "i": lib.c_int, "f": lib.c_float}
-        f = _f[name] = lib.fn(name, [kinds[a] for a in _ARGS[name]] + [lib.c_void_p])
+        f = _f[name] = lib.quick(name, _ARGS[name] + "p")
+    lib.launch_count += 1
     dev = t.get_device()
-    if dev == torch._C._cuda_getDevice():
-        rc = f(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if dev == _current():
+        rc = f(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = f(*args, torch._C._cuda_getCurrentRawStream(dev))
+            rc = f(*args, _stream(dev))
     if rc:
         lib.check_rc(rc, name)
+
+
+_current = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else lambda: -1
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _kernels(t: torch.Tensor) -> bool:
@@ -106,6 +110,8 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check_rows(v: torch.Tensor, s: torch.Tensor, what: str) -> None:
+    if v.dtype is torch.int8 and s.dtype is torch.float32 and v.dim() == 2 and s.dim() == 1 and len(v) == len(s) and s.get_device() == v.get_device():
+        return
     if v.dtype is not torch.int8 or s.dtype is not torch.float32:
         raise TypeError(f"{what}: int8 values with fp32 scales expected, got {v.dtype} and {s.dtype}")
     if v.dim() == 0 or s.shape != v.shape[:-1]:
@@ -117,18 +123,19 @@ def _check_rows(v: torch.Tensor, s: torch.Tensor, what: str) -> None:
 def _check_floats(what: str, like: torch.Tensor, other: Optional[torch.Tensor] = None) -> None:
     if like.dtype not in _FLOATS:
         raise TypeError(f"{what}: rows in bf16 or fp32 expected, got {like.dtype}")
-    if like.dim() == 0 or like.shape[-1] == 0:
-        raise ValueError(f"{what}: rows of at least one element expected, got {tuple(like.shape)}")
-    if other is not None and (other.dtype is not like.dtype or other.shape != like.shape or other.get_device() != like.get_device()):
-        raise ValueError(f"{what}: {tuple(other.shape)} {other.dtype} on {other.device} does not go with {tuple(like.shape)} {like.dtype} on {like.device}")
-    _no_gradient(what, like, other)
+    shape = like.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{what}: rows of at least one element expected, got {tuple(shape)}")
+    if other is not None and (other.dtype is not like.dtype or other.shape != shape or other.get_device() != like.get_device()):
+        raise ValueError(f"{what}: {tuple(other.shape)} {other.dtype} on {other.device} does not go with {tuple(shape)} {like.dtype} on {like.device}")
+    if torch.is_grad_enabled():
+        _no_gradient(what, like, other)
 
 
 def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"{what} has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
 
 
 def _rows_of(t: torch.Tensor, align: int = 1) -> Tuple[torch.Tensor, int, int, int]:
@@ -136,7 +143,10 @@ def _rows_of(t: torch.Tensor, align: int = 1) -> Tuple[torch.Tensor, int, int, i
     overlap and they start at multiples of ``align`` bytes."""
     cols = t.shape[-1]
     if t.is_contiguous():
-        rows, ld, ok = t.numel() // cols, cols, True
+        rows, ptr = t.numel() // cols, t.data_ptr()
+        if ptr % align == 0 and cols % 16 == 0:
+            return t, ptr, rows, cols
+        ld, ok = cols, True
     else:
         t = t if t.dim() == 2 else t.reshape(-1, cols)  # the caller keeps what a copy is read from
         rows, ld = t.shape[0], t.stride(0)
@@ -208,7 +218,8 @@ def rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 
     if weight is not None:
         if weight.dim() != 1 or weight.shape[0] != cols or weight.dtype not in _FLOATS or weight.get_device() != x.get_device():
             raise ValueError(f"rms_norm_int8: weight [{cols}] in bf16 or fp32 on {x.device} expected, got {tuple(weight.shape)} {weight.dtype} on {weight.device}")
-        _no_gradient("rms_norm_int8", weight)
+        if weight.requires_grad and torch.is_grad_enabled():
+            _no_gradient("rms_norm_int8", weight)
     if not _kernels(x):
         x = x.detach()
         h = x if residual is None else (x.float() + residual.detach().float()).to(x.dtype)
@@ -271,27 +282,29 @@ def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dty
     w, sw = weight
     _check_rows(v, sv, "int8_product: rows")
     _check_rows(w, sw, "int8_product: weight")
-    lead, (N, K) = v.shape[:-1], w.shape if w.dim() == 2 else (0, 0)
-    if v.shape[-1] != K or w.get_device() != v.get_device():
-        raise ValueError(f"int8_product: rows {tuple(v.shape)} on {v.device} and weight {tuple(w.shape)} on {w.device} do not go together")
+    shape = v.shape
+    N, K = w.shape if w.dim() == 2 else (0, 0)
+    if shape[-1] != K or w.get_device() != v.get_device():
+        raise ValueError(f"int8_product: rows {tuple(shape)} on {v.device} and weight {tuple(w.shape)} on {w.device} do not go together")
     if not 0 < K <= MAX_COLS:
         raise ValueError(f"int8_product: rows of 1 to {MAX_COLS} elements expected, got {K}")
     if out_dtype not in _FLOATS:
         raise TypeError(f"int8_product: results in bf16 or fp32, not {out_dtype}")
-    shape = (*lead, N)
+    shape = (shape[0], N) if len(shape) == 2 else (*shape[:-1], N)
     if bias is not None or residual is not None:
         for t, want, what in ((bias, (N,), "bias"), (residual, shape, "residual")):
             if t is not None and (t.shape != want or t.dtype not in _FLOATS or t.get_device() != v.get_device()):
                 raise ValueError(f"int8_product: {what} {want} in bf16 or fp32 on {v.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        _no_gradient("int8_product", bias, residual)
+        if torch.is_grad_enabled():
+            _no_gradient("int8_product", bias, residual)
     if not _kernels(v):
         y = torch.matmul(v.double(), w.double().t()).float() * sv.unsqueeze(-1) * sw
         for t in (bias, residual):
             y = y if t is None else y + t.float()
         return y.to(out_dtype)
+    out = torch.empty(*shape, dtype=out_dtype, device=v.device)
     v, a, M, lda = _rows_of(v, 16)
     w, b, _, ldb = _rows_of(w, 16)
-    out = torch.empty(*shape, dtype=out_dtype, device=v.device)
     if M == 0 or N == 0:
         return out
     flags = F_OUT_F32 if out_dtype is torch.float32 else 0
@@ -303,7 +316,8 @@ def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dty
     if residual is not None:
         flags |= F_RESIDUAL | (F_RESIDUAL_F32 if residual.dtype is torch.float32 else 0)
         residual, rptr, _, ldr = _rows_of(residual)
-    sv, sw = _dense(sv), _dense(sw)
+    if not (sv.is_contiguous() and sw.is_contiguous()):
+        sv, sw = sv.contiguous(), sw.contiguous()
     _launch("lvb_int8_gemm", v, a, b, sv.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K, lda, ldb, N, flags, bptr, rptr, ldr, form, splits, stages,
             _status(v))
     return out

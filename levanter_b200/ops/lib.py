@@ -8,6 +8,9 @@ callers use their PyTorch reference implementations.
 from __future__ import annotations
 
 import ctypes
+import functools
+import importlib.machinery
+import importlib.util
 import threading
 from typing import Optional
 
@@ -118,6 +121,36 @@ def fn(name: str, argtypes: list, restype=c_int, launches: int = 1):
 
     counted.__name__ = name
     return counted
+
+
+_quick: dict = {}
+
+
+def quick(name: str, kinds: str):
+    """The launcher ``name`` as a function of its arguments, without ``ctypes``' 2 us per call where the module for that has been built.  ``kinds``: a letter
+    per argument, p pointer, l long long, i int, f float.  A call counts as one kernel launch only where its caller adds it to ``launch_count``."""
+    f = _quick.get(name)
+    if f is None:
+        types = {"p": c_void_p, "l": c_longlong, "i": c_int, "f": c_float}
+        g = getattr(load(), name)
+        g.argtypes, g.restype = [types[k] for k in kinds], c_int
+        module = _launcher()
+        f = _quick[name] = g if module is None else functools.partial(module.call, ctypes.cast(g, c_void_p).value, kinds)
+    return f
+
+
+@functools.lru_cache(maxsize=None)
+def _launcher():
+    path = _build.LIBDIR / _build.LAUNCHER
+    if not path.exists():
+        return None
+    try:
+        loader = importlib.machinery.ExtensionFileLoader("_lvb_launcher", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_lvb_launcher", path, loader=loader))
+        loader.exec_module(module)
+    except ImportError:
+        return None
+    return module
 
 
 def stream_ptr() -> int:
