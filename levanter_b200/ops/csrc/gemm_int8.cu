@@ -390,7 +390,9 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
   if (splits < 1) splits = 1;
   if (splits > 8) splits = 8;
   if (splits > k_blocks) splits = k_blocks;
-  if (stages > kMaxStages) stages = kMaxStages;
+  const int tiles = (p.N + 127) / 128 * ((p.M + TN - 1) / TN);
+  const bool all_at_once = stages == 0;  // a ring that lets all CTAs run at once, up to three per SM: waves of them cost more than a short ring
+  if (stages == 0 || stages > kMaxStages) stages = kMaxStages;
   int per, part, ring;
   while (true) {  // as many splits as the shared memory has room for
     per = (k_blocks + splits - 1) / splits;
@@ -398,7 +400,10 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
     if (stages > per) stages = per;
     if (stages < 1) stages = 1;
     part = splits > 1 ? 128 * 4 * exchange_pitch(exchange_share(p.M < TN ? p.M : TN, splits)) : 0;
-    while (stages > 1 && stages * kStage + (splits - 1) * part > 220 * 1024) --stages;
+    const int per_sm = (tiles * splits + num_sms() - 1) / num_sms();
+    // (one per SM: a long share of K gains by a deep ring, beside a short one the next kernel's first CTAs should have room)
+    const int room = (!all_at_once || (per_sm <= 1 && (TN > 64 || per > 16)) ? 220 : per_sm <= 2 ? 110 : 72) * 1024;
+    while (stages > (room < 220 * 1024 ? 3 : 1) && stages * kStage + (splits - 1) * part > room) --stages;
     ring = stages * kStage > splits * part ? stages * kStage : (splits * part + 1023) / 1024 * 1024;  // it also holds the sums that are sent
     if (ring + (splits - 1) * part <= 220 * 1024) break;
     --splits;  // (one split needs the ring alone)
@@ -692,37 +697,35 @@ int launch_pair(const void* A, const void* B, long long lda, long long ldb, cons
 }
 
 // Which form (us, weights out of the cache).  few / stream: 1 row, 768 x 768 2.0 / 3.2, 2304 x 768 2.6 / 3.3, 2048 x 2048 4.4 / 3.7, 4096 x 4096 7.8 / 5.3; 16 rows, 2304 x 768
-// 3.3 / 3.6.  stream / pair, where the stream's tiles of 128 x 256 are one wave: 512 rows, 2304 x 768 6.7 / 9.6, 6144 x 4096 15.9 / 17.2; 1000 rows, 4096 x 4096
-// 15.3 / 16.6, 4096 x 14336 46 / 42; more than a wave: 777 rows, 6144 x 4096 26.2 / 26.2, 28672 x 4096 116 / 83, 1500 rows, 4096 x 4096 28 / 26; up to 128 rows, 28672 x 4096 24 / 30.
-inline int choose_form(int M, int N, int K) {
-  if (M <= 16 && K <= 1024 && N <= 4096) return 1;
-  if (M <= 128) return 2;
-  return K <= 4096 && static_cast<long long>((N + 127) / 128) * ((M + 255) / 256) <= num_sms() ? 2 : 3;
-}
-// Splits of K and ring stages of the stream form, where they are 0.  A CTA gets 16 KB of weights per 0.28 us wherever they come from, so fewer than some 110 CTAs do
+// 3.3 / 3.6.  stream by tiles of 128 rows / of 256 / pair: 512 rows, 2304 x 768 5.0 / 6.6 / 9.6, 4096 x 4096 13.1 / 15.0 / 15.6; 300 rows, 8192 x 2048 (more than a wave of
+// the first) 11.2 / 10.7 / 11.8; 400 rows, 14336 x 4096 34 / 36 / 27, 4096 x 14336 36 / 42 / 37; 128 rows, 28672 x 4096 24 / 36 / 30.
+// Splits of K in the stream form.  A CTA gets 16 KB of weights per 0.28 us wherever they come from, so fewer than some 110 CTAs do
 // not keep the memory busy, and all that run should run at once; a split costs a start, the exchange of its sums (which grows with the rows) and the rows
 // of activations once more.  us for 1, 2, 4, 8 splits: 4096 x 4096, 1 row 10.8, 7.8, 5.3, 6.4, 64 rows 11.6, 10.4, 8.2, 20, 128 rows 12.3, 13.0, 10.9; 6144 x 4096, 16
-// rows 11.2, 8.7, 6.9, 7.9; 8192 x 2048, 16 rows 7.4, 5.7, 6.3, 10.3; 512 x 8192, 1 row 19.5, 11.4, 7.0, 5.0; 28672 x 4096, 1 row 20.7, 25, 25, 32.
-inline void choose_splits(int M, int N, int K, int& splits, int& stages) {
-  const int tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  const int tiles = (N + 127) / 128 * ((M + tn - 1) / tn), k_blocks = (K + BK - 1) / BK, sms = num_sms();
-  if (splits == 0) {
-    splits = 1;
-    if (tn <= 64) {
-      if (3 * tiles <= sms) splits = 4;  // 48 tiles
-      else if (2 * tiles <= sms && tn <= 32) splits = 2;
-      if (16 * tiles <= sms && k_blocks >= 32) splits = 8;
-      while (splits > 1 && k_blocks < 4 * splits) splits /= 2;
-    } else if (tn == 128) {
-      if (4 * tiles <= sms && k_blocks >= 32) splits = 4;
-    } else if (2 * tiles <= sms && k_blocks >= 64) {
-      splits = 2;
-    }
+// rows 11.2, 8.7, 6.9, 7.9; 8192 x 2048, 16 rows 7.4, 5.7, 6.3, 10.3; 512 x 8192, 1 row 19.5, 11.4, 7.0, 5.0; 28672 x 4096, 1 row 20.7, 25, 25, 32; 4096 x 14336, 1 row 33,
+// 19, 12.7, 12.1.
+struct Plan {
+  int form, rows, splits;  // rows: of activations per tile of the stream form
+};
+inline Plan choose(int M, int N, int K) {
+  const int k_blocks = (K + BK - 1) / BK, sms = num_sms(), columns = (N + 127) / 128;
+  if (M <= 16 && K <= 1024 && N <= 4096) return {1, 0, 0};
+  if (M <= 64) {
+    int splits = 1;
+    if (3 * columns <= sms) splits = 4;  // 48 tiles
+    else if (2 * columns <= sms && M <= 32) splits = 2;
+    if (k_blocks >= 32 && (16 * columns <= sms || (k_blocks >= 96 && M <= 32 && 4 * columns <= sms))) splits = 8;
+    while (splits > 1 && k_blocks < 4 * splits) splits /= 2;
+    return {2, M <= 16 ? 16 : M <= 32 ? 32 : 64, splits};
   }
-  if (stages == 0) {
-    const int per_sm = (tiles * splits + sms - 1) / sms;
-    stages = (per_sm <= 1 ? 216 : per_sm == 2 ? 110 : 72) * 1024 / ((128 + tn) * BK);
+  const long long narrow = static_cast<long long>(columns) * ((M + 127) / 128), wide = static_cast<long long>(columns) * ((M + 255) / 256);
+  if (narrow <= sms || M <= 128) {
+    int splits = 1;
+    if (4 * narrow <= sms && k_blocks >= (M <= 128 ? 32 : 64)) splits = 4;
+    else if (2 * narrow <= sms && k_blocks >= 64) splits = 2;
+    return {2, 128, splits};
   }
+  return {K <= 4096 && wide <= sms ? 2 : 3, 256, 1};
 }
 
 }  // namespace int8_gemm
@@ -730,10 +733,11 @@ inline void choose_splits(int M, int N, int K, int& splits, int& stages) {
 
 // C[M,N] (bf16, or fp32 with flag 1; row stride ldc) = (A[M,K] B[N,K]^T) scale_a[M] scale_b[N] + bias[N] (flag 2; fp32 with flag 4, else bf16)
 // + residual[M,N] (flag 8; fp32 with flag 16, else bf16; row stride ldr).  A and B: int8, 16-byte aligned, row strides multiples of 16 that are at least K.
-// form: 0 lets the launcher choose; 1 few (M <= 16), 2 stream, 3 pair.  splits, stages: of the stream form, 0 lets the launcher choose.
+// form: 0 lets the launcher choose; 1 few (M <= 16), 2 stream, 3 pair.  tile_rows (16, 32, 64, 128 or 256), splits (at most 8), stages: of the stream form, 0
+// lets the launcher choose.
 extern "C" int lvb_int8_gemm(const void* A, const void* B, const float* scale_a, const float* scale_b, void* C, int M, int N, int K, long long lda,
-                             long long ldb, long long ldc, int flags, const void* bias, const void* residual, long long ldr, int form, int splits, int stages,
-                             int* status, void* stream) {
+                             long long ldb, long long ldc, int flags, const void* bias, const void* residual, long long ldr, int form, int tile_rows,
+                             int splits, int stages, int* status, void* stream) {
   using namespace lvb;
   using namespace lvb::int8_gemm;
   if (M <= 0 || N <= 0 || K <= 0 || K > 131071 || (lda & 15) || (ldb & 15) || lda < K || ldb < K || ldc < N) return kErrBadArg;
@@ -743,14 +747,20 @@ extern "C" int lvb_int8_gemm(const void* A, const void* B, const float* scale_a,
   if (((flags & kBias) && bias == nullptr) || ((flags & kResidual) && (residual == nullptr || ldr < N))) return kErrBadArg;
   Params p{C, scale_a, scale_b, bias, residual, M, N, K, ldc, ldr, flags, status};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (form == 0) form = choose_form(M, N, K);
-  if (form == 1) return M <= 16 ? launch_few(A, B, lda, ldb, p, s) : kErrBadArg;
-  if (form == 3) return launch_pair(A, B, lda, ldb, p, s);
-  if (form != 2) return kErrBadArg;
-  choose_splits(M, N, K, splits, stages);
-  if (M <= 16) return launch_stream<16>(A, B, lda, ldb, p, splits, stages, s);
-  if (M <= 32) return launch_stream<32>(A, B, lda, ldb, p, splits, stages, s);
-  if (M <= 64) return launch_stream<64>(A, B, lda, ldb, p, splits, stages, s);
-  if (M <= 128) return launch_stream<128>(A, B, lda, ldb, p, splits, stages, s);
-  return launch_stream<256>(A, B, lda, ldb, p, splits, stages, s);
+  Plan plan = choose(M, N, K);
+  if (form != 0) plan.form = form;
+  if (plan.form == 1) return M <= 16 ? launch_few(A, B, lda, ldb, p, s) : kErrBadArg;
+  if (plan.form == 3) return launch_pair(A, B, lda, ldb, p, s);
+  if (plan.form != 2) return kErrBadArg;
+  if (form != 0) plan.rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  if (tile_rows != 0) plan.rows = tile_rows;
+  if (splits != 0) plan.splits = splits;
+  switch (plan.rows) {
+    case 16: return launch_stream<16>(A, B, lda, ldb, p, plan.splits, stages, s);
+    case 32: return launch_stream<32>(A, B, lda, ldb, p, plan.splits, stages, s);
+    case 64: return launch_stream<64>(A, B, lda, ldb, p, plan.splits, stages, s);
+    case 128: return launch_stream<128>(A, B, lda, ldb, p, plan.splits, stages, s);
+    case 256: return launch_stream<256>(A, B, lda, ldb, p, plan.splits, stages, s);
+    default: return kErrBadArg;
+  }
 }

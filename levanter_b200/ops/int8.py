@@ -74,7 +74,7 @@ class Int8Rows(NamedTuple):
 # ------------------------------------------------------------------------------------------------ calls
 # Arguments of the launchers by letter (p pointer, l long long, i int, f float); a stream follows.
 _ARGS = {"lvb_int8_quantize": "pilliplp", "lvb_int8_rms_norm": "pppilllpiffliplp", "lvb_int8_glu": "ppilliliplp", "lvb_int8_dequantize": "plplipi",
-         "lvb_int8_gemm": "pppppiiilllippliiip", "lvb_int8_quantize_parts": "pppppiiiiiipp"}
+         "lvb_int8_gemm": "pppppiiilllippliiiip", "lvb_int8_quantize_parts": "pppppiiiiiipp"}
 
 
 def _launch(name: str, t: torch.Tensor, *args) -> None:
@@ -277,7 +277,7 @@ def int8_product(rows: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] 
     return _product(rows, weight, bias, residual, out_dtype)
 
 
-def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dtype=torch.bfloat16, form: int = 0, splits: int = 0, stages: int = 0) -> torch.Tensor:
+def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dtype=torch.bfloat16, form: int = 0, splits: int = 0, stages: int = 0, tile: int = 0) -> torch.Tensor:
     v, sv = rows
     w, sw = weight
     _check_rows(v, sv, "int8_product: rows")
@@ -318,7 +318,7 @@ def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dty
         residual, rptr, _, ldr = _rows_of(residual)
     if not (sv.is_contiguous() and sw.is_contiguous()):
         sv, sw = sv.contiguous(), sw.contiguous()
-    _launch("lvb_int8_gemm", v, a, b, sv.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K, lda, ldb, N, flags, bptr, rptr, ldr, form, splits, stages,
+    _launch("lvb_int8_gemm", v, a, b, sv.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K, lda, ldb, N, flags, bptr, rptr, ldr, form, tile, splits, stages,
             _status(v))
     return out
 
@@ -374,7 +374,7 @@ def _held_products(x: torch.Tensor, values: torch.Tensor, scale: torch.Tensor, l
         flags = 0
         if bias is not None:
             flags, bias = F_BIAS | (F_BIAS_F32 if bias.dtype is torch.float32 else 0), _dense(bias)
-        _launch("lvb_int8_gemm", y, q, q + first * ld, s, s + 4 * first, y.data_ptr(), rows, outs, cols, ld, ld, outs, flags, lib.ptr(bias), 0, 0, 0, 0, 0, status)
+        _launch("lvb_int8_gemm", y, q, q + first * ld, s, s + 4 * first, y.data_ptr(), rows, outs, cols, ld, ld, outs, flags, lib.ptr(bias), 0, 0, 0, 0, 0, 0, status)
         return y
 
     if len(weights) > 1 and rows <= MANY_ROWS and all(b is None for b in biases):
