@@ -85,28 +85,25 @@ __device__ __forceinline__ void shift_words(uint32_t (&u)[kIn], uint32_t bytes) 
     for (int j = 0; j < kOut; ++j) u[j] = __funnelshift_r(u[j], u[j + 1], 16);
 }
 template <typename T>
-struct Raw {  // eight elements as they lie in memory
+struct Raw {  // eight elements as they lie in memory, and ahead of them what an aligned load brings along
   static constexpr int kWords = 2 * sizeof(T);
-  uint32_t u[kWords];
+  uint32_t u[kWords + 4];
+  uint32_t before;  // bytes ahead of the first element
   __device__ __forceinline__ void load(const T* p, int live, const char* lo, const char* hi) {
     const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
     const char* base = reinterpret_cast<const char*>(p) - off;
-    if (live >= 8 && off == 0) {
+    const bool inside = live >= 8 && (off == 0 || (base >= lo && base + 4 * kWords + 16 <= hi));
+    before = inside ? off : 0;
+    if (inside) {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
         const uint4 w = __ldg(reinterpret_cast<const uint4*>(base) + i);
         u[4 * i] = w.x; u[4 * i + 1] = w.y; u[4 * i + 2] = w.z; u[4 * i + 3] = w.w;
       }
-    } else if (live >= 8 && base >= lo && base + 4 * kWords + 16 <= hi) {
-      uint32_t e[kWords + 4];
-#pragma unroll
-      for (int i = 0; i < kWords / 4 + 1; ++i) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(base) + i);
-        e[4 * i] = w.x; e[4 * i + 1] = w.y; e[4 * i + 2] = w.z; e[4 * i + 3] = w.w;
+      if (off != 0) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(base) + kWords / 4);
+        u[kWords] = w.x; u[kWords + 1] = w.y; u[kWords + 2] = w.z; u[kWords + 3] = w.w;
       }
-      shift_words<kWords>(e, off);
-#pragma unroll
-      for (int j = 0; j < kWords; ++j) u[j] = e[j];
     } else if constexpr (sizeof(T) == 2) {
       const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
@@ -116,19 +113,24 @@ struct Raw {  // eight elements as they lie in memory
       for (int j = 0; j < 8; ++j) u[j] = j < live ? __float_as_uint(__ldg(p + j)) : 0u;
     }
   }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
+  __device__ __forceinline__ void get(float (&v)[8]) const {  // (not ahead of here: loads that have just been started are not waited for)
+    uint32_t e[kWords + 4];
+#pragma unroll
+    for (int j = 0; j < kWords + 4; ++j) e[j] = u[j];
+    if (before != 0) shift_words<kWords>(e, before);
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(u[j] << 16);
-        v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+        v[2 * j] = __uint_as_float(e[j] << 16);
+        v[2 * j + 1] = __uint_as_float(e[j] & 0xFFFF0000u);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(u[j]);
+      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(e[j]);
     }
   }
   __device__ __forceinline__ void set(const float (&v)[8]) {
+    before = 0;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) u[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
@@ -183,7 +185,7 @@ template <typename T>
 struct Plain {
   Span<T> x;
   using In = Raw<T>;
-  static constexpr bool kSum = false;
+  static constexpr bool kSum = false, kTwiceTheRegisters = false;
   __device__ __forceinline__ void load(In& in, long long row, int c, int live) const { in.load(x.p + row * x.ld + c, live, x.lo, x.hi); }
   __device__ __forceinline__ void get(const In& in, long long, int, int, float (&y)[8], F32x2&) const { in.get(y); }
   __device__ __forceinline__ float factor(float) const { return 1.f; }
@@ -200,7 +202,7 @@ struct Norm {
   struct In {
     Raw<T> a, b;  // (without a residual the second is never loaded and takes no register)
   };
-  static constexpr bool kSum = true;
+  static constexpr bool kSum = true, kTwiceTheRegisters = kResidual;
   __device__ __forceinline__ void load(In& in, long long row, int c, int live) const {
     in.a.load(x.p + row * x.ld + c, live, x.lo, x.hi);
     if constexpr (kResidual) in.b.load(r.p + row * r.ld + c, live, r.lo, r.hi);
@@ -246,7 +248,7 @@ struct Glu {
   struct In {
     Raw<T> a, b;
   };
-  static constexpr bool kSum = false;
+  static constexpr bool kSum = false, kTwiceTheRegisters = false;
   __device__ __forceinline__ void load(In& in, long long row, int c, int live) const {
     in.a.load(g.p + row * g.ld + c, live, g.lo, g.hi);
     in.b.load(u.p + row * u.ld + c, live, u.lo, u.hi);
@@ -458,8 +460,8 @@ __device__ __forceinline__ float warp_ss(F32x2 ss2) {
 // Few rows, and rows that lie anywhere.  kWarp: a row per warp, else a row per block.  kChunks: groups of eight elements per thread, held in registers; 0:
 // any number of them, each made twice.  A block goes through rows far apart and starts the reads of its next row before it reduces and writes the one it
 // has.  q has room for whole groups of eight up to the end of its row stride.
-template <class Src, bool kWarp, int kChunks>
-__global__ void __launch_bounds__(kWarp ? 32 * kRowWarps : kMostThreads) quantize_kernel(Src src, long long rows, int cols, int8_t* __restrict__ q, long long ldq,
+template <class Src, bool kWarp, int kChunks, int kThreads>
+__global__ void __launch_bounds__(kThreads) quantize_kernel(Src src, long long rows, int cols, int8_t* __restrict__ q, long long ldq,
                                                                                         float* __restrict__ scale) {
   __shared__ __align__(16) uint32_t s_top[2][32];
   __shared__ __align__(16) float s_ss[2][32];
@@ -597,11 +599,11 @@ int resident_blocks(int threads, int shared) {  // per SM
   return n < 1 ? 1 : n > 32 ? 32 : n;
 }
 
-template <class Src, bool kWarp, int kChunks>
+template <class Src, bool kWarp, int kChunks, int kThreads>
 int launch(const Src& src, long long rows, int cols, int threads, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
   const long long blocks = kWarp ? (rows + kRowWarps - 1) / kRowWarps : rows;
-  const long long most = static_cast<long long>(num_sms()) * resident_blocks<quantize_kernel<Src, kWarp, kChunks>>(threads, 0);
-  return launch_chained(quantize_kernel<Src, kWarp, kChunks>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(threads), 0, s, src, rows, cols, q,
+  const long long most = static_cast<long long>(num_sms()) * resident_blocks<quantize_kernel<Src, kWarp, kChunks, kThreads>>(threads, 0);
+  return launch_chained(quantize_kernel<Src, kWarp, kChunks, kThreads>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(threads), 0, s, src, rows, cols, q,
                         ldq, scale) == cudaSuccess
              ? kErrOk
              : kErrCuda;
@@ -631,10 +633,14 @@ int quantize(const Src& src, long long rows, int cols, void* q, long long ldq, f
   if (rows <= 0 || cols <= 0 || q == nullptr || scale == nullptr || (ldq & 7) || ldq < cols || (reinterpret_cast<uintptr_t>(q) & 7)) return kErrBadArg;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int8_t* o = reinterpret_cast<int8_t*>(q);
-  if (cols <= 512) return launch<Src, true, 2>(src, rows, cols, 32 * kRowWarps, o, ldq, scale, s);
-  if (cols > kMostThreads * 8 * kHeldGroups) return launch<Src, false, 0>(src, rows, cols, kMostThreads, o, ldq, scale, s);
+  if (cols <= 512) return launch<Src, true, 2, 32 * kRowWarps>(src, rows, cols, 32 * kRowWarps, o, ldq, scale, s);
+  if (cols > kMostThreads * 8 * kHeldGroups) return launch<Src, false, 0, kMostThreads>(src, rows, cols, kMostThreads, o, ldq, scale, s);
   const int threads = ((cols + 7) / 8 + 32 * kHeldGroups - 1) / (32 * kHeldGroups) * 32;
-  return launch<Src, false, kHeldGroups>(src, rows, cols, threads, o, ldq, scale, s);
+  // (a norm with a residual has two inputs and an output that start anywhere: with half the threads and twice the registers 16384 x 4095 take 200 us, not 255)
+  if constexpr (Src::kTwiceTheRegisters) {
+    if (threads <= kMostThreads / 2) return launch<Src, false, kHeldGroups, kMostThreads / 2>(src, rows, cols, threads, o, ldq, scale, s);
+  }
+  return launch<Src, false, kHeldGroups, kMostThreads>(src, rows, cols, threads, o, ldq, scale, s);
 }
 
 // out = q * scale, rounded once, for dense rows `out`.  kGroup elements per thread: 16 of aligned rows of whole groups of 16, else 8, and those may lie
