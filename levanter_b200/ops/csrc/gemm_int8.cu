@@ -9,6 +9,8 @@
 //           exchange their partial sums through distributed shared memory;
 //   pair    256 x 256 tiles on CTA pairs (tcgen05 cta_group::2, kind::i8), persistent, accumulators double-buffered in tensor memory.
 // Every wait is bounded (common.cuh).
+#include <type_traits>
+
 #include "cta_pair.cuh"
 
 namespace lvb {
@@ -31,6 +33,7 @@ struct Params {
   long long ldc, ldr;
   int flags;
   int* status;
+  int aligned = 0;  // 32 columns of C and of the residual from a multiple of 32 on start on 16 bytes in every row
 };
 
 // Instruction descriptor for kind::i8: signed 8-bit A and B, both K-major, 32-bit whole-number accumulator.
@@ -69,41 +72,60 @@ __device__ __forceinline__ void finish(const Params& p, int m, int n, int sum, f
   else reinterpret_cast<__nv_bfloat16*>(p.C)[m * p.ldc + n] = __float2bfloat16(v);
 }
 // The same for the first `live` of kRows rows from m on in one column, whose lanes' neighbours hold the neighbouring columns: 32 of them write a line of
-// a row together.  `in`: the column exists.  sa: the rows' scales in shared memory, 16-byte aligned.
-template <int kRows>
-__device__ __forceinline__ void finish_column(const Params& p, int m, int live, int n, bool in, const int (&sum)[kRows], const float* sa, float sb, float bias) {
+// a row together.  `in`: the column exists.  finish_rows() takes numbers that have their scales and bias, finish_column() sums and the rows' scales in shared memory.
+template <int kRows, class Value>
+__device__ __forceinline__ void finish_rows(const Params& p, int m, int live, int n, bool in, Value value) {
   if (!in) return;
   float v[kRows];
-#pragma unroll
-  for (int j = 0; j < kRows; j += 4) {
-    const float4 f = *reinterpret_cast<const float4*>(sa + j);
-    v[j] = static_cast<float>(sum[j]) * f.x * sb + bias;
-    v[j + 1] = static_cast<float>(sum[j + 1]) * f.y * sb + bias;
-    v[j + 2] = static_cast<float>(sum[j + 2]) * f.z * sb + bias;
-    v[j + 3] = static_cast<float>(sum[j + 3]) * f.w * sb + bias;
-  }
   if (p.flags & kResidual) {
+    // all loads ahead of the first use, and none behind a condition of its own, which would make them wait for one another: rows that do not exist read the last
+    const int last = live - 1;
     if (p.flags & kResidualF32) {
       const float* r = reinterpret_cast<const float*>(p.residual) + m * p.ldr + n;
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) v[j] += j < live ? __ldg(r + j * p.ldr) : 0.f;
+      for (int j = 0; j < kRows; ++j) v[j] = __ldg(r + min(j, last) * p.ldr);
     } else {
-      const __nv_bfloat16* r = reinterpret_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + n;
+      const unsigned short* r = reinterpret_cast<const unsigned short*>(p.residual) + m * p.ldr + n;
+      unsigned short h[kRows];
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) v[j] += j < live ? __bfloat162float(__ldg(r + j * p.ldr)) : 0.f;
+      for (int j = 0; j < kRows; ++j) h[j] = __ldg(r + min(j, last) * p.ldr);
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) v[j] = __uint_as_float(static_cast<uint32_t>(h[j]) << 16);
     }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) v[j] += value(j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) v[j] = value(j);
   }
+  auto put = [&](auto* o, auto whole) {
+#pragma unroll
+    for (int j = 0; j < kRows; ++j, o += p.ldc) {
+      if (decltype(whole)::value || j < live) {
+        if constexpr (sizeof(*o) == 4) *o = v[j];
+        else *o = __float2bfloat16(v[j]);
+      }
+    }
+  };
   if (p.flags & kOutF32) {
     float* o = reinterpret_cast<float*>(p.C) + m * p.ldc + n;
-#pragma unroll
-    for (int j = 0; j < kRows; ++j, o += p.ldc)
-      if (j < live) *o = v[j];
+    if (live >= kRows) put(o, std::true_type{});
+    else put(o, std::false_type{});
   } else {
     __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n;
-#pragma unroll
-    for (int j = 0; j < kRows; ++j, o += p.ldc)
-      if (j < live) *o = __float2bfloat16(v[j]);
+    if (live >= kRows) put(o, std::true_type{});
+    else put(o, std::false_type{});
   }
+}
+template <int kRows>
+__device__ __forceinline__ void finish_column(const Params& p, int m, int live, int n, bool in, const int (&sum)[kRows], const float* sa, float sb, float bias) {
+  finish_rows<kRows>(p, m, live, n, in, [&](int j) { return static_cast<float>(sum[j]) * sa[j] * sb + bias; });
+}
+// Brings `columns` of the residual from row m, column n on (which exist) into the L2 while the sums are still being made.
+__device__ __forceinline__ void prefetch_residual(const Params& p, int m, int n, int columns) {
+  const int size = (p.flags & kResidualF32) ? 4 : 2;
+  const char* at = reinterpret_cast<const char*>(p.residual) + (m * p.ldr + n) * size;
+  for (int i = 0; i < columns * size; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + i));
 }
 
 // ================================================================ few rows
@@ -306,6 +328,8 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
       sb = __ldg(p.scale_b + n);
       bias = bias_at(p, n);
     }
+    if (p.flags & kResidual)
+      for (int i = threadIdx.x - 64; i < live; i += 128) prefetch_residual(p, m0 + i, n0, min(128, p.N - n0));
     named_bar_sync(1, 128);
   }
   // ---- every thread: the tile's sums are complete in this CTA
@@ -362,13 +386,24 @@ stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ C
         const int first = rank * share, count = min(share, live - first);
         const int* own = reinterpret_cast<const int*>(sent + rank * part_bytes) + (quad * 32 + lane) * pitch;
         const int* other = reinterpret_cast<const int*>(got) + (quad * 32 + lane) * pitch;
-        for (int i = 0; i < count; i += 4) {
+        auto add = [&](int i, int* sum) {
           const int4 a = *reinterpret_cast<const int4*>(own + i);
-          int sum[4] = {a.x, a.y, a.z, a.w};
+          sum[0] = a.x; sum[1] = a.y; sum[2] = a.z; sum[3] = a.w;
           for (int s = 0; s < splits - 1; ++s) {
             const int4 v = *reinterpret_cast<const int4*>(other + s * 128 * pitch + i);
             sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
           }
+        };
+        int i = 0;
+        for (; i + 4 < count; i += 8) {  // (a share is a multiple of four)
+          int sum[8];
+          add(i, sum);
+          add(i + 4, sum + 4);
+          finish_column<8>(p, m0 + first + i, count - i, n, in, sum, s_scale + first + i, sb, bias);
+        }
+        if (i < count) {
+          int sum[4];
+          add(i, sum);
           finish_column<4>(p, m0 + first + i, count - i, n, in, sum, s_scale + first + i, sb, bias);
         }
       }
@@ -443,7 +478,7 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
 constexpr int BN = 256, BMP = 256, BMC = 128;
 constexpr int kPairStage = (BMC + BN / 2) * BK;  // per CTA
 constexpr int kPairStages = 6;
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 4 * BN * 4 + (2 * kPairStages + 4) * 8 + 16;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 4 * BN * 4 + 4 * 32 * 33 * 4 + (2 * kPairStages + 4) * 8 + 16;
 
 __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& mb, int& nb) {
   constexpr int GM = 4;  // four row tiles stay in the L2 while the raster sweeps N
@@ -458,7 +493,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* s_scale = reinterpret_cast<float*>(smem + kPairStages * kPairStage);  // the columns' scales, of one tile and the next
   float* s_bias = s_scale + 2 * BN;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_scale + 4 * BN);
+  float* s_turn = s_scale + 4 * BN;  // 32 x 32 numbers of every epilogue warp, rows 33 apart
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_turn + 4 * 32 * 33);
   uint64_t* empty_bar = full_bar + kPairStages;
   uint64_t* tfull_bar = empty_bar + kPairStages;
   uint64_t* tempty_bar = tfull_bar + 2;
@@ -544,6 +580,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   } else {
     // epilogue: a lane has one row of this CTA's 128 and sees it 32 columns at a time
     const int quad = warp & 3;
+    float* turn = s_turn + quad * (32 * 33);
     int buf = 0;
     uint32_t tphase = 0;
     bool alive = true;
@@ -561,6 +598,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         sb[at] = there ? __ldg(p.scale_b + nb * BN + at) : 0.f;
         if (p.flags & kBias) s_bias[buf * BN + at] = there ? bias_at(p, nb * BN + at) : 0.f;
       }
+      if (in && (p.flags & kResidual)) prefetch_residual(p, m, nb * BN, min(BN, p.N - nb * BN));
       named_bar_sync(1, 128);
       if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&tfull_bar[buf], tphase, abort_flag, p.status, 300, buf));
       if (!alive) continue;  // the other warps wait for this one at the barrier above, tile by tile
@@ -573,7 +611,6 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         uint32_t r[32];
         tmem_ld_32x32(taddr + c, r);
         tmem_ld_wait();
-        if (!in) continue;
         const int cols = min(32, p.N - n0);
         float v[32];
 #pragma unroll
@@ -591,62 +628,50 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             v[4 * q] += f.x; v[4 * q + 1] += f.y; v[4 * q + 2] += f.z; v[4 * q + 3] += f.w;
           }
         }
+        if (cols < 32 || !p.aligned) {
+          // Rows that start anywhere, and the last columns: through shared memory, so that the lanes hold neighbouring columns of one row
+#pragma unroll
+          for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = v[j];
+          __syncwarp();
+          const int m0 = m - lane;
+          float* column = turn + lane;
+          finish_rows<32>(p, m0, min(32, p.M - m0), n0 + lane, lane < cols, [&](int i) { return column[i * 33]; });
+          __syncwarp();
+          continue;
+        }
+        if (!in) continue;
         if (p.flags & kResidual) {
           if (p.flags & kResidualF32) {
-            const float* rr = reinterpret_cast<const float*>(p.residual) + m * p.ldr + n0;
-            if (cols == 32 && (reinterpret_cast<uintptr_t>(rr) & 15) == 0) {
+            const float4* rr = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.residual) + m * p.ldr + n0);
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const float4 a = reinterpret_cast<const float4*>(rr)[q];
-                v[4 * q] += a.x; v[4 * q + 1] += a.y; v[4 * q + 2] += a.z; v[4 * q + 3] += a.w;
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < cols) v[j] += rr[j];
+            for (int q = 0; q < 8; ++q) {
+              const float4 a = __ldg(rr + q);
+              v[4 * q] += a.x; v[4 * q + 1] += a.y; v[4 * q + 2] += a.z; v[4 * q + 3] += a.w;
             }
           } else {
-            const __nv_bfloat16* rr = reinterpret_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + n0;
-            if (cols == 32 && (reinterpret_cast<uintptr_t>(rr) & 15) == 0) {
+            const uint4* rr = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + n0);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint4 a = reinterpret_cast<const uint4*>(rr)[q];
-                const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+            for (int q = 0; q < 4; ++q) {
+              const uint4 a = __ldg(rr + q);
+              const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  v[8 * q + 2 * j] += __uint_as_float(u[j] << 16);
-                  v[8 * q + 2 * j + 1] += __uint_as_float(u[j] & 0xFFFF0000u);
-                }
+              for (int j = 0; j < 4; ++j) {
+                v[8 * q + 2 * j] += __uint_as_float(u[j] << 16);
+                v[8 * q + 2 * j + 1] += __uint_as_float(u[j] & 0xFFFF0000u);
               }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < cols) v[j] += __bfloat162float(rr[j]);
             }
           }
         }
         if (p.flags & kOutF32) {
-          float* o = reinterpret_cast<float*>(p.C) + m * p.ldc + n0;
-          if (cols == 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+          float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.C) + m * p.ldc + n0);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) reinterpret_cast<float4*>(o)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < cols) o[j] = v[j];
-          }
+          for (int q = 0; q < 8; ++q) o[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         } else {
-          __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n0;
-          if (cols == 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+          uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n0);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              reinterpret_cast<uint4*>(o)[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                                                          pack_bf16x2(v[8 * q + 4], v[8 * q + 5]), pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < cols) o[j] = __float2bfloat16(v[j]);
-          }
+          for (int q = 0; q < 4; ++q)
+            o[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]), pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
+                              pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
         }
       }
       tc_fence_before();
@@ -664,7 +689,9 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   }
 }
 
-int launch_pair(const void* A, const void* B, long long lda, long long ldb, const Params& p, cudaStream_t s) {
+int launch_pair(const void* A, const void* B, long long lda, long long ldb, Params p, cudaStream_t s) {
+  auto whole = [](const void* x, long long ld, bool f32) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld & (f32 ? 3 : 7)) == 0; };
+  p.aligned = whole(p.C, p.ldc, p.flags & kOutF32) && (!(p.flags & kResidual) || whole(p.residual, p.ldr, p.flags & kResidualF32));
   CUtensorMap tmA, tmB;
   int rc = make_tmap_2d_u8(&tmA, A, p.M, p.K, lda, BMC);
   if (rc == kErrOk) rc = make_tmap_2d_u8(&tmB, B, p.N, p.K, ldb, BN / 2);
