@@ -33,7 +33,7 @@ struct Params {
   long long ldc, ldr;
   int flags;
   int* status;
-  int aligned = 0;  // 32 columns of C and of the residual from a multiple of 32 on start on 16 bytes in every row
+  int aligned = 0;  // C is bf16, and 32 columns of it and of the residual from a multiple of 32 on start on 16 bytes in every row
 };
 
 // Instruction descriptor for kind::i8: signed 8-bit A and B, both K-major, 32-bit whole-number accumulator.
@@ -629,7 +629,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
           }
         }
         if (cols < 32 || !p.aligned) {
-          // Rows that start anywhere, and the last columns: through shared memory, so that the lanes hold neighbouring columns of one row
+          // Rows that start anywhere, the last columns and fp32 (8192 x 11008 x 4096 347 us row by row, 275 so): through shared memory, so that the lanes hold
+          // neighbouring columns of one row
 #pragma unroll
           for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = v[j];
           __syncwarp();
@@ -662,17 +663,11 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
           }
         }
-        if (p.flags & kOutF32) {
-          float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.C) + m * p.ldc + n0);
+        uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n0);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) o[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        } else {
-          uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n0);
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            o[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]), pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
-                              pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
-        }
+        for (int q = 0; q < 4; ++q)
+          o[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]), pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
+                            pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
       }
       tc_fence_before();
       __syncwarp();
@@ -691,7 +686,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 
 int launch_pair(const void* A, const void* B, long long lda, long long ldb, Params p, cudaStream_t s) {
   auto whole = [](const void* x, long long ld, bool f32) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld & (f32 ? 3 : 7)) == 0; };
-  p.aligned = whole(p.C, p.ldc, p.flags & kOutF32) && (!(p.flags & kResidual) || whole(p.residual, p.ldr, p.flags & kResidualF32));
+  p.aligned = !(p.flags & kOutF32) && whole(p.C, p.ldc, false) && (!(p.flags & kResidual) || whole(p.residual, p.ldr, p.flags & kResidualF32));
   CUtensorMap tmA, tmB;
   int rc = make_tmap_2d_u8(&tmA, A, p.M, p.K, lda, BMC);
   if (rc == kErrOk) rc = make_tmap_2d_u8(&tmB, B, p.N, p.K, ldb, BN / 2);
