@@ -4,12 +4,19 @@
 // The mathematics.  A norm multiplies a row by a factor f = rsqrt(mean h^2 + eps) of its own, which leaves q as it is and joins the scale, so the sum
 // of squares and the largest |h w| are taken in one pass over the row and one exchange between its threads.  127 y / max |y| is formed with the reciprocal
 // of max |y| (off by at most 127 * 2^-22); for elements that this leaves within 1e-4 of a tie the sign of 127 y - border max |y|, in one
-// fused operation, says on which side of it they are.  bf16 rows need this: half of the largest value lies on a tie, and a row often holds it.  A row below 2^-100 (or, ahead of its factor, below 2^-120) is stored as zeros with scale 0; a row with an
-// infinity or a NaN as zeros with scale NaN, so that everything made from it is NaN.
+// fused operation, says on which side of it they are.  bf16 rows need this: half of the largest value lies on a tie, and a row often holds it.
+// A row below 2^-100 (or, ahead of its factor, below 2^-120) is stored as zeros with scale 0; a row with an infinity or a NaN as zeros with scale NaN, so
+// that everything made from it is NaN.
 //
-// What bounds it: memory.  One pass reads the inputs and writes 1 byte per element (and h, 2 or 4).  The threads of a row keep it in registers as
-// fp32 between the reduction and the write: a warp per row up to 1024 columns, up to 1024 threads per row beyond that, and above 32768
-// columns the row is read twice.
+// What bounds it: memory.  One pass reads the inputs and writes 1 byte per element (and h, 2 or 4).  The threads of a row keep it in registers as fp32
+// between the reduction and the write, and the reads of a block's next row are under way meanwhile:
+//   - rows of whole groups of 16 bf16 elements that start on 32 bytes, above 512 and up to 16384 columns: a block per row, one load of 32 bytes per thread
+//     and input (rows16_kernel).  16384 x 4096: norm with residual 73 us (470 MB, 6.4 TB/s), without 48 (4.2), a row as it is 38 (5.3); gated activation of
+//     8192 x 11008 87 (5.2).  A norm without residual waits for its reduction: of 4096 columns it holds half of what an SM could read in that time.
+//   - the others (quantize_kernel): up to 512 columns a warp per row; up to 16384 a block per row, eight elements per thread and turn; beyond that the row
+//     is read twice.  Rows of 4095 or 11007 columns, which start anywhere: norm with residual 200 us, gated activation 200, a row as it is 65.
+//   - back: 31 us for 16384 x 4096 (201 MB, 6.4 TB/s), 42 for 8192 x 11008; rows of odd widths 45 and 58.
+// Few rows are bound by a launch: one row of 4096 takes 2.0 us in a graph.
 #include <initializer_list>
 #include <type_traits>
 #include <utility>
@@ -267,10 +274,17 @@ struct Glu {
 // inputs (and of h) have one stride.
 struct Raw16 {
   uint32_t u[8];
+  // What is read once stays out of the L1: a norm with residual of 16384 x 4096 then takes 73 us, not 83.  kAgain: every row reads it (a norm's weight).
+  template <bool kAgain = false>
   __device__ __forceinline__ void load(const void* p) {
-    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
-                 : "l"(p));
+    if constexpr (kAgain)
+      asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+          : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+          : "l"(p));
+    else
+      asm("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+          : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+          : "l"(p));
   }
   __device__ __forceinline__ void store(void* p) const {
     asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]),
@@ -327,9 +341,9 @@ struct Norm16 {
       sum.store(h + at);
     }
     Raw16 w0, w1;
-    if (w != nullptr) {  // from the L1, row after row
-      w0.load(kW32 ? static_cast<const void*>(static_cast<const float*>(w) + c) : static_cast<const void*>(static_cast<const __nv_bfloat16*>(w) + c));
-      if constexpr (kW32) w1.load(static_cast<const float*>(w) + c + 8);
+    if (w != nullptr) {  // from the L1, row after row; from the L2 beside a residual, where the L1 is worth less than its traffic (83 us instead of 73)
+      w0.template load<!kResidual>(kW32 ? static_cast<const void*>(static_cast<const float*>(w) + c) : static_cast<const void*>(static_cast<const __nv_bfloat16*>(w) + c));
+      if constexpr (kW32) w1.template load<!kResidual>(static_cast<const float*>(w) + c + 8);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -652,32 +666,44 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restric
   const long long total = rows * cols;
   const unsigned units = cols / kGroup;
   const bool narrow = total < (1ll << 32);  // a division of 32 bits is three times as fast
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i * kGroup < total; i += gridDim.x * 256ll) {
-    if constexpr (kGroup == 16) {
-      const long long row = narrow ? static_cast<unsigned>(i) / units : i / units;
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + row * ldq + (i - row * units) * 16));
-      const float s = __ldg(scale + row);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-      Raw16 o[sizeof(T) / 2];
+  const long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (i * kGroup >= total) return;
+  if constexpr (kGroup == 16) {
+    const long long row = narrow ? static_cast<unsigned>(i) / units : i / units;
+    uint4 w;
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+        : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+        : "l"(q + row * ldq + (i - row * units) * 16));
+    const float s = __ldg(scale + row);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    Raw16 o[sizeof(T) / 2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t p = u[j / 2] >> (16 * (j & 1));
-        const float a = static_cast<float>(static_cast<int8_t>(p)) * s, b = static_cast<float>(static_cast<int8_t>(p >> 8)) * s;
-        if constexpr (sizeof(T) == 2) {
-          o[0].u[j] = pack_bf16x2(a, b);
-        } else {
-          o[j / 4 % (sizeof(T) / 2)].u[2 * j % 8] = __float_as_uint(a);
-          o[j / 4 % (sizeof(T) / 2)].u[(2 * j + 1) % 8] = __float_as_uint(b);
-        }
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t p = u[j / 2] >> (16 * (j & 1));
+      const float a = static_cast<float>(static_cast<int8_t>(p)) * s, b = static_cast<float>(static_cast<int8_t>(p >> 8)) * s;
+      if constexpr (sizeof(T) == 2) {
+        o[0].u[j] = pack_bf16x2(a, b);
+      } else {
+        o[j / 4 % (sizeof(T) / 2)].u[2 * j % 8] = __float_as_uint(a);
+        o[j / 4 % (sizeof(T) / 2)].u[(2 * j + 1) % 8] = __float_as_uint(b);
       }
+    }
 #pragma unroll
-      for (int k = 0; k < sizeof(T) / 2; ++k) o[k].store(out + i * 16 + k * 8);
+    for (int k = 0; k < sizeof(T) / 2; ++k) o[k].store(out + i * 16 + k * 8);
+  } else {
+    float v[8] = {};
+    Raw<T> group;  // (groups of eight of a dense `out` start on 16 bytes)
+    long long row = narrow ? static_cast<unsigned>(i * 8) / static_cast<unsigned>(cols) : i * 8 / cols;
+    int c = static_cast<int>(i * 8 - row * cols);
+    float s = __ldg(scale + row);
+    if (c >= 4 && c + 12 <= cols) {  // three words of the row have the eight bytes; 16384 x 4095: 75 us byte by byte, 45 so
+      const uintptr_t at = reinterpret_cast<uintptr_t>(q + row * ldq + c);
+      const uint32_t* base = reinterpret_cast<const uint32_t*>(at & ~uintptr_t{3});
+      const uint32_t shift = static_cast<uint32_t>(at & 3) * 8;
+      const uint32_t w[3] = {__ldg(base), __ldg(base + 1), __ldg(base + 2)};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int8_t>(__funnelshift_r(w[j / 4], w[j / 4 + 1], shift) >> (j % 4 * 8))) * s;
     } else {
-      float v[8];
-      Raw<T> group;  // (groups of eight of a dense `out` start on 16 bytes)
-      long long row = narrow ? static_cast<unsigned>(i * 8) / static_cast<unsigned>(cols) : i * 8 / cols;
-      int c = static_cast<int>(i * 8 - row * cols);
-      float s = __ldg(scale + row);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (i * 8 + j < total) {
@@ -688,19 +714,20 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restric
           }
         }
       }
-      group.set(v);
-      const long long left = total - i * 8;
-      if (left >= 8) group.store(out + i * 8, 8);
-      else group.put(out + i * 8, 0, static_cast<int>(left));
     }
+    group.set(v);
+    const long long left = total - i * 8;
+    if (left >= 8) group.store(out + i * 8, 8);
+    else group.put(out + i * 8, 0, static_cast<int>(left));
   }
 }
 
 template <typename T>
 int dequantize(const void* q, long long ldq, const float* scale, long long rows, int cols, void* out, cudaStream_t s) {
   const bool whole = cols % 16 == 0 && (ldq & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0;
-  const long long units = whole ? rows * (cols / 16) : (rows * cols + 7) / 8, most = 8ll * num_sms();
-  const dim3 grid(static_cast<unsigned>((units + 255) / 256 < most ? (units + 255) / 256 : most));
+  const long long units = whole ? rows * (cols / 16) : (rows * cols + 7) / 8;
+  if ((units + 255) / 256 > 0x7FFFFFFF) return kErrBadArg;
+  const dim3 grid(static_cast<unsigned>((units + 255) / 256));  // (8 blocks per SM that go on from group to group: 36.6 us for 16384 x 4096, not 32.1)
   const int8_t* p = reinterpret_cast<const int8_t*>(q);
   const cudaError_t e = whole ? launch_chained(dequantize_kernel<T, 16>, grid, dim3(256), 0, s, p, ldq, scale, rows, cols, reinterpret_cast<T*>(out))
                               : launch_chained(dequantize_kernel<T, 8>, grid, dim3(256), 0, s, p, ldq, scale, rows, cols, reinterpret_cast<T*>(out));
