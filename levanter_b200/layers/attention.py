@@ -377,7 +377,6 @@ def dot_product_attention_with_sink(q, k, v, sink: torch.Tensor, mask=None, bias
 # --------------------------------------------------------------------------------------------- module
 from ..nn import FusedRows, Linear, RmsNorm, linear_many, plain  # noqa: E402  (after function definitions to keep the file readable)
 from ..ops.int8 import Int8Rows, Int8ServingLinear, as_int8_rows, int8_product  # noqa: E402
-from ..ops.int8 import Int8Rows, Int8ServingLinear, as_int8_rows, int8_product
 
 
 @dataclass(frozen=True)

@@ -206,15 +206,15 @@ class LlamaMlp(nn.Module):
     def _int8(self, x, residual: Optional[torch.Tensor]) -> torch.Tensor:
         """The MLP on weights held in 8 bits: every row is quantised where it is made, gate and up are one product where they lie side by side."""
         mods = (self.gate_proj, self.up_proj)
-        rows, shared = as_int8_rows(x), all(m.bias is None for m in mods)
+        shared = all(m.bias is None for m in mods)
         weight = self._rows.get([m.weight for m in mods], build=False) if shared else None
         scale = self._scales.get([m.weight_scale for m in mods], build=False) if shared else None
         if weight is not None and scale is not None:
-            y, ff = int8_product(rows, Int8Rows(weight, scale), out_dtype=x.dtype), self.gate_proj.out_features
+            y, ff = int8_product(as_int8_rows(x), Int8Rows(weight, scale), out_dtype=x.dtype), self.gate_proj.out_features
             gate, up = y[..., :ff], y[..., ff:]
         else:
-            gate, up = self.gate_proj(rows), self.up_proj(rows)
-        return self.down_proj(gated_activation_int8(gate, up, self.act), residual=residual)
+            gate, up = linear_many(x, *mods)
+        return int8_product(gated_activation_int8(gate, up, self.act), self.down_proj.rows, self.down_proj.bias, residual, out_dtype=x.dtype)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if all(plain(m, Int8ServingLinear) for m in (self.gate_proj, self.up_proj, self.down_proj)):

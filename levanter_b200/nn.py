@@ -269,10 +269,11 @@ def fork_norm(norm: nn.Module, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Ten
 def linear_many(x: torch.Tensor, *projections: nn.Module):
     """The projections of the same rows, one by one; in training their input gradients are summed in the epilogues of their products."""
     from .ops.gemm import linear_many as many
-    from .ops.int8 import Int8Linear, Int8ServingLinear, as_int8_rows, int8_linear_many
+    from .ops.int8 import Int8Linear, Int8ServingLinear, as_int8_rows, int8_linear_many, int8_product
 
     if all(plain(m, Int8ServingLinear) for m in projections):
-        x = as_int8_rows(x)  # once for all of them
+        rows = as_int8_rows(x)  # once for all of them
+        return tuple(int8_product(rows, m.rows, m.bias, out_dtype=x.dtype) for m in projections)
     elif all(plain(m, Int8Linear) for m in projections):
         return int8_linear_many(x, [m.operand(x.dtype) for m in projections], [m.bias for m in projections])
     elif x.requires_grad and torch.is_grad_enabled() and all(plain(m, Linear) and m.bias is None and getattr(m.weight, "grad_sink", None) is None

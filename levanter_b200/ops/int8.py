@@ -60,14 +60,17 @@ class Int8Rows(NamedTuple):
         _check_rows(v, s, "rows")
         if dtype not in _FLOATS:
             raise TypeError(f"rows come back as bf16 or fp32, not {dtype}")
+        if s.requires_grad and torch.is_grad_enabled():
+            _no_gradient("dequantize", s)
         if not _kernels(v):
             return (v.float() * s.unsqueeze(-1)).to(dtype)
         out = torch.empty(*v.shape, dtype=dtype, device=v.device)
+        if out.numel() == 0:
+            return out
         cols = v.size(-1)
         v, ptr, rows, ld = _rows_of(v)
-        if rows:
-            s = _dense(s)
-            _launch("lvb_int8_dequantize", v, ptr, ld, s.data_ptr(), rows, cols, out.data_ptr(), int(dtype is torch.float32))
+        s = _dense(s)
+        _launch("lvb_int8_dequantize", v, ptr, ld, s.data_ptr(), rows, cols, out.data_ptr(), int(dtype is torch.float32))
         return out
 
 
@@ -295,8 +298,8 @@ def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dty
         for t, want, what in ((bias, (N,), "bias"), (residual, shape, "residual")):
             if t is not None and (t.shape != want or t.dtype not in _FLOATS or t.get_device() != v.get_device()):
                 raise ValueError(f"int8_product: {what} {want} in bf16 or fp32 on {v.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        if torch.is_grad_enabled():
-            _no_gradient("int8_product", bias, residual)
+    if torch.is_grad_enabled():
+        _no_gradient("int8_product", sv, sw, bias, residual)
     if not _kernels(v):
         y = torch.matmul(v.double(), w.double().t()).float() * sv.unsqueeze(-1) * sw
         for t in (bias, residual):
@@ -390,7 +393,7 @@ def _held_products(x: torch.Tensor, values: torch.Tensor, scale: torch.Tensor, l
 class _Int8ManyFn(torch.autograd.Function):
     """Projections of the same rows.  Kept for the backward pass: the rows and the weights in 8 bits, 1 byte per activation instead of 2, once for all projections.
 
-    ``dx = sum dy w'`` and ``dw = dy^T x'`` are bf16 products of what the whole numbers stand for, rounded to bf16 (2^-9 of each value, as any operand
+    ``dx = sum dy w'`` and ``dw = dy^T x'`` are bf16 products of what the whole numbers stand for, rounded to bf16 (2^-8 of each value at most, as any operand
     of a bf16 layer); output gradients are not quantised, their rows span too many magnitudes for one scale.  The sum over several projections is rounded
     once: of few rows their output gradients are laid side by side for one product each way, of many rows it is formed in fp32 (8192 rows of 4096 by two of
     11008, us in a row of such steps: side by side 1375 to 1414, in fp32 1268 to 1313, rounding what the second product adds to 1158 to 1239)."""
@@ -403,7 +406,8 @@ class _Int8ManyFn(torch.autograd.Function):
         ctx.refs, ctx.bias_dtypes = weights, [None if b is None else b.dtype for b in biases]
         ctx.x_shape, ctx.ld = x.shape, ld
         ctx.set_materialize_grads(False)  # a product that nothing uses has no gradient, and its weight none
-        return _held_products(x, values, scale, ld, weights, biases)
+        # (parts of one tensor, which autograd would take for views of each other and refuse to have written in place)
+        return tuple(y.data for y in _held_products(x, values, scale, ld, weights, biases))
 
     @staticmethod
     def backward(ctx, *dys):
@@ -518,14 +522,14 @@ class Int8Linear(nn.Module):
 
 class Int8ServingLinear(nn.Module):
     """A projection that serves: its weights are held in 8 bits (buffers ``weight`` int8 ``[out, in]`` and ``weight_scale`` fp32 ``[out]``) and have no gradient.
-    It takes rows in bf16 or fp32, or :class:`Int8Rows` that several projections share, and adds a ``residual`` in its product's epilogue."""
+    It takes rows in bf16 or fp32 and gives results of their type, or :class:`Int8Rows` that several projections share (results in bf16), and adds a ``residual`` in
+    its product's epilogue."""
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor]):
         super().__init__()
         if weight.dim() != 2 or weight.dtype not in _FLOATS or not 0 < weight.shape[1] <= MAX_COLS:
             raise ValueError(f"a weight [out, in] in bf16 or fp32 with up to {MAX_COLS} columns expected, got {tuple(weight.shape)} {weight.dtype}")
         self.out_features, self.in_features = weight.shape
-        self.dtype = weight.dtype
         rows = _quantize(weight.detach())
         self.register_buffer("weight", rows.values)
         self.register_buffer("weight_scale", rows.scale)
@@ -547,8 +551,7 @@ class Int8ServingLinear(nn.Module):
         return self
 
     def forward(self, x: Union[torch.Tensor, Int8Rows], *, skip_bias: bool = False, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        out = self.dtype if isinstance(x, Int8Rows) else x.dtype
-        return int8_product(as_int8_rows(x), self.rows, None if skip_bias else self.bias, residual, out_dtype=out)
+        return int8_product(as_int8_rows(x), self.rows, None if skip_bias else self.bias, residual, out_dtype=x.dtype)
 
     def extra_repr(self):
         return f"in={self.in_features}, out={self.out_features}, bias={self.bias is not None}, int8 weights"

@@ -216,3 +216,48 @@ def test_engine_serves_weights_held_in_8_bits(kw):
                 assert logits[t] >= logits.max() - 0.02  # (a cache of other widths sums in another order)
                 seq.append(int(t))
     assert quantize_for_serving(model, cfg.quantization) is model
+
+
+@pytest.mark.parametrize("kw, targets", [(dict(), None), (dict(hybrid_norm=True), None), (dict(use_bias=True), None), (dict(), ["gate_proj", "up_proj"]), (dict(), ["q_proj", "down_proj"]),
+                                         (dict(), ["q_proj", "k_proj", "v_proj", "o_proj"]), (dict(), ["up_proj"])])
+def test_bf16_engine_takes_rows_from_the_norms_where_all_readers_do(kw, targets):
+    from levanter_b200.data.passthrough_tokenizer import PassthroughTokenizer
+    from levanter_b200.inference.engine import InferenceEngine, InferenceEngineConfig, Request
+    from levanter_b200.inference.jit_scheduler import SeqDecodingParams
+    from levanter_b200.layers.attention import AttentionMask
+
+    quant = QuantizationConfig(int8=True) if targets is None else QuantizationConfig(int8=True, targets=targets)
+    model = quantize_for_serving(llama(**kw).build(100, seed=0).eval(), quant).to(BF)  # (a conversion after the weights were quantised)
+    cfg = InferenceEngineConfig(max_pages=32, max_seqs=4, page_size=8, max_pages_per_seq=8, compute_dtype=BF)
+    with torch.no_grad():
+        engine = InferenceEngine.from_model_with_config(model, PassthroughTokenizer(100), cfg)
+        prompts = [[3, 14, 15, 92], [65, 35, 8, 9, 79, 32, 38]]
+        reqs = [Request(prompt_tokens=p, request_id=i, decode_params=SeqDecodingParams(len(p) + 4, None, 0.0, i), n_generations=1) for i, p in enumerate(prompts)]
+        for p, out in zip(prompts, engine.generate(reqs).tokens):
+            logits = model(torch.tensor([p], dtype=torch.int32), AttentionMask.causal())
+            logits = getattr(logits, "array", logits)[0, -1].float()
+            # the paged path forms its norms in 32 bits ahead of the 8 bits, the other rounds them to bf16: some steps of 2^-8 per layer, of logits below 1
+            assert logits.abs().max() < 1 and logits[out[0]] >= logits.max() - 0.05
+
+
+def test_results_have_the_type_of_the_rows():
+    m = I.Int8ServingLinear(torch.randn(8, 32), None)
+    x = torch.randn(3, 32)
+    with torch.no_grad():
+        assert m(x).dtype == torch.float32 and m(x.to(BF)).dtype == BF and m(I.quantize_rows(x)).dtype == BF
+        assert [y.dtype for y in linear_many(x, m, m)] == [torch.float32] * 2
+
+
+@pytest.mark.parametrize("call", [lambda r: r.dequantize(), lambda r: I.int8_product(r, r), lambda r: I.int8_product(I.Int8Rows(r.values, r.scale.detach()), r)])
+def test_scales_that_want_a_gradient_are_refused(call):
+    rows = I.quantize_rows(torch.randn(4, 16))
+    rows = I.Int8Rows(rows.values, rows.scale.requires_grad_())
+    with pytest.raises(RuntimeError):
+        call(rows)
+    with torch.no_grad():
+        call(rows)
+
+
+def test_rows_without_elements_come_back_empty():
+    assert I.Int8Rows(torch.empty(3, 0, dtype=torch.int8), torch.empty(3)).dequantize().shape == (3, 0)
+    assert I.quantize_rows(torch.empty(0, 16)).dequantize().shape == (0, 16)

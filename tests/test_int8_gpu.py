@@ -150,6 +150,17 @@ def test_dequantize(rows, cols, dtype):
     assert torch.equal(part.dequantize(dtype), (part.values.float() * part.scale[:, None]).to(dtype))
 
 
+@pytest.mark.parametrize("cols", [12, 17, 333, 4095, 4097])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_dequantize_of_rows_that_start_and_end_anywhere(cols, dtype):
+    values = torch.randint(-128, 128, (37, cols + 40), device="cuda", dtype=torch.int8)
+    scale = torch.rand(37, device="cuda")
+    for first in (0, 1, 2, 3, 6, 16):
+        for ld in (cols, cols + 3, cols + 24):
+            part = values.flatten()[first:].as_strided((37, cols), (ld, 1), first)
+            assert torch.equal(I.Int8Rows(part, scale).dequantize(dtype), (part.float() * scale[:, None]).to(dtype))
+
+
 # ------------------------------------------------------------------------------------------------ products
 def int8(rows, cols, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -325,6 +336,88 @@ def test_main_grad_receives_the_weight_gradient():
     w.main_grad = torch.ones(32, 512, device="cuda")
     I.int8_linear(x, w).sum().backward()
     assert w.grad is None and bool(((w.main_grad - 1 - want.float()).abs() <= 2.0 ** -8 * want.float().abs() + 2.0 ** -22).all())
+
+
+def test_one_weight_twice_and_results_written_in_place():
+    x, w = rand(64, 512).requires_grad_(), rand(32, 512, seed=2).requires_grad_()
+    a, b = I.int8_linear_many(x, [w, w])
+    assert torch.equal(a, b)
+    a.mul_(2.0)  # its neighbour stays as it is
+    assert torch.equal(a, 2 * b)
+    dy = rand(64, 32, seed=3)
+    gx, gw = torch.autograd.grad([a, b], [x, w], [dy, dy])
+    wx, ww = torch.autograd.grad(I.int8_linear(x, w), [x, w], dy)
+    # three times the gradient, of which each part was rounded (2^-8), the larger one being twice as large, and their sum once
+    assert bool(((gw.double() - 3 * ww.double()).abs() <= 3 * 2.0 ** -8 * 3 * ww.double().abs()).all())
+    size = dy.double().abs() @ held(w.detach()).abs() * 3
+    assert bool(((gx.double() - 3 * wx.double()).abs() <= 2.0 ** -8 * (gx.double().abs() + 3 * wx.double().abs()) + 2.02 * 2.0 ** -8 * size).all())
+
+
+def test_gradients_that_are_broadcast_or_lie_anywhere():
+    x, w = rand(4, 16, 512).requires_grad_(), rand(40, 512, seed=2).requires_grad_()
+    wide = rand(4, 16, 83, seed=3)
+    for dy in (torch.ones(1, 1, 1, dtype=BF, device="cuda").expand(4, 16, 40), rand(4, 1, 40, seed=4).expand(4, 16, 40), wide[:, :, 3:43], wide[:, :, 1:81:2],
+               rand(16, 4, 40, seed=5).transpose(0, 1)):
+        for got, want in zip(torch.autograd.grad(I.int8_linear(x, w), [x, w], dy), torch.autograd.grad(I.int8_linear(x, w), [x, w], dy.contiguous())):
+            assert torch.equal(got, want)
+
+
+def training_pass(x, ws, dys):
+    return torch.autograd.grad(I.int8_linear_many(x, ws), [x, *ws], dys)
+
+
+def test_training_is_captured_and_replayed():
+    """Two graphs over the same weights, replayed in turn on new inputs."""
+    ws = [rand(n, 1024, seed=n, std=0.05).requires_grad_() for n in (512, 64)]
+    sets = [(rand(n, 1024, seed=n).requires_grad_(), [rand(n, w.shape[0], seed=n + w.shape[0]) for w in ws]) for n in (70, 2100)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for x, dys in sets:
+            training_pass(x, ws, dys)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x, dys in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(training_pass(x, ws, dys))
+        graphs.append(g)
+    for turn in range(2):
+        for x, _ in sets:
+            with torch.no_grad():
+                x.copy_(rand(*x.shape, seed=50 + turn))
+        with torch.no_grad():
+            ws[0].copy_(rand(512, 1024, seed=60 + turn, std=0.05))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for out, (x, dys) in zip(outs, sets):
+            assert all(torch.equal(a, b) for a, b in zip(out, training_pass(x, ws, dys)))
+    lib.check_status()
+
+
+def test_training_from_two_threads():
+    import threading
+
+    sets = [(rand(n, 1024, seed=n).requires_grad_(), [rand(m, 1024, seed=m, std=0.05).requires_grad_() for m in (512, 64)]) for n in (70, 2100)]
+    dys = [[rand(x.shape[0], w.shape[0], seed=4) for w in ws] for x, ws in sets]
+    want = [training_pass(*s, d) for s, d in zip(sets, dys)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i] = training_pass(*sets[i], dys[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
 
 
 def test_sizes_without_a_kernel_take_the_library():
