@@ -12,7 +12,8 @@
 //
 // What bounds them: few and stream read every weight once, so memory from some 100 MB of weights on (28672 x 4096, one row: 20.8 us, 5.6 TB/s), and below
 // that a launch and the first loads' way (4096 x 4096, one row: 5.2 us; 64 rows of 6144 x 4096: 10.4).  pair is bound by the matrix units and, in long
-// runs, by the power they draw: 8192 x 11008 x 4096 in 245 to 286 us, 2.6 to 3.0 Pop/s, 1.5 to 1.8 times what bf16 gets out of them.
+// runs, by the power they draw: 8192 x 11008 x 4096 in 237 us, 3.1 Pop/s; 8192 x 4096 x 14336 with residual in
+// 315.  From some 2000 columns of K down the results' way to memory counts too: 2000 x 16384 x 2048 53 us, of which the sums 39.
 // Every wait is bounded (common.cuh).
 #include <type_traits>
 
@@ -38,7 +39,7 @@ struct Params {
   long long ldc, ldr;
   int flags;
   int* status;
-  int aligned = 0;  // C is bf16, and 32 columns of it and of the residual from a multiple of 32 on start on 16 bytes in every row
+  int aligned = 0;  // 32 columns of C and of the residual from a multiple of 32 on start on 32 bytes in every row
 };
 
 // Instruction descriptor for kind::i8: signed 8-bit A and B, both K-major, 32-bit whole-number accumulator.
@@ -483,7 +484,8 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
 constexpr int BN = 256, BMP = 256, BMC = 128;
 constexpr int kPairStage = (BMC + BN / 2) * BK;  // per CTA
 constexpr int kPairStages = 6;
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 4 * BN * 4 + 4 * 32 * 33 * 4 + (2 * kPairStages + 4) * 8 + 16;
+constexpr int kTurn = 33;  // from row to row of 32 x 32 numbers in shared memory, which are written by rows and read by columns
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 4 * BN * 4 + 4 * 32 * kTurn * 4 + (2 * kPairStages + 4) * 8 + 16;
 
 __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int& mb, int& nb) {
   constexpr int GM = 4;  // four row tiles stay in the L2 while the raster sweeps N
@@ -492,14 +494,57 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
   nb = r / gm;
 }
 
+// 32 bytes of a row at a time: whole sectors (16 bytes at a time 8192 x 11008 x 4096 takes 277 us instead of 237; by way of shared memory, so that four lanes write
+// 64 bytes of a row together, 265; eight epilogue warps instead of four 291).
+struct Line {
+  uint32_t u[8];
+  __device__ __forceinline__ void load(const void* p) {
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+                 : "l"(p));
+  }
+  __device__ __forceinline__ void store(void* p) const {
+    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]),
+                 "r"(u[7]), "l"(p)
+                 : "memory");
+  }
+};
+// 32 columns of the residual in the lane's row, which are read while the 32 columns before them are written.
+struct Ahead {
+  Line l[4];
+  __device__ __forceinline__ void load(const Params& p, int m, int n) {
+    const long long at = m * p.ldr + n;
+    if (p.flags & kResidualF32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[i].load(reinterpret_cast<const float*>(p.residual) + at + 8 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) l[i].load(reinterpret_cast<const __nv_bfloat16*>(p.residual) + at + 16 * i);
+    }
+  }
+  __device__ __forceinline__ void add(float (&v)[32], bool f32) const {
+    if (f32) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(l[j / 8].u[j % 8]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j += 2) {
+        const uint32_t w = l[j / 16].u[j % 16 / 2];
+        v[j] += __uint_as_float(w << 16);
+        v[j + 1] += __uint_as_float(w & 0xFFFF0000u);
+      }
+    }
+  }
+};
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* s_scale = reinterpret_cast<float*>(smem + kPairStages * kPairStage);  // the columns' scales, of one tile and the next
   float* s_bias = s_scale + 2 * BN;
-  float* s_turn = s_scale + 4 * BN;  // 32 x 32 numbers of every epilogue warp, rows 33 apart
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_turn + 4 * 32 * 33);
+  float* s_turn = s_scale + 4 * BN;  // 32 x 32 numbers of every epilogue warp
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_turn + 4 * 32 * kTurn);
   uint64_t* empty_bar = full_bar + kPairStages;
   uint64_t* tfull_bar = empty_bar + kPairStages;
   uint64_t* tempty_bar = tfull_bar + 2;
@@ -585,7 +630,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   } else {
     // epilogue: a lane has one row of this CTA's 128 and sees it 32 columns at a time
     const int quad = warp & 3;
-    float* turn = s_turn + quad * (32 * 33);
+    float* turn = s_turn + quad * (32 * kTurn);
     int buf = 0;
     uint32_t tphase = 0;
     bool alive = true;
@@ -604,6 +649,9 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         if (p.flags & kBias) s_bias[buf * BN + at] = there ? bias_at(p, nb * BN + at) : 0.f;
       }
       if (in && (p.flags & kResidual)) prefetch_residual(p, m, nb * BN, min(BN, p.N - nb * BN));
+      const int m0 = m - lane, rows = min(32, p.M - m0);
+      Ahead residual;
+      if ((p.flags & kResidual) && p.aligned && nb * BN + 32 <= p.N) residual.load(p, min(m, p.M - 1), nb * BN);
       named_bar_sync(1, 128);
       if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&tfull_bar[buf], tphase, abort_flag, p.status, 300, buf));
       if (!alive) continue;  // the other warps wait for this one at the barrier above, tile by tile
@@ -612,7 +660,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll 1
       for (int c = 0; c < BN; c += 32) {
         const int n0 = nb * BN + c;
-        if (n0 >= p.N) break;
+        if (n0 >= p.N || rows <= 0) break;
         uint32_t r[32];
         tmem_ld_32x32(taddr + c, r);
         tmem_ld_wait();
@@ -634,45 +682,39 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
           }
         }
         if (cols < 32 || !p.aligned) {
-          // Rows that start anywhere, the last columns and fp32 (8192 x 11008 x 4096 347 us row by row, 275 so): through shared memory, so that the lanes hold
-          // neighbouring columns of one row
+          // Rows that start anywhere, and the last columns: through shared memory, so that the lanes hold neighbouring columns of one row
 #pragma unroll
-          for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = v[j];
+          for (int j = 0; j < 32; ++j) turn[lane * kTurn + j] = v[j];
           __syncwarp();
-          const int m0 = m - lane;
-          float* column = turn + lane;
-          finish_rows<32>(p, m0, min(32, p.M - m0), n0 + lane, lane < cols, [&](int i) { return column[i * 33]; });
+          const float* column = turn + lane;
+          finish_rows<32>(p, m0, rows, n0 + lane, lane < cols, [&](int i) { return column[i * kTurn]; });
           __syncwarp();
           continue;
         }
-        if (!in) continue;
         if (p.flags & kResidual) {
-          if (p.flags & kResidualF32) {
-            const float4* rr = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.residual) + m * p.ldr + n0);
+          residual.add(v, p.flags & kResidualF32);
+          if (n0 + 64 <= p.N && c + 32 < BN) residual.load(p, min(m, p.M - 1), n0 + 32);  // the next 32 columns
+        }
+        if (!in) continue;
+        if (p.flags & kOutF32) {
+          float* o = reinterpret_cast<float*>(p.C) + m * p.ldc + n0;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const float4 a = __ldg(rr + q);
-              v[4 * q] += a.x; v[4 * q + 1] += a.y; v[4 * q + 2] += a.z; v[4 * q + 3] += a.w;
-            }
-          } else {
-            const uint4* rr = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + n0);
+          for (int i = 0; i < 4; ++i) {
+            Line l;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint4 a = __ldg(rr + q);
-              const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+            for (int j = 0; j < 8; ++j) l.u[j] = __float_as_uint(v[8 * i + j]);
+            l.store(o + 8 * i);
+          }
+        } else {
+          __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n0;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                v[8 * q + 2 * j] += __uint_as_float(u[j] << 16);
-                v[8 * q + 2 * j + 1] += __uint_as_float(u[j] & 0xFFFF0000u);
-              }
-            }
+          for (int i = 0; i < 2; ++i) {
+            Line l;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) l.u[j] = pack_bf16x2(v[16 * i + 2 * j], v[16 * i + 2 * j + 1]);
+            l.store(o + 16 * i);
           }
         }
-        uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.C) + m * p.ldc + n0);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          o[q] = make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]), pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
-                            pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
       }
       tc_fence_before();
       __syncwarp();
@@ -690,8 +732,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 }
 
 int launch_pair(const void* A, const void* B, long long lda, long long ldb, Params p, cudaStream_t s) {
-  auto whole = [](const void* x, long long ld, bool f32) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld & (f32 ? 3 : 7)) == 0; };
-  p.aligned = !(p.flags & kOutF32) && whole(p.C, p.ldc, false) && (!(p.flags & kResidual) || whole(p.residual, p.ldr, p.flags & kResidualF32));
+  auto whole = [](const void* x, long long ld, bool f32) { return (reinterpret_cast<uintptr_t>(x) & 31) == 0 && (ld & (f32 ? 7 : 15)) == 0; };
+  p.aligned = whole(p.C, p.ldc, p.flags & kOutF32) && (!(p.flags & kResidual) || whole(p.residual, p.ldr, p.flags & kResidualF32));
   CUtensorMap tmA, tmB;
   int rc = make_tmap_2d_u8(&tmA, A, p.M, p.K, lda, BMC);
   if (rc == kErrOk) rc = make_tmap_2d_u8(&tmB, B, p.N, p.K, ldb, BN / 2);
