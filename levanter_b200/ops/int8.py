@@ -341,9 +341,17 @@ def _straight_through(x: torch.Tensor) -> torch.Tensor:
     return x + (quantize_reference(x.detach()).dequantize(torch.float32).to(x.dtype) - x).detach()
 
 
-# Up to so many rows the host's part bounds a layer: the projections of a layer without biases are one product, whose columns are their results, and so are
-# their gradients.  Above it their results are tensors of their own, as their readers expect them.
+# Up to so many rows the host's part bounds a layer: the projections of a layer without biases are one product, whose columns are their results.  Above it their
+# results are tensors of their own, as their readers expect them.
 MANY_ROWS = 2048
+
+
+def _side_by_side(rows: int, cols: int, outs: int) -> bool:
+    """Whether the output gradients of several projections, ``outs`` columns in all, are copied side by side for one product each way.  That moves 4 bytes
+    per row and output; a sum over the projections in fp32 moves 18 or more per row and column.  Forward and backward, us side by side / in fp32: 8192 rows of
+    4096 by 4096 + 1024 + 1024 868 / 1034, 16384 of 2048 by 2048 + 512 + 512 516 / 828, 4096 of 2048 by two of 8192 639 / 682; two of 11008 by
+    8192 rows of 4096 2904 / 2898, by 32768 12731 / 12044."""
+    return rows <= 4096 or outs <= 5 * cols
 
 
 def _hold(x: torch.Tensor, weights: Sequence[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, int]:
@@ -395,8 +403,8 @@ class _Int8ManyFn(torch.autograd.Function):
 
     ``dx = sum dy w'`` and ``dw = dy^T x'`` are bf16 products of what the whole numbers stand for, rounded to bf16 (2^-8 of each value at most, as any operand
     of a bf16 layer); output gradients are not quantised, their rows span too many magnitudes for one scale.  The sum over several projections is rounded
-    once: of few rows their output gradients are laid side by side for one product each way, of many rows it is formed in fp32 (8192 rows of 4096 by two of
-    11008, us in a row of such steps: side by side 1375 to 1414, in fp32 1268 to 1313, rounding what the second product adds to 1158 to 1239)."""
+    once: their output gradients are laid side by side for one product each way (:func:`_side_by_side`), or it is formed in fp32 (8192 rows of 4096 by two of
+    11008 1268 to 1313 us; rounding the first product ahead of the second 1158 to 1239, at the price of a second rounding)."""
 
     @staticmethod
     def forward(ctx, x, count, *tensors):
@@ -430,7 +438,7 @@ class _Int8ManyFn(torch.autograd.Function):
         back = torch.empty(last - first, cols, dtype=torch.bfloat16, device=values.device) if last > first else None
         if back is not None:
             _launch("lvb_int8_dequantize", values, values.data_ptr() + first * ld, ld, scale.data_ptr() + 4 * first, last - first, cols, back.data_ptr(), 0)
-        side = d2[0] if len(live) == 1 else torch.cat(d2, dim=1) if rows <= MANY_ROWS else None
+        side = d2[0] if len(live) == 1 else torch.cat(d2, dim=1) if _side_by_side(rows, cols, sum(d.shape[1] for d in d2)) else None
         dx = None
         if need[0]:
             w = back[rows - first:]

@@ -251,7 +251,7 @@ def held(x):
     return q * s[..., None]
 
 
-@pytest.mark.parametrize("shape,outs,bias", [((1, 64), [8], False), ((5, 7, 768), [256, 1000, 8], False), ((3, 200), [16, 24], True), ((2100, 1024), [512, 528], False),
+@pytest.mark.parametrize("shape,outs,bias", [((1, 64), [8], False), ((5, 7, 768), [256, 1000, 8], False), ((3, 200), [16, 24], True), ((2100, 1024), [512, 528], False), ((4100, 64), [256, 72], False),
                                              ((999, 768), [2304], True), ((2, 3, 1040), [64, 8, 16, 24], False), ((130, 544), [16, 8, 8, 8, 8, 16], False)])
 def test_linear_many_and_its_gradients(shape, outs, bias):
     x = rand(*shape, seed=1).requires_grad_()
