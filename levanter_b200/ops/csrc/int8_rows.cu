@@ -13,8 +13,9 @@
 //   - rows of whole groups of 16 bf16 elements that start on 32 bytes, above 512 and up to 16384 columns: a block per row, one load of 32 bytes per thread
 //     and input (rows16_kernel).  16384 x 4096: norm with residual 73 us (470 MB, 6.4 TB/s), without 48 (4.2), a row as it is 38 (5.3); gated activation of
 //     8192 x 11008 87 (5.2).  A norm without residual waits for its reduction: of 4096 columns it holds half of what an SM could read in that time.
-//   - the others (quantize_kernel): up to 512 columns a warp per row; up to 16384 a block per row, eight elements per thread and turn; beyond that the row
-//     is read twice.  Rows of 4095 or 11007 columns, which start anywhere: norm with residual 200 us, gated activation 200, a row as it is 65.
+//   - the others (quantize_kernel): up to 512 columns a warp per row; up to 16384 a block per row, eight elements per thread and turn; beyond that (norms with
+//     residual: beyond 12288, in fp32 8192) the row is read twice.  Rows of 4095 or 11007 columns, which start anywhere: 16384 x 4095 norm with residual 200 us, a row
+//     as it is 65; gated activation of 8192 x 11007 187.
 //   - back: 31 us for 16384 x 4096 (201 MB, 6.4 TB/s), 42 for 8192 x 11008; rows of odd widths 45 and 58.
 // Few rows are bound by a launch: one row of 4096 takes 2.0 us in a graph.
 #include <initializer_list>
@@ -186,13 +187,15 @@ struct Raw {  // eight elements as they lie in memory, and ahead of them what an
   }
 };
 
-// ---- where a row comes from: load() starts the reads of eight of its elements, get() gives them and adds what the row's factor needs to `ss`.  All
+// ---- where a row comes from: load() starts the reads of eight of its elements, get() gives them and adds what the row's factor needs to `ss`.  kWide: it takes
+// many registers; kMostHeld: the most threads whose registers hold a row (both: quantize()).  All
 // lanes of a warp call get(); `live` of the elements exist (none where it is not positive), the others are zero.
 template <typename T>
 struct Plain {
   Span<T> x;
   using In = Raw<T>;
-  static constexpr bool kSum = false, kTwiceTheRegisters = false;
+  static constexpr bool kSum = false, kWide = false;
+  static constexpr int kMostHeld = 1024;
   __device__ __forceinline__ void load(In& in, long long row, int c, int live) const { in.load(x.p + row * x.ld + c, live, x.lo, x.hi); }
   __device__ __forceinline__ void get(const In& in, long long, int, int, float (&y)[8], F32x2&) const { in.get(y); }
   __device__ __forceinline__ float factor(float) const { return 1.f; }
@@ -209,7 +212,8 @@ struct Norm {
   struct In {
     Raw<T> a, b;  // (without a residual the second is never loaded and takes no register)
   };
-  static constexpr bool kSum = true, kTwiceTheRegisters = kResidual;
+  static constexpr bool kSum = true, kWide = kResidual;
+  static constexpr int kMostHeld = !kResidual ? 1024 : sizeof(T) == 2 ? 768 : 512;
   __device__ __forceinline__ void load(In& in, long long row, int c, int live) const {
     in.a.load(x.p + row * x.ld + c, live, x.lo, x.hi);
     if constexpr (kResidual) in.b.load(r.p + row * r.ld + c, live, r.lo, r.hi);
@@ -255,7 +259,8 @@ struct Glu {
   struct In {
     Raw<T> a, b;
   };
-  static constexpr bool kSum = false, kTwiceTheRegisters = false;
+  static constexpr bool kSum = false, kWide = sizeof(T) == 4;
+  static constexpr int kMostHeld = 1024;
   __device__ __forceinline__ void load(In& in, long long row, int c, int live) const {
     in.a.load(g.p + row * g.ld + c, live, g.lo, g.hi);
     in.b.load(u.p + row * u.ld + c, live, u.lo, u.hi);
@@ -648,13 +653,24 @@ int quantize(const Src& src, long long rows, int cols, void* q, long long ldq, f
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int8_t* o = reinterpret_cast<int8_t*>(q);
   if (cols <= 512) return launch<Src, true, 2, 32 * kRowWarps>(src, rows, cols, 32 * kRowWarps, o, ldq, scale, s);
-  if (cols > kMostThreads * 8 * kHeldGroups) return launch<Src, false, 0, kMostThreads>(src, rows, cols, kMostThreads, o, ldq, scale, s);
   const int threads = ((cols + 7) / 8 + 32 * kHeldGroups - 1) / (32 * kHeldGroups) * 32;
-  // (a norm with a residual has two inputs and an output that start anywhere: with half the threads and twice the registers 16384 x 4095 take 200 us, not 255)
-  if constexpr (Src::kTwiceTheRegisters) {
-    if (threads <= kMostThreads / 2) return launch<Src, false, kHeldGroups, kMostThreads / 2>(src, rows, cols, threads, o, ldq, scale, s);
+  // The fewer threads a form is made for, the more registers each has.  us, 8192 rows: norms with residual, columns 4095 / 11007 / 14335 as forms of 1024 threads
+  // 127 / 474 / 514, of 512 101, of 768 284, read twice by 512 threads (by 1024) 306 (417) for 11007 and 399 (445) for 14335; fp32, 11008 / 14336: 456 / 544, of 768 450,
+  // read twice 268 (371) / 367 (424).  Gated activations of 4096 rows in fp32, 4096 / 11008 columns 38 / 136, of 512 and 768 26 / 106; in bf16, 8192 rows of 8191
+  // / 11007 115 / 201, of 512 171, of 768 187.  Norms without a residual, 11007 columns 165, of 768 146.
+  constexpr int kMost = Src::kMostHeld, kHalf = kMostThreads / 2;
+  if (threads > kMost) {
+    constexpr int kTwice = kMost < kMostThreads ? kHalf : kMostThreads;
+    return launch<Src, false, 0, kTwice>(src, rows, cols, kTwice, o, ldq, scale, s);
   }
-  return launch<Src, false, kHeldGroups, kMostThreads>(src, rows, cols, threads, o, ldq, scale, s);
+  if constexpr (Src::kWide) {
+    if (threads <= kHalf) return launch<Src, false, kHeldGroups, kHalf>(src, rows, cols, threads, o, ldq, scale, s);
+  }
+  if constexpr (kMost >= 768) {
+    if (threads <= 768 && (Src::kWide || threads > kHalf)) return launch<Src, false, kHeldGroups, 768>(src, rows, cols, threads, o, ldq, scale, s);
+  }
+  if constexpr (kMost == kMostThreads) return launch<Src, false, kHeldGroups, kMostThreads>(src, rows, cols, threads, o, ldq, scale, s);
+  return kErrBadArg;  // (not reached: the forms above hold every row up to kMost threads)
 }
 
 // out = q * scale, rounded once, for dense rows `out`.  kGroup elements per thread: 16 of aligned rows of whole groups of 16, else 8, and those may lie
