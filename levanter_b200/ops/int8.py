@@ -530,6 +530,7 @@ class Int8Linear(nn.Module):
 
 class Int8ServingLinear(nn.Module):
     """A projection that serves: its weights are held in 8 bits (buffers ``weight`` int8 ``[out, in]`` and ``weight_scale`` fp32 ``[out]``) and have no gradient.
+    A state with the weight in another type is quantised as it is loaded.
     It takes rows in bf16 or fp32 and gives results of their type, or :class:`Int8Rows` that several projections share (results in bf16), and adds a ``residual`` in
     its product's epilogue."""
 
@@ -557,6 +558,13 @@ class Int8ServingLinear(nn.Module):
         if self.weight_scale.dtype != torch.float32:  # a model's conversion to another type leaves the scales as they are
             self.weight_scale = scale.to(self.weight.device)
         return self
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        w = state_dict.get(prefix + "weight")
+        if w is not None and w.is_floating_point() and w.shape == self.weight.shape:  # of a model that was not quantised
+            rows = _quantize(w.detach().to(self.weight.device, torch.bfloat16 if w.dtype is torch.bfloat16 else torch.float32))
+            state_dict[prefix + "weight"], state_dict[prefix + "weight_scale"] = rows
+        super()._load_from_state_dict(state_dict, prefix, *args)
 
     def forward(self, x: Union[torch.Tensor, Int8Rows], *, skip_bias: bool = False, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         return int8_product(as_int8_rows(x), self.rows, None if skip_bias else self.bias, residual, out_dtype=x.dtype)

@@ -261,3 +261,25 @@ def test_scales_that_want_a_gradient_are_refused(call):
 def test_rows_without_elements_come_back_empty():
     assert I.Int8Rows(torch.empty(3, 0, dtype=torch.int8), torch.empty(3)).dequantize().shape == (3, 0)
     assert I.quantize_rows(torch.empty(0, 16)).dequantize().shape == (0, 16)
+
+
+def test_weights_of_a_model_that_was_not_quantised_are_quantised_as_they_load():
+    plain = llama().build(100, seed=1)
+    want = quantize_for_serving(copy.deepcopy(plain), QuantizationConfig(int8=True))
+    model = quantize_for_serving(llama().build(100, seed=0), QuantizationConfig(int8=True))
+    state = plain.state_dict()
+    before = {k: v.clone() for k, v in state.items()}
+    model.load_state_dict(state)
+    assert state.keys() == before.keys() and all(torch.equal(state[k], before[k]) for k in state)
+    for (n, a), (_, b) in zip(model.state_dict().items(), want.state_dict().items()):
+        assert a.dtype == b.dtype and torch.equal(a, b), n
+    with pytest.raises(RuntimeError):
+        I.Int8ServingLinear(torch.zeros(8, 20), None).load_state_dict({"weight": torch.zeros(8, 21)})
+
+
+def test_engine_config_takes_the_quantization_from_a_file():
+    from levanter_b200.config import decode
+    from levanter_b200.inference.engine import InferenceEngineConfig
+
+    cfg = decode(InferenceEngineConfig, {"max_seqs": 2, "quantization": {"int8": True, "targets": ["mlp"]}})
+    assert cfg.quantization.int8 and cfg.quantization.matches("layers.0.mlp.up_proj") and not cfg.quantization.matches("layers.0.self_attn.q_proj")
