@@ -283,3 +283,39 @@ def test_engine_config_takes_the_quantization_from_a_file():
 
     cfg = decode(InferenceEngineConfig, {"max_seqs": 2, "quantization": {"int8": True, "targets": ["mlp"]}})
     assert cfg.quantization.int8 and cfg.quantization.matches("layers.0.mlp.up_proj") and not cfg.quantization.matches("layers.0.self_attn.q_proj")
+
+
+@pytest.mark.parametrize("family", ["fedolorn", "zadepel", "zosipel", "mumizen"])
+@pytest.mark.parametrize("name", ["mixed", "odd"])
+def test_other_decoders_serve_weights_held_in_8_bits(family, name, tmp_path):
+    """Attention without positions, with gates, windows, differences and mixed values: the tokens are those of the same layers as training computes them."""
+    import importlib
+    import json
+
+    import test_fedolorn as F
+    from levanter_b200.inference.engine import Request
+    from levanter_b200.inference.jit_scheduler import SeqDecodingParams
+    from levanter_b200.layers.attention import Attention
+    from levanter_b200.models.llama import LlamaMlp
+    from safetensors.torch import save_file
+
+    cfg = importlib.import_module(f"test_{family}")._config(name)
+    (tmp_path / "config.json").write_text(json.dumps(cfg))
+    save_file(importlib.import_module(f"{family}_oracle").random_weights(cfg, seed=3), str(tmp_path / "model.safetensors"))
+    place = ("cpu", torch.float32)
+    tokens, counts = [], []
+    with torch.no_grad():
+        for serving in (False, True):
+            model = F._load(str(tmp_path), place)
+            if serving:
+                quantize_for_serving(model, QuantizationConfig(int8=True))
+            else:
+                for m in [m for m in model.modules() if isinstance(m, (Attention, LlamaMlp))]:
+                    for child_name, child in list(m.named_children()):
+                        if type(child) is Linear:
+                            setattr(m, child_name, I.Int8Linear.from_linear(child))
+            counts.append(sum(isinstance(m, (I.Int8Linear, I.Int8ServingLinear)) for m in model.modules()))
+            prompts = [[1, 2, 3, 4, 5, 6, 7], [9, 8, 7]]
+            reqs = [Request(prompt_tokens=p, request_id=i, decode_params=SeqDecodingParams(len(p) + 6, None, 0.0, i), n_generations=1) for i, p in enumerate(prompts)]
+            tokens.append(F._engine(model, place).generate(reqs).tokens)
+    assert counts[0] == counts[1] > 0 and tokens[0] == tokens[1]
