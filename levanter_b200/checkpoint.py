@@ -30,6 +30,7 @@ from fsspec.core import url_to_fs
 
 from . import tensorstore_serialization as tss
 from .distributed import broadcast_one_to_all
+from .quantization import check_not_quantized
 from .utils import fsspec_utils
 
 logger = logging.getLogger(__name__)
@@ -187,6 +188,8 @@ def save_checkpoint(tree: Any, step: int, checkpoint_path: PathLike, manager: Op
                     commit_callback: Optional[Callable[[], None]] = None, is_temporary: bool = False,
                     layouts: Optional[Dict[str, tss.ParamLayout]] = None):
     """Write ``tree`` under ``checkpoint_path``; ``metadata.json`` is written by process 0 once every leaf is durable."""
+    if isinstance(tree, torch.nn.Module):
+        check_not_quantized(tree, "save_checkpoint")
     checkpoint_path = str(checkpoint_path)
     fsspec_utils.mkdirs(checkpoint_path)
 
@@ -282,6 +285,7 @@ def load_checkpoint(state, checkpoint_path: PathLike, *, subpath: Optional[str] 
 def load_model_params(model: torch.nn.Module, checkpoint_path: str, prefix: str = "model", *, allow_partial: bool = False,
                       only: Optional[Callable[[str], bool]] = None) -> List[str]:
     """Copy parameters from a reference-layout checkpoint into ``model``.  Returns the names that were missing."""
+    check_not_quantized(model, "load_model_params")
     layouts = tss.layouts_of(model)
     missing = []
     with torch.no_grad():

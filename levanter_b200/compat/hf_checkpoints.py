@@ -26,6 +26,7 @@ import torch
 import torch.nn as nn
 
 from ..models.lm_model import LmConfig, LmHeadModel
+from ..quantization import check_not_quantized
 from ..utils import fsspec_utils
 
 logger = logging.getLogger(__name__)
@@ -104,6 +105,7 @@ def _hf_name(torch_name: str, key_map: Dict[str, Optional[str]]) -> str:
 
 def to_hf_state_dict(model: nn.Module, dtype: Optional[torch.dtype] = None, params: Optional[Dict[str, torch.Tensor]] = None) -> Dict[str, torch.Tensor]:
     """HF-named, HF-shaped tensors of ``model`` (CPU).  ``params`` overrides the values (e.g. fp32 master weights)."""
+    check_not_quantized(model, "to_hf_state_dict")
     key_map = model.hf_key_map() if hasattr(model, "hf_key_map") else {}
     out: Dict[str, torch.Tensor] = {}
     for name, p in model.named_parameters():
@@ -135,6 +137,7 @@ def to_hf_state_dict(model: nn.Module, dtype: Optional[torch.dtype] = None, para
 def load_hf_state_dict(model: nn.Module, state_dict: Dict[str, torch.Tensor], *, strict: bool = True,
                        ignore_prefix: Optional[str] = None) -> List[str]:
     """Copy HF tensors into ``model``.  Returns the names of model parameters that had no counterpart."""
+    check_not_quantized(model, "load_hf_state_dict")
     key_map = model.hf_key_map() if hasattr(model, "hf_key_map") else {}
 
     def lookup(name: str) -> Optional[torch.Tensor]:

@@ -467,7 +467,7 @@ int launch_stream(const void* A, const void* B, long long lda, long long ldb, co
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.N + 127) / 128 * splits), static_cast<unsigned>(row_tiles));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = 3072 + bytes;
+  cfg.dynamicSmemBytes = 3 * 1024 + bytes;  // alignment, barriers and scales ahead of the ring
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -90,3 +90,12 @@ def quantize_for_serving(model: nn.Module, config: QuantizationConfig) -> nn.Mod
     if held == 0:
         raise ValueError("no projection of an attention or MLP layer matches the quantization targets")
     return model
+
+
+def check_not_quantized(model: nn.Module, what: str) -> None:
+    """Refuses ``what`` of a model that serves: weights held in 8 bits are not parameters, so it would pass them over."""
+    from .ops.int8 import Int8ServingLinear
+
+    for name, m in model.named_modules():
+        if type(m) is Int8ServingLinear:
+            raise ValueError(f"{what}: the weight of {name} is held in 8 bits; use the model as it was before quantize_for_serving")

@@ -319,3 +319,16 @@ def test_other_decoders_serve_weights_held_in_8_bits(family, name, tmp_path):
             reqs = [Request(prompt_tokens=p, request_id=i, decode_params=SeqDecodingParams(len(p) + 6, None, 0.0, i), n_generations=1) for i, p in enumerate(prompts)]
             tokens.append(F._engine(model, place).generate(reqs).tokens)
     assert counts[0] == counts[1] > 0 and tokens[0] == tokens[1]
+
+
+def test_checkpoints_neither_read_nor_write_weights_held_in_8_bits(tmp_path):
+    from levanter_b200.checkpoint import load_model_params, save_checkpoint
+    from levanter_b200.compat.hf_checkpoints import load_hf_state_dict, to_hf_state_dict
+
+    model = llama().build(100, seed=0)
+    state = to_hf_state_dict(model)
+    quantize_for_serving(model, QuantizationConfig(int8=True))
+    for call in (lambda: to_hf_state_dict(model), lambda: load_hf_state_dict(model, state), lambda: load_model_params(model, str(tmp_path)),
+                 lambda: save_checkpoint(model, 0, str(tmp_path / "out"))):
+        with pytest.raises(ValueError, match="held in 8 bits"):
+            call()
