@@ -102,6 +102,7 @@ def test_product_is_exact_in_whole_numbers():
     (lambda x, w: I.Int8ServingLinear(torch.ones(3, 16).half(), None), ValueError),
     (lambda x, w: quantize_for_serving(Linear(8, 8), QuantizationConfig(int8=True)), ValueError),
     (lambda x, w: quantize_for_serving(Linear(8, 8), QuantizationConfig(fp8=True)), ValueError),
+    (lambda x, w: quantize_linear_layers(Linear(8, 8), QuantizationConfig(fp8=True, int8=True)), ValueError),
 ])
 def test_refusals(call, error):
     torch.manual_seed(3)
@@ -256,6 +257,14 @@ def test_scales_that_want_a_gradient_are_refused(call):
         call(rows)
     with torch.no_grad():
         call(rows)
+
+
+def test_a_single_row_without_a_leading_dimension():
+    x, w, bias = torch.randn(20), I.quantize_rows(torch.randn(7, 20)), torch.randn(7)
+    row = I.quantize_rows(x)
+    assert row.scale.shape == () and I.int8_product(row, w, bias).shape == (7,)
+    assert torch.equal(I.int8_product(row, w, bias), I.int8_product(I.quantize_rows(x[None]), w, bias)[0])
+    assert torch.equal(I.rms_norm_int8(x, None, residual=x)[1], x + x) and row.dequantize().shape == (20,)
 
 
 def test_rows_without_elements_come_back_empty():

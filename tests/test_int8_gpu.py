@@ -505,6 +505,26 @@ def test_on_other_streams_and_from_two_threads():
     lib.check_status()
 
 
+def test_calls_through_ctypes_give_the_same(monkeypatch):
+    """Where Python's headers are missing the library is called without the module that launches faster."""
+    ops = half_layer_operands(9, 1024, 768)
+    want, rows = half_layer(*ops), I.quantize_rows(ops[0])
+    monkeypatch.setattr(lib, "_launcher", lambda: None)
+    monkeypatch.setattr(lib, "_quick", {})
+    monkeypatch.setattr(I, "_f", {})
+    assert torch.equal(half_layer(*ops), want) and torch.equal(I.quantize_rows(ops[0]).values, rows.values) and torch.equal(rows.dequantize(F32), rows.values * rows.scale[:, None])
+
+
+def test_a_single_row_without_a_leading_dimension():
+    x, w, bias = rand(333), I.quantize_rows(rand(7, 333, seed=2)), rand(7, seed=3)
+    for row in (I.quantize_rows(x), I.Int8Rows(I.quantize_rows(rand(2, 700, seed=4)).values[1, 9:342], torch.tensor(0.5, device="cuda"))):
+        want = (row.values.double() @ w.values.double().t()) * row.scale.double() * w.scale.double() + bias.double()
+        got = I.int8_product(row, w, bias, out_dtype=F32)
+        # a product of three numbers and a sum: one rounding each
+        assert got.shape == (7,) and bool(((got.double() - want).abs() <= 2.0 ** -22 * (want.abs() + 2 * bias.double().abs())).all())
+        assert torch.equal(row.dequantize(F32), row.values * row.scale)
+
+
 def test_inputs_are_left_as_they_are_and_results_are_new():
     x, r, w, gu, down = half_layer_operands(9, 512, 256)
     before = [t.clone() for t in (x, r, w, gu.values, gu.scale, down.values, down.scale)]
