@@ -12,7 +12,7 @@
 // between the reduction and the write, and the reads of a block's next row are under way meanwhile:
 //   - rows of whole groups of 16 bf16 elements that start on 32 bytes, above 512 and up to 16384 columns: a block per row, one load of 32 bytes per thread
 //     and input (rows16_kernel).  16384 x 4096: norm with residual 73 us (470 MB, 6.4 TB/s), without 48 (4.2), a row as it is 38 (5.3); gated activation of
-//     8192 x 11008 87 (5.2).  A norm without residual waits for its reduction: of 4096 columns it holds half of what an SM could read in that time.
+//     8192 x 11008 84 (5.4).  A norm without residual waits for its reduction: of 4096 columns it holds half of what an SM could read in that time.
 //   - the others (quantize_kernel): up to 512 columns a warp per row; up to 16384 a block per row, eight elements per thread and turn; beyond that (norms with
 //     residual: beyond 12288, in fp32 8192) the row is read twice.  Rows of 4095 or 11007 columns, which start anywhere: 16384 x 4095 norm with residual 200 us, a row
 //     as it is 65; gated activation of 8192 x 11007 187.
@@ -306,7 +306,7 @@ struct Plain16 {  // rows of up to five matrices, one behind the other: those fr
   struct In {
     Raw16 x;
   };
-  static constexpr bool kSum = false;
+  static constexpr bool kSum = false, kTwoBlocks = false;
   __device__ __forceinline__ void load(In& in, long long at, int row) const {
     long long o = off[0];
 #pragma unroll
@@ -329,7 +329,7 @@ struct Norm16 {
   struct In {
     Raw16 x, r;
   };
-  static constexpr bool kSum = true;
+  static constexpr bool kSum = true, kTwoBlocks = true;
   __device__ __forceinline__ void load(In& in, long long at, int) const {
     in.x.load(x + at);
     if constexpr (kResidual) in.r.load(r + at);
@@ -372,7 +372,7 @@ struct Glu16 {
   struct In {
     Raw16 g, u;
   };
-  static constexpr bool kSum = false;
+  static constexpr bool kSum = false, kTwoBlocks = true;
   __device__ __forceinline__ void load(In& in, long long at, int) const {
     in.g.load(g + at);
     in.u.load(u + at);
@@ -551,9 +551,10 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(Src src, long long r
   }
 }
 
-// Aligned rows of whole groups of 16 elements, a thread has one: 32 bytes of each input in one load.
-template <class Src>
-__global__ void __launch_bounds__(kMostThreads) rows16_kernel(Src src, long long ld, int rows, int cols, int8_t* __restrict__ q, long long ldq,
+// Aligned rows of whole groups of 16 elements, a thread has one: 32 bytes of each input in one load.  kAhead: the next row's are started ahead of this one's
+// reduction; else two blocks per SM of up to 768 threads.
+template <class Src, bool kAhead>
+__global__ void __launch_bounds__(kAhead ? kMostThreads : 768, kAhead ? 1 : 2) rows16_kernel(Src src, long long ld, int rows, int cols, int8_t* __restrict__ q, long long ldq,
                                                               float* __restrict__ scale) {
   __shared__ uint32_t s_top[2][32];
   __shared__ float s_ss[2][32];
@@ -570,17 +571,18 @@ __global__ void __launch_bounds__(kMostThreads) rows16_kernel(Src src, long long
   int row = blockIdx.x;
   long long at = row * ld + c;
   typename Src::In in;
-  if (mine) src.load(in, at, row);
+  if (kAhead && mine) src.load(in, at, row);
   for (int odd = 0; row < rows; row += step, odd ^= 1) {
     float y[16] = {};
     F32x2 ss2 = f2(0.f, 0.f);
     float largest = 0.f;
     if (mine) {
+      if constexpr (!kAhead) src.load(in, at, row);
       src.get(in, at, c, y, ss2);
 #pragma unroll
       for (int j = 0; j < 16; j += 2) largest = largest_of(largest, y[j], y[j + 1]);
       at += step * ld;
-      if (row + step < rows) src.load(in, at, row + step);
+      if (kAhead && row + step < rows) src.load(in, at, row + step);
     }
     uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
     float ss = warp_ss<Src::kSum>(ss2);
@@ -628,15 +630,25 @@ int launch(const Src& src, long long rows, int cols, int threads, int8_t* q, lon
              : kErrCuda;
 }
 
+template <class Src, bool kAhead>
+int launch16(const Src& src, long long ld, long long rows, int cols, int threads, void* q, long long ldq, float* scale, void* stream) {
+  const long long most = static_cast<long long>(num_sms()) * resident_blocks<rows16_kernel<Src, kAhead>>(threads, 0);
+  return launch_chained(rows16_kernel<Src, kAhead>, dim3(static_cast<unsigned>(rows < most ? rows : most)), dim3(threads), 0, reinterpret_cast<cudaStream_t>(stream), src,
+                        ld, static_cast<int>(rows), cols, reinterpret_cast<int8_t*>(q), ldq, scale) == cudaSuccess
+             ? kErrOk
+             : kErrCuda;
+}
+
 template <class Src>
 int quantize16(const Src& src, long long ld, long long rows, int cols, void* q, long long ldq, float* scale, void* stream) {
   if (rows <= 0 || q == nullptr || scale == nullptr || (ldq & 15) || ldq < cols || (reinterpret_cast<uintptr_t>(q) & 15)) return kErrBadArg;
   const int threads = (cols / 16 + 31) / 32 * 32;
-  const long long most = static_cast<long long>(num_sms()) * resident_blocks<rows16_kernel<Src>>(threads, 0);
-  return launch_chained(rows16_kernel<Src>, dim3(static_cast<unsigned>(rows < most ? rows : most)), dim3(threads), 0, reinterpret_cast<cudaStream_t>(stream), src, ld,
-                        static_cast<int>(rows), cols, reinterpret_cast<int8_t*>(q), ldq, scale) == cudaSuccess
-             ? kErrOk
-             : kErrCuda;
+  // Of 513 to 768 threads with 64 registers an SM has one block, which stands still at its barrier; with 40, which the next row does not fit into, two.  us, one / two
+  // blocks, 8192 rows of 11008: gated activation 88 / 84, norm with residual 112 / 107, without 76 / 73, but a row as it is 60 / 67.
+  if constexpr (Src::kTwoBlocks) {
+    if (threads > kMostThreads / 2 && threads <= 768) return launch16<Src, false>(src, ld, rows, cols, threads, q, ldq, scale, stream);
+  }
+  return launch16<Src, true>(src, ld, rows, cols, threads, q, ldq, scale, stream);
 }
 
 // Whether rows are of whole groups of 16 elements, few enough for a block and more than a warp takes, start on 32 bytes and have one stride.
