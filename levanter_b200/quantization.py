@@ -69,7 +69,7 @@ def quantize_linear_layers(model: nn.Module, config: QuantizationConfig) -> nn.M
 
 def quantize_for_serving(model: nn.Module, config: QuantizationConfig) -> nn.Module:
     """Hold the weights of the targeted projections of attention and MLP layers in 8 bits, one scale per output channel (in place; returns the model).  The
-    model serves from then on: those weights are not parameters any more.  A model that is quantised already comes back as it is."""
+    model serves from then on: those weights are not parameters any more, and engines made of it before (their CUDA graphs read the old weights) are done.  A model that is quantised already comes back as it is."""
     if config.fp8:
         raise ValueError("serving holds weights in 8-bit integers: use QuantizationConfig(int8=True)")
     if not config.int8:
