@@ -469,7 +469,8 @@ class _Int8ManyFn(torch.autograd.Function):
 
 def int8_linear_many(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: Optional[Sequence[Optional[torch.Tensor]]] = None) -> Tuple[torch.Tensor, ...]:
     """``[x' w'^T + b for w, b in ...]`` with ``x [..., in]`` and the ``weights [out, in]`` held in 8 bits (``x'``, ``w'``: what their whole numbers stand for);
-    differentiable in ``x``, weights and biases.  bf16 with sizes that are multiples of 8 runs on the kernels, everything else on PyTorch's operations."""
+    differentiable in ``x``, weights and biases.  bf16 with sizes that are multiples of 8 runs on the kernels, everything else on PyTorch's operations.  Of several
+    projections without biases of up to ``MANY_ROWS`` rows the results are columns of one tensor: each has the others' columns between its rows."""
     weights = list(weights)
     biases = [None] * len(weights) if biases is None else list(biases)
     if not weights or len(biases) != len(weights):
