@@ -29,6 +29,7 @@ namespace int8_rows {
 
 constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100
 constexpr float kLeast = 7.52316384526264e-37f;  // 2^-120: 127 over it is still a finite number
+constexpr float kMostScale = 0x1.020406p+121f;   // times 127 it is still a finite number
 
 enum Act : int { kSilu = 0, kGeluTanh = 1, kGelu = 2, kRelu = 3, kQuickGelu = 4 };
 
@@ -409,10 +410,12 @@ __device__ __forceinline__ uint2 whole8(const float* y, float top, float inv) {
     b[j + 1] = __float_as_uint(m1);
   }
   if (far > 0.4999f) {  // is 127 y above, on or below the border of two whole numbers, (floor + 1/2) max |y|?
+    const bool large = top >= 1e30f;  // both sides 2^-20 times, so that neither runs over
+    const float t = large ? top * 9.5367431640625e-07f : top, by = large ? 127.f * 9.5367431640625e-07f : 127.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float border = floorf(y[j] * inv) + 0.5f;
-      const float above = fmaf(-border, top, y[j] * 127.f);
+      const float above = fmaf(-border, t, y[j] * by);
       b[j] = __float_as_uint(__fadd_rn(above > 0.f ? border + 0.5f : above < 0.f ? border - 0.5f : border, kMagic));
     }
   }
@@ -439,6 +442,10 @@ struct RowScale {
     inv = !live ? 0.f : most < 1e30f ? __fdividef(127.f, most) : 127.f / most;
     scale = most * f;
     if (!live) scale = finite ? 0.f : __uint_as_float(0x7FC00000u);
+  }
+  __device__ __forceinline__ float step() const {  // (NaN stays)
+    const float s = scale / 127.f;
+    return s > kMostScale ? kMostScale : s;
   }
   __device__ __forceinline__ void put(int8_t* out, const float (&v)[8]) const {
     *reinterpret_cast<uint2*>(out) = live ? whole8(v, most, inv) : make_uint2(0, 0);
@@ -547,7 +554,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(Src src, long long r
         if (c < cols) r.put(out + c, y[0]);
       }
     }
-    if (t == 0) scale[row] = r.scale / 127.f;
+    if (t == 0) scale[row] = r.step();
   }
 }
 
@@ -602,7 +609,7 @@ __global__ void __launch_bounds__(kAhead ? kMostThreads : 768, kAhead ? 1 : 2) r
       }
       *reinterpret_cast<uint4*>(q + row * ldq + c) = make_uint4(a.x, a.y, b.x, b.y);
     }
-    if (threadIdx.x == 0) scale[row] = r.scale / 127.f;
+    if (threadIdx.x == 0) scale[row] = r.step();
   }
 }
 

@@ -26,6 +26,7 @@ from . import lib
 from .glu import _ACT, GatedActivation, gated_activation
 
 TINY = 2.0 ** -100
+MOST_SCALE = float.fromhex("0x1.020406p+121")  # the largest scale whose 127-fold is an fp32 number
 MAX_COLS = 131071  # 128 * 128 * cols has to fit into the 32-bit sums
 _FLOATS = (torch.bfloat16, torch.float32)
 _f = {}
@@ -185,8 +186,8 @@ def quantize_reference(y: torch.Tensor, factor: Optional[torch.Tensor] = None) -
     top = y.abs().amax(-1, keepdim=True)
     most = top if factor is None else top * factor
     live = (most >= TINY) & (top >= 2.0 ** -120)
-    q = torch.where(live & torch.isfinite(top), torch.round(y * 127.0 / top), torch.zeros_like(y))
-    scale = torch.where(live, most / 127.0, torch.zeros_like(most))
+    q = torch.where(live & torch.isfinite(top), torch.round(y.double() * 127.0 / top.double()).float(), torch.zeros_like(y))  # (fp32 would run over)
+    scale = torch.where(live, (most / 127.0).clamp_max(MOST_SCALE), torch.zeros_like(most))
     ok = torch.isfinite(top) & ~torch.isnan(most)
     scale = torch.where(ok, scale, torch.full_like(scale, float("nan")))
     values = _room(y.shape, torch.int8, y.device)

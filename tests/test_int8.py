@@ -44,6 +44,16 @@ def test_special_rows():
     assert rows.scale[:2].tolist() == [0, 0] and rows.scale[2:4].isnan().all() and not rows.values[:4].any() and rows.values[4, 5] == 127
 
 
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_rows_of_the_largest_numbers(dtype):
+    m = torch.finfo(dtype).max  # as masks have it
+    x = torch.tensor([[m, m / 2, -m / 2, m / 4, -m, m / 127 * 3, 1.0, 0.0], [-m] * 8], dtype=dtype)
+    rows = I.quantize_rows(x)
+    assert torch.equal(rows.values.double(), (127 * x.double() / x.double().abs().amax(-1, keepdim=True)).round())
+    back = rows.dequantize(torch.float32)
+    assert bool(back.isfinite().all()) and bool(((back[:, 4].double() + m).abs() <= 2.0 ** -22 * m).all())
+
+
 def test_norm_with_its_residual_and_gated_activation():
     torch.manual_seed(1)
     x, r, w = torch.randn(6, 48).to(BF), torch.randn(6, 48).to(BF), (1 + 0.1 * torch.randn(48)).to(BF)

@@ -85,6 +85,20 @@ def test_rows_of_zeros_tiny_values_infinities_and_nan():
     assert empty.shape == (0, 64) and empty.dequantize().shape == (0, 64)
 
 
+@pytest.mark.parametrize("cols", [64, 1000, 4096, 9007])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_of_the_largest_numbers(cols, dtype):
+    m = torch.finfo(dtype).max  # as masks have it
+    x = (rand(3, cols, seed=6, dtype=F32).clamp(-1, 1) * m).to(dtype).clamp(-m, m)
+    x[:, :7] = torch.tensor([m, m / 2, -m / 2, m / 4, -m, m / 127 * 3, 1.0], dtype=dtype)
+    x[1] = -m
+    x[2, 7:] = torch.arange(cols - 7, device="cuda").remainder(254).sub(127).double().add(0.5).mul(m).div(127).to(dtype)  # close to ties
+    rows = I.quantize_rows(x)
+    check_rows(rows, x, slack=0.0 if dtype == BF else 2.0 ** -23)
+    back = rows.dequantize(F32)
+    assert bool(back.isfinite().all()) and bool(((back[:, 4].double() + m).abs() <= 2.0 ** -22 * m).all())
+
+
 @pytest.mark.parametrize("rows,cols", SIZES)
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("residual", [False, True])
