@@ -1,7 +1,8 @@
 // Products of rows held in 8 bits: C[M,N] = (A[M,K] B[N,K]^T) scale_a[M] scale_b[N] (+ bias[N]) (+ residual[M,N]) for int8 A and B.
 //
 // The sums are whole numbers in 32 bits and exact (K <= 131071, as 128 * 128 * K has to fit), so their order and any split of them change nothing.
-// The scales are applied once, to the sum, in fp32; then bias and residual are added and the result is rounded once.
+// The scales are applied once, to the sum, in fp32 (a row of very large numbers in two steps, see times_scales); then bias and residual are added and the
+// result is rounded once.
 //
 // Three kernels, for rows of activations that are few, some or many:
 //   few     up to 16 rows: a stream over the weights, which the lanes read straight into the fragments of warp-level matrix instructions;
@@ -68,9 +69,16 @@ __device__ __forceinline__ float bias_at(const Params& p, int n) {
   return (p.flags & kBiasF32) ? __ldg(reinterpret_cast<const float*>(p.bias) + n)
                               : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p.bias) + n));
 }
+// Rows of very large numbers (bf16 reaches 3e38): sum * sa may run over where sum * sa * sb does not.  2^-32 of such a scale does not, and the 2^32 at
+// the end are exact, so that other rows' results are the same bits with and without them.
+constexpr float kLargeScale = 0x1p+64f, kDown = 0x1p-32f, kUp = 0x1p+32f;
+__device__ __forceinline__ float times_scales(int sum, float sa, float sb, float bias) {
+  const float v = static_cast<float>(sum) * sa * sb + bias;
+  return fabsf(v) <= 3.402823466e+38f ? v : static_cast<float>(sum) * (sa * kDown) * sb * kUp + bias;
+}
 // One element of the result: the sum of whole numbers, its scales, bias and residual.
 __device__ __forceinline__ void finish(const Params& p, int m, int n, int sum, float sa, float sb, float bias) {
-  float v = static_cast<float>(sum) * sa * sb + bias;
+  float v = times_scales(sum, sa, sb, bias);
   if (p.flags & kResidual)
     v += (p.flags & kResidualF32) ? __ldg(reinterpret_cast<const float*>(p.residual) + m * p.ldr + n)
                                   : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + n));
@@ -125,7 +133,7 @@ __device__ __forceinline__ void finish_rows(const Params& p, int m, int live, in
 }
 template <int kRows>
 __device__ __forceinline__ void finish_column(const Params& p, int m, int live, int n, bool in, const int (&sum)[kRows], const float* sa, float sb, float bias) {
-  finish_rows<kRows>(p, m, live, n, in, [&](int j) { return static_cast<float>(sum[j]) * sa[j] * sb + bias; });
+  finish_rows<kRows>(p, m, live, n, in, [&](int j) { return times_scales(sum[j], sa[j], sb, bias); });
 }
 // Brings `columns` of the residual from row m, column n on (which exist) into the L2 while the sums are still being made.
 __device__ __forceinline__ void prefetch_residual(const Params& p, int m, int n, int columns) {
@@ -639,7 +647,9 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       tile_coords(t, tiles_m, tiles_n, mb, nb);
       const int m = mb * BMP + static_cast<int>(cta) * BMC + quad * 32 + lane;
       const bool in = m < p.M;
-      const float sa = in ? __ldg(p.scale_a + m) : 0.f;
+      float sa = in ? __ldg(p.scale_a + m) : 0.f;
+      const bool large = fabsf(sa) > kLargeScale, any_large = __any_sync(0xffffffffu, large);  // as in times_scales()
+      if (large) sa *= kDown;
       float* sb = s_scale + buf * BN;  // (the tile before the last one read it, and all four warps have been at a barrier since)
 #pragma unroll
       for (int j = 0; j < BN; j += 128) {
@@ -673,6 +683,11 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
           v[4 * q + 1] = static_cast<float>(static_cast<int>(r[4 * q + 1])) * sa * f.y;
           v[4 * q + 2] = static_cast<float>(static_cast<int>(r[4 * q + 2])) * sa * f.z;
           v[4 * q + 3] = static_cast<float>(static_cast<int>(r[4 * q + 3])) * sa * f.w;
+        }
+        if (any_large) {
+          const float up = large ? kUp : 1.f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= up;
         }
         if (p.flags & kBias) {
 #pragma unroll

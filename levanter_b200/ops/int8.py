@@ -302,7 +302,9 @@ def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dty
     if torch.is_grad_enabled():
         _no_gradient("int8_product", sv, sw, bias, residual)
     if not _kernels(v):
-        y = torch.matmul(v.double(), w.double().t()).float() * sv.unsqueeze(-1) * sw
+        sums, sv = torch.matmul(v.double(), w.double().t()).float(), sv.unsqueeze(-1)
+        y = sums * sv * sw
+        y = torch.where(torch.isfinite(y), y, sums * (sv * 2.0 ** -32) * sw * 2.0 ** 32)  # rows of very large numbers run over in the first product
         for t in (bias, residual):
             y = y if t is None else y + t.float()
         return y.to(out_dtype)

@@ -351,3 +351,18 @@ def test_checkpoints_neither_read_nor_write_weights_held_in_8_bits(tmp_path):
                  lambda: save_checkpoint(model, 0, str(tmp_path / "out"))):
         with pytest.raises(ValueError, match="held in 8 bits"):
             call()
+
+
+@pytest.mark.parametrize("swap", [False, True])
+def test_product_of_the_largest_numbers(swap):
+    """Scales as rows of up to 3e38 have them: results that fit into fp32 are right, the others infinite, zeros stay zeros."""
+    torch.manual_seed(5)
+    a = I.Int8Rows(torch.randint(-127, 128, (5, 64), dtype=torch.int8), torch.tensor([I.MOST_SCALE, 2.0 ** 100, 2.0 ** 64, 1.0, 2.0 ** -60]))
+    b = I.Int8Rows(torch.randint(-127, 128, (6, 64), dtype=torch.int8), torch.tensor([2.0 ** -60, 1e-9, 0.01, 1.0, 2.0 ** 40, 0.0]))
+    a.values[:, :] = a.values.abs()
+    b.values[:5] = b.values[:5].abs()  # sums of some 2^18 and more
+    a, b = (b, a) if swap else (a, b)
+    got = I.int8_product(a, b, out_dtype=torch.float32).double()
+    want = (a.values.double() @ b.values.double().t()) * a.scale.double()[:, None] * b.scale.double()
+    fits = want.abs() < torch.finfo(torch.float32).max
+    assert 20 < int(fits.sum()) < 30 and bool(((got - want).abs() <= 3 * 2.0 ** -24 * want.abs())[fits].all()) and got[~fits].isinf().all()  # three roundings

@@ -230,6 +230,31 @@ def test_product_of_the_largest_sums():
         assert bool((y == float(2 ** 31 - 16384)).all())
 
 
+@pytest.mark.parametrize("M,form", [(5, dict(form=1)), (13, dict(form=1)), (20, dict(form=2, splits=1)), (20, dict(form=2, splits=3)), (300, dict(form=2, splits=1)),
+                                    (300, dict(form=3))])
+@pytest.mark.parametrize("N", [64, 61])
+def test_product_of_the_largest_numbers(M, form, N):
+    """Scales as rows of up to 3e38 have them, beside ordinary ones whose results are the same bits without such neighbours."""
+    a, b = int8(M, 512, 1), int8(N, 512, 2)
+    a = I.Int8Rows(a.values.abs().clamp(min=0), a.scale.clone())
+    b = I.Int8Rows(b.values.abs().clamp(min=0), (0.5 + b.scale) * torch.logspace(-20, 12, N, base=10.0, device="cuda"))  # sums of some 2^21
+    ordinary = {dtype: I._product(a, b, rand(N), rand(M, N), dtype, **form) for dtype in (BF, F32)}
+    a.scale[::2] = (0.5 + a.scale[::2]) * torch.logspace(15, 35, len(a.scale[::2]), base=10.0, device="cuda")
+    a.scale[0], b.scale[5] = I.MOST_SCALE, 0.0
+    want = (a.values.double() @ b.values.double().t()) * a.scale.double()[:, None] * b.scale.double()
+    for dtype in (BF, F32):
+        got = I._product(a, b, rand(N), rand(M, N), dtype, **form)
+        assert torch.equal(torch.cat([got[1::2, :5], got[1::2, 6:]], 1), torch.cat([ordinary[dtype][1::2, :5], ordinary[dtype][1::2, 6:]], 1))
+        w = want + rand(N).double() + rand(M, N).double()
+        size = want.abs() + rand(N).double().abs() + rand(M, N).double().abs()
+        fits = w.abs() < 0.99 * torch.finfo(dtype).max
+        # two scales, two additions and the result rounded once each
+        assert not got[w.abs() > 1.01 * torch.finfo(dtype).max].isfinite().any()
+        assert bool(((got.double() - w).abs() <= 5 * 2.0 ** -24 * size + STEP[dtype] * w.abs())[fits].all()) and int((~fits).sum()) > 0
+        assert got[:, 5].isfinite().all()
+    lib.check_status()
+
+
 def test_product_of_views():
     """Rows with strides, rows that start anywhere, more dimensions, transposed biases and residuals."""
     a, b = int8(40, 1000, 1), int8(70, 1000, 2)
