@@ -228,8 +228,12 @@ def rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 
         x = x.detach()
         h = x if residual is None else (x.float() + residual.detach().float()).to(x.dtype)
         f = h.float()
+        mean = f.square().mean(-1, keepdim=True) + eps
+        # squares that leave the range of fp32: of the elements times 2^-80 or 2^80, a factor that cancels
+        s = torch.where(mean > torch.finfo(torch.float32).max, 2.0 ** -80, torch.where(mean < 2.0 ** -90, 2.0 ** 80, 1.0))
+        f = f * s
         y = f if weight is None else f * (weight.detach().float() + w_offset)
-        return quantize_reference(y, torch.rsqrt(f.square().mean(-1, keepdim=True) + eps)), None if residual is None else h
+        return quantize_reference(y, torch.rsqrt(f.square().mean(-1, keepdim=True) + eps * s * s)), None if residual is None else h
     x, ptr, rows, ldx = _rows_of(x)
     dev = x.device
     h, rptr, hptr, ldr = None, 0, 0, 0

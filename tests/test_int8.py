@@ -366,3 +366,20 @@ def test_product_of_the_largest_numbers(swap):
     want = (a.values.double() @ b.values.double().t()) * a.scale.double()[:, None] * b.scale.double()
     fits = want.abs() < torch.finfo(torch.float32).max
     assert 20 < int(fits.sum()) < 30 and bool(((got - want).abs() <= 3 * 2.0 ** -24 * want.abs())[fits].all()) and got[~fits].isinf().all()  # three roundings
+
+
+@pytest.mark.parametrize("size, eps", [(1e20, 1e-6), (1e30, 1e-6), (3e37, 1e-6), (1e-15, 0.0), (1e-22, 0.0), (1e-30, 0.0)])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_norms_whose_squares_leave_the_range_of_fp32(size, eps, dtype):
+    torch.manual_seed(6)
+    x, w = (torch.randn(4, 96).clamp(-5, 5) * size).to(dtype), 1 + 0.1 * torch.randn(96)
+    x[1] = 0
+    x[2] = torch.randn(96).to(dtype)  # an ordinary row
+    rows, _ = I.rms_norm_int8(x, w, eps if eps else 0.0)
+    d = x.double()
+    y = (d * torch.rsqrt(d.square().mean(-1, keepdim=True) + eps)).nan_to_num() * w.double()
+    live = [0, 2, 3]
+    assert ((rows.dequantize(torch.float32).double() - y).abs() <= y.abs().amax(-1, keepdim=True) / 254 * (1 + 1e-5))[live].all()
+    assert (rows.values.abs().amax(-1) == 127)[live].all()
+    x[3, 5], x[0, 7] = float("inf"), float("nan")
+    assert I.rms_norm_int8(x, w, eps)[0].scale.isnan().tolist()[0::3] == [True, True]

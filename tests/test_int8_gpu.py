@@ -127,6 +127,33 @@ def test_rms_norm_int8_offset_no_weight_and_tiny_rows():
     assert rows.scale[[2, 3]].isnan().all() and not rows.scale[[0, 1, 4]].isnan().any()
 
 
+@pytest.mark.parametrize("rows,cols", [(1500, 64), (3, 1000), (700, 4096), (700, 8208), (5, 4095), (700, 11007), (400, 14335), (2, 40001)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("eps", [1e-5, 0.0])
+def test_norms_whose_squares_leave_the_range_of_fp32(rows, cols, dtype, residual, eps):
+    """Among ordinary rows, whose bits do not depend on them."""
+    x, w = rand(rows, cols, seed=cols, dtype=dtype).clamp(-4, 4), (1 + rand(cols, seed=1, std=0.1, dtype=F32)).to(dtype)
+    r = rand(rows, cols, seed=2, dtype=dtype).clamp(-4, 4) if residual else None
+    first = I.rms_norm_int8(x, w, eps, residual=r)[0]
+    sizes = torch.ones(rows, device="cuda")
+    sizes[1::7], sizes[2::7] = 1e20, 3e37
+    if eps == 0.0:
+        sizes[3::7], sizes[4::7] = 1e-22, 1e-30
+    x = (x.float() * sizes[:, None]).to(dtype)
+    r = None if r is None else (r.float() * sizes[:, None]).to(dtype)
+    x[0, cols // 2] = float("inf")
+    got, h = I.rms_norm_int8(x, w, eps, residual=r)
+    want = x if r is None else (x.float() + r.float()).to(dtype)
+    assert h is None or torch.equal(h, want)
+    assert got.scale[0].isnan() and not got.values[0].any()
+    same = sizes == 1
+    same[0] = False
+    assert torch.equal(got.values[same], first.values[same]) and torch.equal(got.scale[same], first.scale[same])
+    d = want[1:].double()
+    check_rows(I.Int8Rows(got.values[1:], got.scale[1:]), d * w.double(), (d.square().mean(-1, keepdim=True) + eps).rsqrt(), slack=0.0 if dtype == BF else 2.0 ** -22)
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 500), (2, 4096), (3, 5001), (2, 14336), (1, 40001)])
 @pytest.mark.parametrize("act", ["silu", "gelu_new", "gelu", "relu", "quick_gelu"])
 def test_gated_activation_int8(rows, cols, act):
