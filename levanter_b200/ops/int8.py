@@ -184,7 +184,7 @@ def quantize_reference(y: torch.Tensor, factor: Optional[torch.Tensor] = None) -
     """PyTorch statement: the rows of ``factor * y`` (a positive number per row, which leaves the whole numbers as they are)."""
     y = y.float()
     top = y.abs().amax(-1, keepdim=True)
-    most = top if factor is None else top * factor
+    most = top if factor is None else torch.where(top == 0, top, top * factor)  # (a row of zeros without an eps has an infinite factor)
     live = (most >= TINY) & (top >= 2.0 ** -120)
     q = torch.where(live & torch.isfinite(top), torch.round(y.double() * 127.0 / top.double()).float(), torch.zeros_like(y))  # (fp32 would run over)
     scale = torch.where(live, (most / 127.0).clamp_max(MOST_SCALE), torch.zeros_like(most))

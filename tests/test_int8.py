@@ -383,3 +383,10 @@ def test_norms_whose_squares_leave_the_range_of_fp32(size, eps, dtype):
     assert (rows.values.abs().amax(-1) == 127)[live].all()
     x[3, 5], x[0, 7] = float("inf"), float("nan")
     assert I.rms_norm_int8(x, w, eps)[0].scale.isnan().tolist()[0::3] == [True, True]
+
+
+def test_norms_of_zeros_without_an_eps():
+    rows, _ = I.rms_norm_int8(torch.zeros(3, 40), None, 0.0)
+    assert not rows.values.any() and not rows.scale.any()  # (as on the GPU)
+    rows, _ = I.rms_norm_int8(torch.randn(3, 40), torch.zeros(40), 0.0)
+    assert not rows.values.any() and not rows.scale.any()

@@ -700,3 +700,10 @@ def test_training_step_of_a_model_in_int8():
         # eight quantisers of 0.9 % on the way through two layers and back, and as much again from the weights
         assert (p.grad.float() - q.grad.float()).norm() <= 0.15 * q.grad.float().norm() + 1e-6, n
     lib.check_status()
+
+
+@pytest.mark.parametrize("cols", [40, 1000, 4096])
+def test_norms_of_zeros_without_an_eps(cols):
+    for x, w in ((torch.zeros(3, cols, dtype=BF, device="cuda"), None), (rand(3, cols), torch.zeros(cols, device="cuda"))):
+        for rows in (I.rms_norm_int8(x, w, 0.0)[0], I.rms_norm_int8(x.cpu(), None if w is None else w.cpu(), 0.0)[0]):
+            assert not rows.values.any() and not rows.scale.any()
