@@ -297,15 +297,15 @@ struct Glu {
 // inputs (and of h) have one stride.
 struct Raw16 {
   uint32_t u[8];
-  // What is read once stays out of the L1: a norm with residual of 16384 x 4096 then takes 73 us, not 83.  kAgain: every row reads it (a norm's weight).
+  // (Volatile: not ahead of chain_wait().)  What is read once stays out of the L1: a norm with residual of 16384 x 4096 then takes 73 us, not 83.  kAgain: every row reads it (a norm's weight).
   template <bool kAgain = false>
   __device__ __forceinline__ void load(const void* p) {
     if constexpr (kAgain)
-      asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
           : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
           : "l"(p));
     else
-      asm("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
           : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
           : "l"(p));
   }
@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const int8_t* __restric
   if constexpr (kGroup == 16) {
     const long long row = narrow ? static_cast<unsigned>(i) / units : i / units;
     uint4 w;
-    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
         : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
         : "l"(q + row * ldq + (i - row * units) * 16));
     const float s = __ldg(scale + row);

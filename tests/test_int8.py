@@ -390,3 +390,15 @@ def test_norms_of_zeros_without_an_eps():
     assert not rows.values.any() and not rows.scale.any()  # (as on the GPU)
     rows, _ = I.rms_norm_int8(torch.randn(3, 40), torch.zeros(40), 0.0)
     assert not rows.values.any() and not rows.scale.any()
+
+
+def test_memory_accesses_in_assembly_keep_their_place():
+    """Kernels start before the kernel ahead of them has finished: a load that is not volatile could move ahead of the wait for what it reads."""
+    import re
+    from pathlib import Path
+
+    import levanter_b200.ops
+
+    csrc = Path(levanter_b200.ops.__file__).parent / "csrc"
+    free = [f"{p.name}: {m.group(1)}" for p in sorted(csrc.glob("*.cu*")) for m in re.finditer(r'\basm\s*\(\s*"([^"]*)', p.read_text())]
+    assert free and not [f for f in free if re.search(r": (\{|\\n|\\t|\s)*(ld|st|atom|red|cp)\.", f)]
