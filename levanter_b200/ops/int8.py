@@ -344,8 +344,9 @@ def _status(t: torch.Tensor) -> int:
 
 # ------------------------------------------------------------------------------------------------ training
 def _straight_through(x: torch.Tensor) -> torch.Tensor:
-    """What the 8-bit rows of ``x`` stand for, with the gradient passed on as it is."""
-    return x + (quantize_reference(x.detach()).dequantize(torch.float32).to(x.dtype) - x).detach()
+    """What the 8-bit rows of ``x`` stand for, in fp32, with the gradient passed on as it is."""
+    x = x.float()
+    return x + (quantize_reference(x.detach()).dequantize(torch.float32) - x).detach()
 
 
 # Up to so many rows the host's part bounds a layer: the projections of a layer without biases are one product, whose columns are their results.  Above it their
@@ -405,6 +406,14 @@ def _held_products(x: torch.Tensor, values: torch.Tensor, scale: torch.Tensor, l
     return tuple(ys)
 
 
+def _gemm_rows(d: torch.Tensor) -> torch.Tensor:
+    """``d [rows, cols]`` as bf16 rows that the GEMM reads where they lie."""
+    cols = d.shape[1]
+    if d.dtype is torch.bfloat16 and d.stride(1) == 1 and d.stride(0) >= cols and d.stride(0) % 8 == 0 and d.data_ptr() % 16 == 0:
+        return d
+    return _room(d.shape, torch.bfloat16, d.device, 8).copy_(d)
+
+
 class _Int8ManyFn(torch.autograd.Function):
     """Projections of the same rows.  Kept for the backward pass: the rows and the weights in 8 bits, 1 byte per activation instead of 2, once for all projections.
 
@@ -437,29 +446,29 @@ class _Int8ManyFn(torch.autograd.Function):
         dws, dbs = [None] * n, [None] * n
         if not live:
             return (None, None, *dws, *dbs)
-        d2 = [dys[i].reshape(rows, refs[i].shape[0]) for i in live]
-        d2 = [d if d.dtype is torch.bfloat16 else d.to(torch.bfloat16) for d in d2]
+        d2 = [_gemm_rows(dys[i].reshape(rows, refs[i].shape[0])) for i in live]
         need_w = [i for i in live if need[2 + i]]
         # what the rows in question stand for, in one launch: x, the weights or both
         first, last = 0 if need_w else rows, total if need[0] else rows
-        back = torch.empty(last - first, cols, dtype=torch.bfloat16, device=values.device) if last > first else None
+        wide = -(-cols // 8) * 8  # (the GEMM's rows start on 16 bytes; what is held has room for as many columns)
+        back = torch.empty(last - first, wide, dtype=torch.bfloat16, device=values.device) if last > first else None
         if back is not None:
-            _launch("lvb_int8_dequantize", values, values.data_ptr() + first * ld, ld, scale.data_ptr() + 4 * first, last - first, cols, back.data_ptr(), 0)
-        side = d2[0] if len(live) == 1 else torch.cat(d2, dim=1) if _side_by_side(rows, cols, sum(d.shape[1] for d in d2)) else None
+            _launch("lvb_int8_dequantize", values, values.data_ptr() + first * ld, ld, scale.data_ptr() + 4 * first, last - first, wide, back.data_ptr(), 0)
+        side = d2[0] if len(live) == 1 else _gemm_rows(torch.cat(d2, dim=1)) if _side_by_side(rows, cols, sum(d.shape[1] for d in d2)) else None
         dx = None
         if need[0]:
             w = back[rows - first:]
             if len(live) < n or side is None:
                 ws = [p for i, p in enumerate(w.split([r.shape[0] for r in refs])) if i in live]
             if side is not None:
-                dx = gemm(side, w if len(live) == n else torch.cat(ws), b_mn=True)
+                dx = gemm(side, (w if len(live) == n else torch.cat(ws))[:, :cols], b_mn=True)
             else:
                 for d, w in zip(d2, ws):
-                    dx = gemm(d, w, b_mn=True, out=dx, accumulate=dx is not None, out_dtype=torch.float32)
+                    dx = gemm(d, w[:, :cols], b_mn=True, out=dx, accumulate=dx is not None, out_dtype=torch.float32)
                 dx = dx.to(torch.bfloat16)
             dx = dx.view(shape)
         if need_w:
-            x2 = back[:rows]
+            x2 = back[:rows, :cols]
             own = all(getattr(refs[i], "main_grad", None) is None and getattr(refs[i], "grad_sink", None) is None and refs[i].dtype is torch.bfloat16 for i in live)
             if len(live) > 1 and side is not None and need_w == live and own:
                 for i, dw in zip(live, gemm(side, x2, a_mn=True, b_mn=True).split([refs[i].shape[0] for i in live])):
@@ -476,7 +485,7 @@ class _Int8ManyFn(torch.autograd.Function):
 
 def int8_linear_many(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: Optional[Sequence[Optional[torch.Tensor]]] = None) -> Tuple[torch.Tensor, ...]:
     """``[x' w'^T + b for w, b in ...]`` with ``x [..., in]`` and the ``weights [out, in]`` held in 8 bits (``x'``, ``w'``: what their whole numbers stand for);
-    differentiable in ``x``, weights and biases.  bf16 with sizes that are multiples of 8 runs on the kernels, everything else on PyTorch's operations.  Of several
+    differentiable in ``x``, weights and biases.  bf16 on a GPU runs on the kernels, everything else on PyTorch's operations in fp32, rounded once.  Of several
     projections without biases of up to ``MANY_ROWS`` rows the results are columns of one tensor: each has the others' columns between its rows."""
     weights = list(weights)
     biases = [None] * len(weights) if biases is None else list(biases)
@@ -489,14 +498,12 @@ def int8_linear_many(x: torch.Tensor, weights: Sequence[torch.Tensor], biases: O
             raise ValueError(f"int8_linear_many: x {tuple(x.shape)} on {x.device} and a weight {tuple(w.shape)} {w.dtype} on {w.device} do not go together")
         if b is not None and (b.shape != (w.shape[0],) or b.device != x.device or b.dtype not in _FLOATS):
             raise ValueError(f"int8_linear_many: bias [{w.shape[0]}] on {x.device} expected, got {tuple(b.shape)} {b.dtype} on {b.device}")
-    from .gemm import _tma_shapes_ok
-
-    if _kernels(x) and x.dtype == torch.bfloat16 and x.numel() and all(w.dtype == torch.bfloat16 and _tma_shapes_ok(w) and w.shape[0] > 0 for w in weights):
+    if _kernels(x) and x.dtype == torch.bfloat16 and x.numel() and all(w.dtype == torch.bfloat16 and w.shape[0] > 0 for w in weights):
         if lib.plain_call():
             return _held_products(x, *_hold(x, weights), weights, biases)
         return _Int8ManyFn.apply(x, len(weights), *weights, *biases)
     x8 = _straight_through(x)
-    return tuple(F.linear(x8, _straight_through(w).to(x.dtype), None if b is None else b.to(x.dtype)) for w, b in zip(weights, biases))
+    return tuple(F.linear(x8, _straight_through(w), None if b is None else b.float()).to(x.dtype) for w, b in zip(weights, biases))
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

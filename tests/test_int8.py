@@ -402,3 +402,21 @@ def test_memory_accesses_in_assembly_keep_their_place():
     csrc = Path(levanter_b200.ops.__file__).parent / "csrc"
     free = [f"{p.name}: {m.group(1)}" for p in sorted(csrc.glob("*.cu*")) for m in re.finditer(r'\basm\s*\(\s*"([^"]*)', p.read_text())]
     assert free and not [f for f in free if re.search(r": (\{|\\n|\\t|\s)*(ld|st|atom|red|cp)\.", f)]
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_products_without_a_kernel_round_once(bias):
+    """The operands stay what the whole numbers stand for; the result is rounded to the rows' type, and so are the gradients."""
+    torch.manual_seed(7)
+    x, w, b = torch.randn(64, 100).to(BF), torch.randn(31, 100).to(BF), torch.randn(31).to(BF) if bias else None
+    xh, wh = (I.quantize_rows(t).dequantize(torch.float32).double() for t in (x, w))
+    x.requires_grad_(), w.requires_grad_()
+    y, dy = I.int8_linear(x, w, b), torch.randn(64, 31).to(BF)
+    gx, gw = torch.autograd.grad(y, [x, w], dy)
+    want = xh @ wh.t() + (b.double() if bias else 0)
+    size = xh.abs() @ wh.abs().t() + 10
+    # sums of 101 numbers in fp32 (and what is held, off by two roundings of the dequantisation and two of the difference), one rounding to bf16
+    assert y.dtype == BF and ((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 110 * 2.0 ** -24 * size).all()
+    d = dy.double()
+    assert gx.dtype == BF and ((gx.double() - d @ wh).abs() <= 2.0 ** -8 * (d @ wh).abs() + 110 * 2.0 ** -24 * (d.abs() @ wh.abs())).all()
+    assert ((gw.double() - d.t() @ xh).abs() <= 2.0 ** -8 * (d.t() @ xh).abs() + 110 * 2.0 ** -24 * (d.abs().t() @ xh.abs())).all()

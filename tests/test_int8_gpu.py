@@ -707,3 +707,39 @@ def test_norms_of_zeros_without_an_eps(cols):
     for x, w in ((torch.zeros(3, cols, dtype=BF, device="cuda"), None), (rand(3, cols), torch.zeros(cols, device="cuda"))):
         for rows in (I.rms_norm_int8(x, w, 0.0)[0], I.rms_norm_int8(x.cpu(), None if w is None else w.cpu(), 0.0)[0]):
             assert not rows.values.any() and not rows.scale.any()
+
+
+@pytest.mark.parametrize("shape,outs,bias", [((6, 100), [13], True), ((64, 1000), [301], False), ((3, 7, 77), [5, 1, 130], False), ((1, 1), [1], False), ((2500, 331), [129, 7], True),
+                                             ((301, 515), [260, 300], False), ((5000, 40), [203, 51], False), ((129, 1111), [641], False), ((33, 17), [9, 8, 7, 6, 5, 4], True)])
+def test_sizes_that_are_no_multiples_of_8(shape, outs, bias):
+    """The products round once, as int8_product does; the gradients' operands are rounded to bf16, as at any other size."""
+    x, ws = rand(*shape).requires_grad_(), [rand(n, shape[-1], seed=2 + n).requires_grad_() for n in outs]
+    bs = [rand(n, seed=3).requires_grad_() for n in outs] if bias else None
+    ys = I.int8_linear_many(x, ws, bs)
+    dys = [rand(*y.shape, seed=4 + i) for i, y in enumerate(ys)]
+    grads = torch.autograd.grad(ys, [x, *ws, *(bs or [])], dys)
+    lib.check_status()
+    rows = I.quantize_rows(x.detach())
+    dx = size = 0
+    for i, (y, w, d) in enumerate(zip(ys, ws, dys)):
+        assert torch.equal(y, I.int8_product(rows, I.quantize_rows(w.detach()), bs[i].detach() if bias else None))
+        xh, wh, d = held(x.detach()).flatten(0, -2), held(w.detach()), d.double().flatten(0, -2)
+        dx, size = dx + d @ wh, size + d.abs() @ wh.abs()
+        want, mag = d.t() @ xh, d.abs().t() @ xh.abs()
+        assert grads[1 + i].dtype == BF and bool(((grads[1 + i].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * 2.0 ** -8 * mag).all())
+        if bias:
+            assert bool(((grads[1 + len(outs) + i].double() - d.sum(0)).abs() <= 2.0 ** -8 * d.sum(0).abs() + 2.0 ** -18 * d.abs().sum(0)).all())
+    got = grads[0].double().flatten(0, -2)
+    assert grads[0].dtype == BF and bool(((got - dx).abs() <= 2.0 ** -8 * dx.abs() + 1.01 * 2.0 ** -8 * size).all())
+    some = torch.autograd.grad(I.int8_linear_many(x, ws, bs)[-1], [x, ws[-1]], dys[-1])
+    alone = torch.autograd.grad(I.int8_linear(x, ws[-1], bs[-1] if bias else None), [x, ws[-1]], dys[-1])
+    assert torch.equal(some[0], alone[0]) and torch.equal(some[1], alone[1])
+
+
+def test_gradients_of_sums_over_rows():
+    """Such output gradients are one row, read again and again."""
+    x, w = rand(70, 512).requires_grad_(), rand(40, 512, seed=2).requires_grad_()
+    v = rand(40, seed=3)
+    got = torch.autograd.grad(I.int8_linear(x, w).sum(0), [x, w], v)
+    want = torch.autograd.grad(I.int8_linear(x, w), [x, w], v.expand(70, 40).contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
