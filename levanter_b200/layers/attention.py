@@ -768,6 +768,8 @@ class Attention(nn.Module):
         out, _ = self._paged_heads(x, kv_cache, batch_info, pos_ids)
         if type(self.o_proj) is Linear and self.o_proj.bias is None:
             return add_linear(stream, out, self.o_proj.weight), kv_cache
+        if plain(self.o_proj, Int8ServingLinear):
+            return self.o_proj(out, residual=stream, out_dtype=torch.float32), kv_cache
         return stream + self.o_proj(out).float(), kv_cache
 
     def paged_decode_mixing_values(self, x: torch.Tensor, kv_cache: "KvPageCache", batch_info, pos_ids, v_first: Optional[torch.Tensor] = None):
@@ -778,6 +780,8 @@ class Attention(nn.Module):
         out, v_first = self._paged_heads(x, kv_cache, batch_info, pos_ids, v_first)
         if type(self.o_proj) is Linear:
             return project(out, self.o_proj.weight, bias=self.o_proj.bias, out_dtype=torch.float32), v_first
+        if plain(self.o_proj, Int8ServingLinear):
+            return self.o_proj(out, out_dtype=torch.float32), v_first
         return self.o_proj(out).float(), v_first
 
     def empty_page_cache(self, max_pages: int, page_size: int, *, dtype=torch.bfloat16, device=None) -> "KvPageCache":

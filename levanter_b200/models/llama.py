@@ -194,6 +194,8 @@ class LlamaMlp(nn.Module):
         h = self._inner(x)
         if type(self.down_proj) is Linear:
             return project(h, self.down_proj.weight, bias=self.down_proj.bias, out_dtype=torch.float32)
+        if plain(self.down_proj, Int8ServingLinear):
+            return self.down_proj(h, out_dtype=torch.float32)
         return self.down_proj(h).float()
 
     def add_to_stream(self, stream: torch.Tensor, x: torch.Tensor, batch_info=None) -> torch.Tensor:
@@ -201,6 +203,8 @@ class LlamaMlp(nn.Module):
         h = self._inner(x.reshape(-1, x.shape[-1])).view(*x.shape[:-1], -1)
         if type(self.down_proj) is Linear and self.down_proj.bias is None:
             return add_linear(stream, h, self.down_proj.weight)
+        if plain(self.down_proj, Int8ServingLinear):
+            return self.down_proj(h, residual=stream, out_dtype=torch.float32)
         return stream + self.down_proj(h).float()
 
     def _int8(self, x, residual: Optional[torch.Tensor]) -> torch.Tensor:

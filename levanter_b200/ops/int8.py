@@ -546,8 +546,8 @@ class Int8Linear(nn.Module):
 class Int8ServingLinear(nn.Module):
     """A projection that serves: its weights are held in 8 bits (buffers ``weight`` int8 ``[out, in]`` and ``weight_scale`` fp32 ``[out]``) and have no gradient.
     A state with the weight in another type is quantised as it is loaded.
-    It takes rows in bf16 or fp32 and gives results of their type, or :class:`Int8Rows` that several projections share (results in bf16), and adds a ``residual`` in
-    its product's epilogue."""
+    It takes rows in bf16 or fp32, or :class:`Int8Rows` that several projections share, gives results of their type (of 8-bit rows: bf16) or in ``out_dtype``, and
+    adds a ``residual`` in its product's epilogue."""
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor]):
         super().__init__()
@@ -581,8 +581,9 @@ class Int8ServingLinear(nn.Module):
             state_dict[prefix + "weight"], state_dict[prefix + "weight_scale"] = rows
         super()._load_from_state_dict(state_dict, prefix, *args)
 
-    def forward(self, x: Union[torch.Tensor, Int8Rows], *, skip_bias: bool = False, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return int8_product(as_int8_rows(x), self.rows, None if skip_bias else self.bias, residual, out_dtype=x.dtype)
+    def forward(self, x: Union[torch.Tensor, Int8Rows], *, skip_bias: bool = False, residual: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return int8_product(as_int8_rows(x), self.rows, None if skip_bias else self.bias, residual, out_dtype=x.dtype if out_dtype is None else out_dtype)
 
     def extra_repr(self):
         return f"in={self.in_features}, out={self.out_features}, bias={self.bias is not None}, int8 weights"

@@ -420,3 +420,24 @@ def test_products_without_a_kernel_round_once(bias):
     d = dy.double()
     assert gx.dtype == BF and ((gx.double() - d @ wh).abs() <= 2.0 ** -8 * (d @ wh).abs() + 110 * 2.0 ** -24 * (d.abs() @ wh.abs())).all()
     assert ((gw.double() - d.t() @ xh).abs() <= 2.0 ** -8 * (d.t() @ xh).abs() + 110 * 2.0 ** -24 * (d.abs().t() @ xh.abs())).all()
+
+
+def test_fp32_streams_get_results_that_were_not_rounded_to_bf16():
+    """What ends a block is added to an fp32 stream, or normed in fp32, as the product's epilogue has it."""
+    from levanter_b200.layers.attention import Attention, AttentionConfig
+    from levanter_b200.models.llama import LlamaMlp
+
+    torch.manual_seed(8)
+    x, stream = torch.randn(5, 64).to(BF), torch.randn(5, 64)
+    with torch.no_grad():
+        mlp = quantize_for_serving(LlamaMlp(64, 96, Act.silu, init_std=0.2), QuantizationConfig(int8=True, targets=["down_proj"])).to(BF)
+        down = mlp.down_proj
+        want = I.int8_product(I.quantize_rows(mlp._inner(x)), down.rows, out_dtype=torch.float32)
+        assert not torch.equal(want, want.to(BF).float())
+        assert torch.equal(mlp.forward_fp32(x), want) and torch.equal(mlp.add_to_stream(stream, x), want + stream)
+        assert torch.equal(mlp.add_to_stream(stream.view(1, 5, 64), x.view(1, 5, 64)), (want + stream).view(1, 5, 64))
+        attn = quantize_for_serving(Attention(AttentionConfig(64, 4, 2)), QuantizationConfig(int8=True)).to(BF)
+        attn._paged_heads = lambda *a: (x, None)
+        want = I.int8_product(I.quantize_rows(x), attn.o_proj.rows, out_dtype=torch.float32)
+        assert torch.equal(attn.paged_decode_mixing_values(x, None, None, None)[0], want)
+        assert torch.equal(attn.paged_decode_stream(x, None, None, None, stream)[0], want + stream)

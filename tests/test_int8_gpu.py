@@ -743,3 +743,18 @@ def test_gradients_of_sums_over_rows():
     got = torch.autograd.grad(I.int8_linear(x, w).sum(0), [x, w], v)
     want = torch.autograd.grad(I.int8_linear(x, w), [x, w], v.expand(70, 40).contiguous())
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_fp32_streams_get_results_that_were_not_rounded_to_bf16():
+    from levanter_b200.models.llama import LlamaMlp
+    from levanter_b200.quantization import QuantizationConfig, quantize_for_serving
+
+    x, stream = rand(37, 256), rand(37, 256, seed=1, dtype=F32)
+    mlp = quantize_for_serving(LlamaMlp(256, 512, Act.silu, init_std=0.2).to("cuda", BF).eval(), QuantizationConfig(int8=True, targets=["down_proj"]))
+    with torch.no_grad():
+        rows = I.quantize_rows(mlp._inner(x))
+        want = (rows.values.double() @ mlp.down_proj.weight.double().t()) * rows.scale.double()[:, None] * mlp.down_proj.weight_scale.double()
+        # a sum, two scales and an addition, rounded once each
+        assert bool(((mlp.forward_fp32(x).double() - want).abs() <= 3 * 2.0 ** -24 * want.abs()).all())
+        got = mlp.add_to_stream(stream.clone(), x).double()
+        assert bool(((got - want - stream.double()).abs() <= 4 * 2.0 ** -24 * (want.abs() + stream.double().abs())).all())
