@@ -24,7 +24,7 @@ from ..layers.rotary import rope_config_from_hf, rope_to_hf_dict, DefaultRotaryE
 from ..nn import Embedding, FusedRows, Linear, fork_norm, linear_many, norm_for, plain
 from ..ops.gemm import linear_residual
 from ..ops.glu import ClampedGlu, GatedActivation, gated_activation
-from ..ops.int8 import Int8Rows, Int8ServingLinear, as_int8_rows, gated_activation_int8, int8_product
+from ..ops.int8 import Int8Linear, Int8Rows, Int8ServingLinear, as_int8_rows, gated_activation_int8, int8_product
 from ..ops.residual_stream import add_linear, glu_of_rows, project
 from ..utils.activation import ActivationFunctionEnum
 from ..utils.flop_utils import lm_flops_per_token
@@ -186,11 +186,15 @@ class LlamaMlp(nn.Module):
             w = self._rows.get([m.weight for m in mods], build)
         if w is not None:
             return glu_of_rows(project(x, w), self.gate_proj.weight.shape[0], self.act)
+        if all(plain(m, Int8ServingLinear) for m in mods) or all(plain(m, Int8Linear) for m in mods):
+            return gated_activation(*linear_many(x, *mods), self.act)  # the rows are quantised once
         return gated_activation(self.gate_proj(x), self.up_proj(x), self.act)
 
     def forward_fp32(self, x: torch.Tensor) -> torch.Tensor:
         """The MLP of packed rows ``x [T, hidden]`` in fp32 straight from the last product, for blocks whose output is normed before it
         joins an fp32 stream."""
+        if self._held_in_8_bits():
+            return self._int8(x, None, torch.float32)
         h = self._inner(x)
         if type(self.down_proj) is Linear:
             return project(h, self.down_proj.weight, bias=self.down_proj.bias, out_dtype=torch.float32)
@@ -200,6 +204,8 @@ class LlamaMlp(nn.Module):
 
     def add_to_stream(self, stream: torch.Tensor, x: torch.Tensor, batch_info=None) -> torch.Tensor:
         """``stream + mlp(x)`` on an fp32 stream, added in the epilogue of the last product."""
+        if self._held_in_8_bits():
+            return self._int8(x, stream, torch.float32)
         h = self._inner(x.reshape(-1, x.shape[-1])).view(*x.shape[:-1], -1)
         if type(self.down_proj) is Linear and self.down_proj.bias is None:
             return add_linear(stream, h, self.down_proj.weight)
@@ -207,7 +213,10 @@ class LlamaMlp(nn.Module):
             return self.down_proj(h, residual=stream, out_dtype=torch.float32)
         return stream + self.down_proj(h).float()
 
-    def _int8(self, x, residual: Optional[torch.Tensor]) -> torch.Tensor:
+    def _held_in_8_bits(self) -> bool:
+        return all(plain(m, Int8ServingLinear) for m in (self.gate_proj, self.up_proj, self.down_proj))
+
+    def _int8(self, x, residual: Optional[torch.Tensor], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """The MLP on weights held in 8 bits: every row is quantised where it is made, gate and up are one product where they lie side by side."""
         mods = (self.gate_proj, self.up_proj)
         shared = all(m.bias is None for m in mods)
@@ -218,10 +227,10 @@ class LlamaMlp(nn.Module):
             gate, up = y[..., :ff], y[..., ff:]
         else:
             gate, up = linear_many(x, *mods)
-        return int8_product(gated_activation_int8(gate, up, self.act), self.down_proj.rows, self.down_proj.bias, residual, out_dtype=x.dtype)
+        return int8_product(gated_activation_int8(gate, up, self.act), self.down_proj.rows, self.down_proj.bias, residual, out_dtype=out_dtype or x.dtype)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        if all(plain(m, Int8ServingLinear) for m in (self.gate_proj, self.up_proj, self.down_proj)):
+        if self._held_in_8_bits():
             return self._int8(x, residual)
         if self.tp is not None and self.tp.size > 1:
             x = self.tp.copy_to_region(x)

@@ -441,3 +441,31 @@ def test_fp32_streams_get_results_that_were_not_rounded_to_bf16():
         want = I.int8_product(I.quantize_rows(x), attn.o_proj.rows, out_dtype=torch.float32)
         assert torch.equal(attn.paged_decode_mixing_values(x, None, None, None)[0], want)
         assert torch.equal(attn.paged_decode_stream(x, None, None, None, stream)[0], want + stream)
+
+
+@pytest.mark.parametrize("act", ["silu", "tanh"])
+def test_blocks_on_an_fp32_stream_quantise_their_rows_once(act, monkeypatch):
+    """Once for gate and up, and the gated activation as it is made, in 32 bits."""
+    from levanter_b200.models.llama import LlamaMlp
+
+    torch.manual_seed(9)
+    x, stream = torch.randn(5, 64).to(BF), torch.randn(5, 64)
+    mlp = quantize_for_serving(LlamaMlp(64, 96, Act(act), init_std=0.2), QuantizationConfig(int8=True)).to(BF).eval()
+    with torch.no_grad():
+        gate, up = linear_many(x, mlp.gate_proj, mlp.up_proj)
+        want = I.int8_product(I.gated_activation_int8(gate, up, mlp.act), mlp.down_proj.rows, out_dtype=torch.float32)
+        calls = []
+        monkeypatch.setattr(I, "_quantize", lambda x, real=I._quantize: calls.append(1) or real(x))
+        assert torch.equal(mlp.forward_fp32(x), want) and torch.equal(mlp.add_to_stream(stream, x), want + stream)
+        assert len(calls) == (2 if act == "silu" else 4)  # (an activation without a kernel of its own is quantised as it comes)
+        calls.clear()
+        mlp.down_proj.register_forward_hook(lambda *a: None)  # then it has to see the rows
+        mlp.forward_fp32(x)
+        assert len(calls) == 2
+    model = LlamaMlp(64, 96, Act(act))
+    quantize_linear_layers(model, QuantizationConfig(int8=True))
+    calls, many = [], I._straight_through
+    monkeypatch.setattr(I, "_straight_through", lambda x: calls.append(x.shape) or many(x))
+    with torch.no_grad():
+        model.forward_fp32(torch.randn(5, 64))
+    assert calls.count((5, 64)) == 1 and calls.count((5, 96)) == 1
