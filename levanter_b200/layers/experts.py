@@ -34,7 +34,7 @@ class GroupedSoftmaxMoe(nn.Module):
     per token.  ``activation`` and ``shared_activation``: of the experts and of the shared one.
 
     Serving: the shared expert's two projections, the router and the number that weighs the shared expert read the same rows, so they are
-    one product with fp32 output."""
+    one product with fp32 output.  A shared expert whose weights are held in 8 bits is a block of its own beside it."""
 
     def __init__(self, hidden: int, intermediate: int, num_experts: int, top: int, *, groups: int = 1, keep: int = 1,
                  shared_intermediate: Optional[int] = None, shared_gated: bool = True, activation: GatedActivation = ActivationFunctionEnum.silu,
@@ -50,19 +50,25 @@ class GroupedSoftmaxMoe(nn.Module):
             self.shared_gate = Linear(hidden, 1, init_std=init_std) if shared_gated else None
             rows += 2 * shared_intermediate + int(shared_gated)
         self._rows = FusedRows(-rows % 8)
+        self._router_rows = FusedRows(-(num_experts + int(shared_gated and shared_intermediate is not None)) % 8)
+
+    def _shared_in_8_bits(self) -> bool:
+        return self.shared_intermediate is not None and self.shared.held_in_8_bits()
 
     def _joint_weight(self) -> Optional[torch.Tensor]:
-        """``[gate; up; router; shared gate; padding]`` (or the router alone); None in training or when a projection is wrapped."""
-        mods = [self.router]
+        """``[gate; up; router; shared gate; padding]`` (or the router alone; without gate and up where those are held in 8 bits); None in training or when a
+        projection is wrapped."""
+        mods, held = [self.router], self._shared_in_8_bits()
         if self.shared_intermediate is not None:
-            mods = [self.shared.gate_proj, self.shared.up_proj, self.router] + ([] if self.shared_gate is None else [self.shared_gate])
-        if self.training or not all(type(m) is Linear for m in mods) or (self.shared_intermediate is not None and type(self.shared.down_proj) is not Linear):
+            mods = ([] if held else [self.shared.gate_proj, self.shared.up_proj]) + mods + ([] if self.shared_gate is None else [self.shared_gate])
+        if self.training or not all(type(m) is Linear for m in mods) or (self.shared_intermediate is not None and not held and type(self.shared.down_proj) is not Linear):
             return None
-        return self._rows.get([m.weight for m in mods])
+        return (self._router_rows if held else self._rows).get([m.weight for m in mods])
 
     def add_to_stream(self, stream: torch.Tensor, h: torch.Tensor, batch_info=None) -> torch.Tensor:
         """``stream + moe(h)``.  ``batch_info``: padding tokens of a packed batch (no cache destination) are sent to no expert."""
-        e, E, ff = self.experts, self.num_experts, self.shared_intermediate or 0
+        held = self._shared_in_8_bits()
+        e, E, ff = self.experts, self.num_experts, 0 if held else self.shared_intermediate or 0
         shape = h.shape
         h2 = h.reshape(-1, shape[-1])
         w = self._joint_weight() if _kernels(h2, stream) else None
@@ -76,12 +82,15 @@ class GroupedSoftmaxMoe(nn.Module):
             if ff:
                 a = glu_of_rows(y, ff, self.shared.act, gate_logit=None if self.shared_gate is None else y[:, 2 * ff + E], out_dtype=h2.dtype)
                 add_linear(flat, a, self.shared.down_proj.weight)
+            if held:
+                shared = self.shared.forward_fp32(h2)
+                flat.add_(shared if self.shared_gate is None else torch.sigmoid(y[:, E:E + 1]) * shared)
             return flat.view(shape)
         z = project(h2, self.router.weight, out_dtype=torch.float32) if type(self.router) is Linear else self.router(h2).float()
         # a plain router leaves its bias to the routing, a wrapped one (LoRA) has added it
         idx, weights = moe.route_softmax_reference(z, self.top, self.groups, self.keep, self.router.bias if type(self.router) is Linear else None)
         out = moe.expert_outputs(h2, idx, weights, e.gate_up, e.down, gated=True, act=self.activation)
-        if ff:
-            shared = self.shared(h2).float()
+        if self.shared_intermediate is not None:
+            shared = self.shared.forward_fp32(h2) if held else self.shared(h2).float()
             out = out + (shared if self.shared_gate is None else torch.sigmoid(self.shared_gate(h2).float()) * shared)
         return stream + out.view(shape)

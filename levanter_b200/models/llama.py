@@ -193,7 +193,7 @@ class LlamaMlp(nn.Module):
     def forward_fp32(self, x: torch.Tensor) -> torch.Tensor:
         """The MLP of packed rows ``x [T, hidden]`` in fp32 straight from the last product, for blocks whose output is normed before it
         joins an fp32 stream."""
-        if self._held_in_8_bits():
+        if self.held_in_8_bits():
             return self._int8(x, None, torch.float32)
         h = self._inner(x)
         if type(self.down_proj) is Linear:
@@ -204,7 +204,7 @@ class LlamaMlp(nn.Module):
 
     def add_to_stream(self, stream: torch.Tensor, x: torch.Tensor, batch_info=None) -> torch.Tensor:
         """``stream + mlp(x)`` on an fp32 stream, added in the epilogue of the last product."""
-        if self._held_in_8_bits():
+        if self.held_in_8_bits():
             return self._int8(x, stream, torch.float32)
         h = self._inner(x.reshape(-1, x.shape[-1])).view(*x.shape[:-1], -1)
         if type(self.down_proj) is Linear and self.down_proj.bias is None:
@@ -213,7 +213,7 @@ class LlamaMlp(nn.Module):
             return self.down_proj(h, residual=stream, out_dtype=torch.float32)
         return stream + self.down_proj(h).float()
 
-    def _held_in_8_bits(self) -> bool:
+    def held_in_8_bits(self) -> bool:
         return all(plain(m, Int8ServingLinear) for m in (self.gate_proj, self.up_proj, self.down_proj))
 
     def _int8(self, x, residual: Optional[torch.Tensor], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -230,7 +230,7 @@ class LlamaMlp(nn.Module):
         return int8_product(gated_activation_int8(gate, up, self.act), self.down_proj.rows, self.down_proj.bias, residual, out_dtype=out_dtype or x.dtype)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        if self._held_in_8_bits():
+        if self.held_in_8_bits():
             return self._int8(x, residual)
         if self.tp is not None and self.tp.size > 1:
             x = self.tp.copy_to_region(x)

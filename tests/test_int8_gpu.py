@@ -758,3 +758,34 @@ def test_fp32_streams_get_results_that_were_not_rounded_to_bf16():
         assert bool(((mlp.forward_fp32(x).double() - want).abs() <= 3 * 2.0 ** -24 * want.abs()).all())
         got = mlp.add_to_stream(stream.clone(), x).double()
         assert bool(((got - want - stream.double()).abs() <= 4 * 2.0 ** -24 * (want.abs() + stream.double().abs())).all())
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("hidden,ff,shared,experts", [(64, 32, 96, 8), (72, 24, 40, 10), (128, 16, 22, 9)])
+def test_a_shared_expert_in_8_bits_leaves_the_others_on_their_kernels(gated, hidden, ff, shared, experts, monkeypatch):
+    from levanter_b200.layers.experts import GroupedSoftmaxMoe
+    from levanter_b200.ops import moe
+    from levanter_b200.quantization import QuantizationConfig, quantize_for_serving
+
+    torch.manual_seed(3)
+    block = GroupedSoftmaxMoe(hidden, ff, experts, 2, shared_intermediate=shared, shared_gated=gated, init_std=0.2).to("cuda", BF).eval()
+    alone = GroupedSoftmaxMoe(hidden, ff, experts, 2).to("cuda", BF).eval()
+    alone.load_state_dict({k: v for k, v in block.state_dict().items() if not k.startswith("shared")})
+    quantize_for_serving(block, QuantizationConfig(int8=True))
+    x, h = rand(21, hidden, seed=1, dtype=F32), rand(21, hidden, seed=2)
+    monkeypatch.setattr(moe, "expert_outputs", None)  # what runs where the kernels do not
+    with torch.no_grad():
+        part = block.shared.forward_fp32(h)
+        if gated:
+            part = part * torch.sigmoid(h.float() @ block.shared_gate.weight.float().t())
+        base = alone.add_to_stream(x.clone(), h)
+        want = base.double() + part.double()
+        got = block.add_to_stream(x.clone(), h)
+        # the routing weights and the gate from sums of some hundred products in fp32, in another order
+        tol = 200 * 2.0 ** -24 * (x.abs() + (base - x).abs() + part.abs() + 1)
+        assert bool(((got.double() - want).abs() <= tol).all())
+        replayed, g = x.clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            block.add_to_stream(replayed, h)
+        g.replay()
+        assert torch.equal(replayed, got)
