@@ -496,8 +496,9 @@ class Attention(nn.Module):
     difference_names = ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2")
 
     def row_readers(self):
-        """The projections that read this layer's input rows."""
-        return self._projections()
+        """The projections that read the rows given to :meth:`paged_decode`, and nothing else of this layer does; none where a subclass or a method of
+        the instance may read them too."""
+        return self._projections() if type(self) is Attention and "paged_decode" not in self.__dict__ else ()
 
     def _projections(self):
         return [self.q_proj, self.k_proj, self.v_proj] + ([self.g_proj] if self.config.output_gate or self.config.head_gate else [])

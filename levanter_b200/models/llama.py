@@ -166,8 +166,9 @@ class LlamaMlp(nn.Module):
         self._rows, self._scales = FusedRows(), FusedRows()
 
     def row_readers(self):
-        """The projections that read this layer's input rows."""
-        return self.gate_proj, self.up_proj
+        """The projections that read the rows this layer is called with, and nothing else does; none where a hook, a subclass or a method of the
+        instance sees them too."""
+        return (self.gate_proj, self.up_proj) if plain(self, LlamaMlp) else ()
 
     def lay_out_for_serving(self) -> None:
         """Lays gate and up side by side for serving steps of a few rows, as the attention layer does with its projections."""

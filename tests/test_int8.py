@@ -469,3 +469,44 @@ def test_blocks_on_an_fp32_stream_quantise_their_rows_once(act, monkeypatch):
     with torch.no_grad():
         model.forward_fp32(torch.randn(5, 64))
     assert calls.count((5, 64)) == 1 and calls.count((5, 96)) == 1
+
+
+@pytest.mark.parametrize("watch", ["pre_hook", "hook", "subclass", "instance", "attention subclass", "attention instance"])
+def test_layers_that_are_watched_get_tensors(watch):
+    """Rows in 8 bits are handed to the layers' own code only."""
+    from levanter_b200.data.passthrough_tokenizer import PassthroughTokenizer
+    from levanter_b200.inference.engine import InferenceEngine, InferenceEngineConfig, Request
+    from levanter_b200.inference.jit_scheduler import SeqDecodingParams
+    from levanter_b200.layers.attention import Attention
+    from levanter_b200.models.llama import LlamaMlp
+
+    seen = []
+
+    class Mlp(LlamaMlp):
+        def forward(self, x, residual=None):
+            seen.append(x)
+            return super().forward(x, residual)
+
+    class Attn(Attention):
+        def paged_decode(self, x, *args, **kw):
+            seen.append(x)
+            return super().paged_decode(x, *args, **kw)
+
+    model = quantize_for_serving(llama().build(100, seed=0).eval(), QuantizationConfig(int8=True)).to(BF)
+    layer = model.transformer.layers[1]
+    if watch == "pre_hook":
+        layer.mlp.register_forward_pre_hook(lambda m, args: seen.append(args[0]))
+    elif watch == "hook":
+        layer.mlp.register_forward_hook(lambda m, args, out: seen.append(args[0]))
+    elif watch == "subclass":
+        layer.mlp.__class__ = Mlp
+    elif watch == "instance":
+        layer.mlp.forward = lambda x, residual=None: (seen.append(x), LlamaMlp.forward(layer.mlp, x, residual))[1]
+    elif watch == "attention subclass":
+        layer.self_attn.__class__ = Attn
+    else:
+        layer.self_attn.paged_decode = lambda x, *a, **kw: (seen.append(x), Attention.paged_decode(layer.self_attn, x, *a, **kw))[1]
+    with torch.no_grad():
+        engine = InferenceEngine.from_model_with_config(model, PassthroughTokenizer(100), InferenceEngineConfig(max_pages=32, max_seqs=4, page_size=8, max_pages_per_seq=8, compute_dtype=BF))
+        engine.generate([Request(prompt_tokens=[3, 4, 5], request_id=0, decode_params=SeqDecodingParams(6, None, 0.0, 0), n_generations=1)])
+    assert seen and all(type(x) is torch.Tensor and x.dtype == BF for x in seen)
