@@ -20,6 +20,7 @@ from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from ..utils.activation import ActivationFunctionEnum
 from . import lib
@@ -61,7 +62,7 @@ class Int8Rows(NamedTuple):
         _check_rows(v, s, "rows")
         if dtype not in _FLOATS:
             raise TypeError(f"rows come back as bf16 or fp32, not {dtype}")
-        if s.requires_grad and torch.is_grad_enabled():
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0:
             _no_gradient("dequantize", s)
         if not _kernels(v):
             return (v.float() * s.unsqueeze(-1)).to(dtype)
@@ -132,14 +133,17 @@ def _check_floats(what: str, like: torch.Tensor, other: Optional[torch.Tensor] =
         raise ValueError(f"{what}: rows of at least one element expected, got {tuple(shape)}")
     if other is not None and (other.dtype is not like.dtype or other.shape != shape or other.get_device() != like.get_device()):
         raise ValueError(f"{what}: {tuple(other.shape)} {other.dtype} on {other.device} does not go with {tuple(shape)} {like.dtype} on {like.device}")
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         _no_gradient(what, like, other)
 
 
 def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors whose derivative, backward or forward, would be lost."""
     for t in tensors:
-        if t is not None and t.requires_grad:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{what} has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
+        if t is not None and forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative: call it with the primal values")
 
 
 def _rows_of(t: torch.Tensor, align: int = 1) -> Tuple[torch.Tensor, int, int, int]:
@@ -222,7 +226,7 @@ def rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 
     if weight is not None:
         if weight.dim() != 1 or weight.shape[0] != cols or weight.dtype not in _FLOATS or weight.get_device() != x.get_device():
             raise ValueError(f"rms_norm_int8: weight [{cols}] in bf16 or fp32 on {x.device} expected, got {tuple(weight.shape)} {weight.dtype} on {weight.device}")
-        if weight.requires_grad and torch.is_grad_enabled():
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0:
             _no_gradient("rms_norm_int8", weight)
     if not _kernels(x):
         x = x.detach()
@@ -303,7 +307,7 @@ def _product(rows: Int8Rows, weight: Int8Rows, bias=None, residual=None, out_dty
         for t, want, what in ((bias, (N,), "bias"), (residual, shape, "residual")):
             if t is not None and (t.shape != want or t.dtype not in _FLOATS or t.get_device() != v.get_device()):
                 raise ValueError(f"int8_product: {what} {want} in bf16 or fp32 on {v.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         _no_gradient("int8_product", sv, sw, bias, residual)
     if not _kernels(v):
         sums, sv = torch.matmul(v.double(), w.double().t()).float(), sv.unsqueeze(-1)

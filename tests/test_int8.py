@@ -510,3 +510,30 @@ def test_layers_that_are_watched_get_tensors(watch):
         engine = InferenceEngine.from_model_with_config(model, PassthroughTokenizer(100), InferenceEngineConfig(max_pages=32, max_seqs=4, page_size=8, max_pages_per_seq=8, compute_dtype=BF))
         engine.generate([Request(prompt_tokens=[3, 4, 5], request_id=0, decode_params=SeqDecodingParams(6, None, 0.0, 0), n_generations=1)])
     assert seen and all(type(x) is torch.Tensor and x.dtype == BF for x in seen)
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_tangents_are_refused_or_kept_but_not_dropped(no_grad):
+    import contextlib
+
+    import torch.autograd.forward_ad as ad
+
+    torch.manual_seed(10)
+    x, t, w = torch.randn(4, 16), torch.randn(4, 16), I.quantize_rows(torch.randn(16, 16))
+    rows = I.quantize_rows(x)
+    with torch.no_grad() if no_grad else contextlib.nullcontext(), ad.dual_level():
+        d, s = ad.make_dual(x, t), ad.make_dual(rows.scale, rows.scale)
+        for call in (lambda: I.quantize_rows(d), lambda: I.rms_norm_int8(d, None), lambda: I.rms_norm_int8(x, None, residual=d), lambda: I.rms_norm_int8(x, d[0]),
+                     lambda: I.gated_activation_int8(d, x, Act.silu), lambda: I.gated_activation_int8(x, d, "tanh"), lambda: I.int8_product(rows, w, residual=d),
+                     lambda: I.int8_product(rows, w, bias=d[0]), lambda: I.int8_product(I.Int8Rows(rows.values, s), w), lambda: I.Int8Rows(rows.values, s).dequantize()):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        I.int8_product(I.quantize_rows(x), w, residual=x)  # others go on as ever
+        weight = torch.randn(5, 16)
+        y = ad.unpack_dual(I.int8_linear(d, weight))
+        torch.testing.assert_close(y.tangent, t @ I.quantize_rows(weight).dequantize(torch.float32).t(), atol=2e-5, rtol=1e-5)
+    assert torch.equal(I.quantize_rows(x).values, rows.values)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda a: I.quantize_rows(a).scale, (x,), (t,))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: I.quantize_rows(a).scale.sum())(x)

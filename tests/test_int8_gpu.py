@@ -789,3 +789,16 @@ def test_a_shared_expert_in_8_bits_leaves_the_others_on_their_kernels(gated, hid
             block.add_to_stream(replayed, h)
         g.replay()
         assert torch.equal(replayed, got)
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as ad
+
+    x, w = rand(4, 64), I.quantize_rows(rand(64, 64, seed=2))
+    rows = I.quantize_rows(x)
+    with torch.no_grad(), ad.dual_level():
+        d = ad.make_dual(x, rand(4, 64, seed=3))
+        for call in (lambda: I.quantize_rows(d), lambda: I.rms_norm_int8(x, None, residual=d), lambda: I.gated_activation_int8(x, d, Act.silu),
+                     lambda: I.int8_product(rows, w, residual=d), lambda: I.int8_linear(d, rand(8, 64))):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
