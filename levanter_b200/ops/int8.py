@@ -576,7 +576,14 @@ class Int8ServingLinear(nn.Module):
         super()._apply(fn, recurse)
         if self.weight_scale.dtype != torch.float32:  # a model's conversion to another type leaves the scales as they are
             self.weight_scale = scale.to(self.weight.device)
+        self._keep_rows_apart()
         return self
+
+    def _keep_rows_apart(self):
+        """A move or a load may have packed rows of a width that is no multiple of 16: every product would copy them back to where it reads them."""
+        w = self.weight
+        if w.stride(0) % 16 and w.shape[0] > 1:
+            self.weight = _room(w.shape, w.dtype, w.device).copy_(w)
 
     def _load_from_state_dict(self, state_dict, prefix, *args):
         w = state_dict.get(prefix + "weight")
@@ -584,6 +591,7 @@ class Int8ServingLinear(nn.Module):
             rows = _quantize(w.detach().to(self.weight.device, torch.bfloat16 if w.dtype is torch.bfloat16 else torch.float32))
             state_dict[prefix + "weight"], state_dict[prefix + "weight_scale"] = rows
         super()._load_from_state_dict(state_dict, prefix, *args)
+        self._keep_rows_apart()
 
     def forward(self, x: Union[torch.Tensor, Int8Rows], *, skip_bias: bool = False, residual: Optional[torch.Tensor] = None,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:

@@ -537,3 +537,27 @@ def test_tangents_are_refused_or_kept_but_not_dropped(no_grad):
         torch.func.jvp(lambda a: I.quantize_rows(a).scale, (x,), (t,))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda a: I.quantize_rows(a).scale.sum())(x)
+
+
+def test_weights_of_any_width_stay_where_products_read_them(tmp_path):
+    """Rows of a width that is no multiple of 16 lie apart; moves, copies and loads keep them so."""
+    torch.manual_seed(11)
+    m = I.Int8ServingLinear(torch.randn(8, 20), None)
+    values, x = m.weight.clone(), torch.randn(3, 20)
+    with torch.no_grad():
+        y = m(x)
+    state = m.state_dict()
+    torch.save(state, tmp_path / "state.pt")
+    packed = {k: v.contiguous() for k, v in torch.load(tmp_path / "state.pt").items()}
+    steps = [lambda: m._apply(lambda t: t.contiguous().clone()), lambda: m.load_state_dict(packed), lambda: m.load_state_dict(packed, assign=True), lambda: m.load_state_dict(state, assign=True), lambda: m.to(BF),
+             lambda: copy.deepcopy(m), lambda: m.to("meta") and m.to_empty(device="cpu").load_state_dict(packed)]
+    for step in steps:
+        got = step()
+        for mod in (m, got) if isinstance(got, I.Int8ServingLinear) else (m,):
+            assert mod.weight.stride() == (32, 1)
+            if mod.weight.device.type != "meta":
+                assert torch.equal(mod.weight, values)
+    with torch.no_grad():
+        assert torch.equal(m(x), y)
+    wide = I.Int8ServingLinear(torch.randn(8, 32), None)
+    assert wide.to(BF).weight is wide.weight and wide.weight.stride() == (32, 1)

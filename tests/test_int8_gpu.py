@@ -802,3 +802,14 @@ def test_tangents_are_refused():
                      lambda: I.int8_product(rows, w, residual=d), lambda: I.int8_linear(d, rand(8, 64))):
             with pytest.raises((RuntimeError, NotImplementedError)):
                 call()
+
+
+def test_weights_that_moved_are_read_where_they_lie():
+    m = I.Int8ServingLinear(torch.randn(40, 100), None).cuda()
+    assert m.weight.stride() == (112, 1) and m.weight_scale.is_cuda
+    x = rand(5, 100)
+    with torch.no_grad():
+        m(x)
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        m(x)
+        assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == 3  # values and scales of the rows, the result
