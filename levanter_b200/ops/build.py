@@ -15,6 +15,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 from typing import Optional
@@ -94,23 +95,28 @@ LAUNCHER = "_lvb_launcher.so"
 
 
 def build_launcher(force: bool = False) -> Optional[Path]:
-    """Compile ``csrc/host/launcher.c``, a Python module that calls the library's launchers (:func:`levanter_b200.ops.lib.quick`).  None where Python's own
-    headers are not installed; the launchers are then called through ``ctypes``."""
+    """Compile ``csrc/host/launcher.c``, a Python module that calls the library's launchers (:func:`levanter_b200.ops.lib.quick`), unless the one that is there
+    is of this source.  None where that cannot be done (no compiler, no headers of Python, another calling convention, a place that cannot be written); the
+    launchers are then called through ``ctypes``."""
     src, out = CSRC / "host" / "launcher.c", LIBDIR / LAUNCHER
-    include = sysconfig.get_paths()["include"]
-    gcc = shutil.which("gcc") or shutil.which("cc")
-    if not (Path(include) / "Python.h").exists() or gcc is None:
-        return out if out.exists() else None
     stamp, digest = LIBDIR / "launcher.stamp", hashlib.sha256(src.read_bytes()).hexdigest()
     if not force and out.exists() and stamp.exists() and stamp.read_text().strip() == digest:
         return out
-    LIBDIR.mkdir(parents=True, exist_ok=True)
-    part = out.with_suffix(f".{os.getpid()}.part")
-    r = subprocess.run([gcc, "-O2", "-shared", "-fPIC", "-I", include, str(src), "-o", str(part)], capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"{gcc} failed for {src.name}:\n{r.stderr}")
-    os.replace(part, out)
-    stamp.write_text(digest)
+    include = sysconfig.get_paths()["include"]
+    gcc = shutil.which("gcc") or shutil.which("cc")
+    if not (Path(include) / "Python.h").exists() or gcc is None:
+        return None
+    try:
+        LIBDIR.mkdir(parents=True, exist_ok=True)
+        part = out.with_suffix(f".{os.getpid()}.part")
+        r = subprocess.run([gcc, "-O2", "-shared", "-fPIC", "-I", include, str(src), "-o", str(part)], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise OSError(r.stderr)
+        os.replace(part, out)
+        stamp.write_text(digest)
+    except OSError as e:
+        warnings.warn(f"{src.name} was not built, kernels are launched through ctypes: {e}")
+        return None
     return out
 
 

@@ -141,8 +141,8 @@ def quick(name: str, kinds: str):
 
 @functools.lru_cache(maxsize=None)
 def _launcher():
-    path = _build.LIBDIR / _build.LAUNCHER
-    if not path.exists():
+    path = _build.build_launcher()
+    if path is None:
         return None
     try:
         loader = importlib.machinery.ExtensionFileLoader("_lvb_launcher", str(path))

@@ -561,3 +561,29 @@ def test_weights_of_any_width_stay_where_products_read_them(tmp_path):
         assert torch.equal(m(x), y)
     wide = I.Int8ServingLinear(torch.randn(8, 32), None)
     assert wide.to(BF).weight is wide.weight and wide.weight.stride() == (32, 1)
+
+
+def test_the_launcher_module_is_built_where_it_can_be(tmp_path, monkeypatch):
+    """Missing or of another source: built when it is first wanted.  What cannot be built keeps nothing else from being built."""
+    from levanter_b200.ops import build as B
+    from levanter_b200.ops import lib
+
+    src = B.CSRC / "host" / "launcher.c"
+    (tmp_path / "csrc" / "host").mkdir(parents=True)
+    mine = tmp_path / "csrc" / "host" / "launcher.c"
+    mine.write_bytes(src.read_bytes())
+    monkeypatch.setattr(B, "CSRC", tmp_path / "csrc")
+    monkeypatch.setattr(B, "LIBDIR", tmp_path / "lib")
+    module = lib._launcher.__wrapped__()
+    assert module is not None and (tmp_path / "lib" / B.LAUNCHER).exists()
+    first = (tmp_path / "lib" / B.LAUNCHER).stat().st_mtime_ns
+    assert B.build_launcher() is not None and (tmp_path / "lib" / B.LAUNCHER).stat().st_mtime_ns == first
+    mine.write_text(mine.read_text() + "\n// another\n")
+    assert B.build_launcher() is not None and (tmp_path / "lib" / B.LAUNCHER).stat().st_mtime_ns != first
+    mine.write_text("#error no such calling convention\n")
+    with pytest.warns(UserWarning, match="ctypes"):
+        assert B.build_launcher() is None
+    with pytest.warns(UserWarning):
+        assert lib._launcher.__wrapped__() is None  # not the module of the other source
+    monkeypatch.setattr(B.shutil, "which", lambda name: None)
+    assert B.build_launcher() is None
