@@ -716,9 +716,10 @@ class Attention(nn.Module):
         biased = [m.bias is not None for m in mods]
         if any(biased) != all(biased) or mods[0].in_features % 16 != 0:
             return None
-        w, s = self._rows.get([m.weight for m in mods], build), self._scale_rows.get([m.weight_scale for m in mods], build)
-        b = self._bias_rows.get([m.bias for m in mods], build) if biased[0] else None
-        return None if w is None or s is None or (biased[0] and b is None) else (Int8Rows(w, s), b)
+        w = self._rows.get([m.weight for m in mods], build)
+        s = self._scale_rows.get([m.weight_scale for m in mods], build) if w is not None else None
+        b = self._bias_rows.get([m.bias for m in mods], build) if s is not None and biased[0] else None
+        return None if s is None or (biased[0] and b is None) else (Int8Rows(w, s), b)
 
     def _paged_heads(self, x, kv_cache: "KvPageCache", batch_info, pos_ids, v_first: Optional[torch.Tensor] = None):
         """``(heads, v_first)``: the (gated) concatenated heads ``[T, heads * v_head_size]`` of packed tokens, for the forms of attention

@@ -174,8 +174,8 @@ class LlamaMlp(nn.Module):
         """Lays gate and up side by side for serving steps of a few rows, as the attention layer does with its projections."""
         mods = (self.gate_proj, self.up_proj)
         if all(type(m) is Int8ServingLinear and m.bias is None and m.in_features % 16 == 0 for m in mods):
-            self._rows.get([m.weight for m in mods])
-            self._scales.get([m.weight_scale for m in mods])
+            if self._rows.get([m.weight for m in mods]) is not None:
+                self._scales.get([m.weight_scale for m in mods])
         if all(type(m) is Linear and m.bias is None and m.weight.is_cuda and m.weight.dtype == torch.bfloat16 for m in mods):
             self._rows.get([m.weight for m in mods])
 
@@ -188,6 +188,7 @@ class LlamaMlp(nn.Module):
         if w is not None:
             return glu_of_rows(project(x, w), self.gate_proj.weight.shape[0], self.act)
         if all(plain(m, Int8ServingLinear) for m in mods) or all(plain(m, Int8Linear) for m in mods):
+            self._hold_apart()
             return gated_activation(*linear_many(x, *mods), self.act)  # the rows are quantised once
         return gated_activation(self.gate_proj(x), self.up_proj(x), self.act)
 
@@ -214,6 +215,12 @@ class LlamaMlp(nn.Module):
             return self.down_proj(h, residual=stream, out_dtype=torch.float32)
         return stream + self.down_proj(h).float()
 
+    def _hold_apart(self) -> None:
+        """Gate and up are read one by one from here on."""
+        mods = (self.gate_proj, self.up_proj)
+        self._rows.hold([m.weight for m in mods if type(m) in (Linear, Int8ServingLinear)])
+        self._scales.hold([m.weight_scale for m in mods if type(m) is Int8ServingLinear])
+
     def held_in_8_bits(self) -> bool:
         return all(plain(m, Int8ServingLinear) for m in (self.gate_proj, self.up_proj, self.down_proj))
 
@@ -238,7 +245,7 @@ class LlamaMlp(nn.Module):
         if x.dim() == 2 and x.shape[0] <= DECODE_ROWS and not torch.is_grad_enabled() and x.dtype == self.gate_proj.weight.dtype == torch.bfloat16:
             h = self._inner(x, build=False)
         else:
-            self._rows.hold([m.weight for m in (self.gate_proj, self.up_proj) if type(m) is Linear])
+            self._hold_apart()
             h = gated_activation(*linear_many(x, self.gate_proj, self.up_proj), self.act)
         if self.tp is not None and self.tp.size > 1:
             out = self.tp.row_linear(h, self.down_proj)

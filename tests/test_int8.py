@@ -587,3 +587,36 @@ def test_the_launcher_module_is_built_where_it_can_be(tmp_path, monkeypatch):
         assert lib._launcher.__wrapped__() is None  # not the module of the other source
     monkeypatch.setattr(B.shutil, "which", lambda name: None)
     assert B.build_launcher() is None
+
+
+def test_what_a_graph_reads_one_by_one_stays_where_it_is():
+    """Laying weights out moves nothing of a layer whose weights a recorded graph reads where they lie."""
+    from levanter_b200.layers.attention import Attention, AttentionConfig
+    from levanter_b200.models.llama import LlamaMlp
+
+    attn = quantize_for_serving(Attention(AttentionConfig(64, 4, 2, head_dim=64, use_bias=True)), QuantizationConfig(int8=True))
+    mods = attn._projections()
+    attn._rows._held.update(m.weight.data_ptr() for m in mods)  # as hold() notes them under capture
+    attn._scale_rows._held.update(m.weight_scale.data_ptr() for m in mods)
+    mlp = quantize_for_serving(LlamaMlp(64, 96, Act.silu), QuantizationConfig(int8=True))
+    mlp._rows._held.update((mlp.gate_proj.weight.data_ptr(),))
+    tensors = [t for m in mods + [mlp.gate_proj, mlp.up_proj] for t in (m.weight, m.weight_scale, m.bias) if t is not None]
+    before = [t.data_ptr() for t in tensors]
+    attn.lay_out_for_serving()
+    mlp.lay_out_for_serving()
+    assert [t.data_ptr() for t in tensors] == before
+
+
+@pytest.mark.parametrize("path", ["forward", "forward_fp32", "add_to_stream"])
+@pytest.mark.parametrize("targets", [None, ["gate_proj", "up_proj"]])
+def test_weights_read_one_by_one_are_noted(path, targets, monkeypatch):
+    from levanter_b200.models.llama import LlamaMlp
+    from levanter_b200.nn import FusedRows
+
+    noted = []
+    monkeypatch.setattr(FusedRows, "hold", lambda self, params: noted.extend(p.data_ptr() for p in params))
+    mlp = quantize_for_serving(LlamaMlp(64, 96, Act.silu), QuantizationConfig(int8=True, targets=targets)).eval()
+    x = torch.randn(300, 64)
+    with torch.no_grad():
+        mlp.add_to_stream(x, x) if path == "add_to_stream" else getattr(mlp, path)(x)
+    assert {t.data_ptr() for m in (mlp.gate_proj, mlp.up_proj) for t in (m.weight, m.weight_scale)} <= set(noted)
