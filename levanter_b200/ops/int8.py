@@ -410,6 +410,21 @@ def _held_products(x: torch.Tensor, values: torch.Tensor, scale: torch.Tensor, l
     return tuple(ys)
 
 
+class _WeightRef:
+    """What the backward pass wants to know of a weight, without keeping a converted copy of it."""
+
+    __slots__ = ("shape", "dtype", "parameter")
+
+    def __init__(self, w: torch.Tensor):
+        self.shape, self.dtype = w.shape, w.dtype
+        p = getattr(w, "converted_from", w)
+        named = getattr(p, "main_grad", None) is not None or getattr(p, "grad_sink", None) is not None
+        self.parameter = p if p.requires_grad and (p.is_leaf or named) else None
+
+    main_grad = property(lambda self: getattr(self.parameter, "main_grad", None))
+    grad_sink = property(lambda self: getattr(self.parameter, "grad_sink", None))
+
+
 def _gemm_rows(d: torch.Tensor) -> torch.Tensor:
     """``d [rows, cols]`` as bf16 rows that the GEMM reads where they lie."""
     cols = d.shape[1]
@@ -431,7 +446,7 @@ class _Int8ManyFn(torch.autograd.Function):
         weights, biases = tensors[:count], tensors[count:]
         values, scale, ld = _hold(x, weights)
         ctx.save_for_backward(values, scale)
-        ctx.refs, ctx.bias_dtypes = weights, [None if b is None else b.dtype for b in biases]
+        ctx.refs, ctx.bias_dtypes = [_WeightRef(w) for w in weights], [None if b is None else b.dtype for b in biases]
         ctx.x_shape, ctx.ld = x.shape, ld
         ctx.set_materialize_grads(False)  # a product that nothing uses has no gradient, and its weight none
         # (parts of one tensor, which autograd would take for views of each other and refuse to have written in place)
@@ -530,14 +545,11 @@ class Int8Linear(nn.Module):
         return Int8Linear(linear.weight, getattr(linear, "bias", None))
 
     def operand(self, dtype: torch.dtype) -> torch.Tensor:
-        """The weight in ``dtype``; a converted one passes its gradient on to the buffer that the weight names."""
-        w = self.weight
-        if w.dtype == dtype:
-            return w
-        w = w.to(dtype)
-        for name in ("main_grad", "grad_sink"):
-            if hasattr(self.weight, name):
-                setattr(w, name, getattr(self.weight, name))
+        """The weight in ``dtype``; the gradient of a converted one goes into the buffer that the weight names."""
+        if self.weight.dtype == dtype:
+            return self.weight
+        w = self.weight.to(dtype)
+        w.converted_from = self.weight
         return w
 
     def forward(self, x: torch.Tensor, *, skip_bias: bool = False) -> torch.Tensor:

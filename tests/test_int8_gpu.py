@@ -813,3 +813,22 @@ def test_weights_that_moved_are_read_where_they_lie():
         before = torch.cuda.memory_stats()["allocation.all.allocated"]
         m(x)
         assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == 3  # values and scales of the rows, the result
+
+
+def test_converted_weights_are_not_kept():
+    """Of fp32 weights the forward pass makes bf16 copies, of which the backward pass needs nothing."""
+    lin = I.Int8Linear(torch.nn.Parameter(rand(4096, 2048, dtype=F32, std=0.05)), None)
+    x, dy = rand(64, 2048).requires_grad_(), rand(64, 4096, seed=3)
+    lin(x)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = lin(x)
+    assert torch.cuda.memory_allocated() - before <= y.nbytes + 1.05 * (x.numel() + lin.weight.numel())
+    y.backward(dy)
+    want = torch.autograd.grad(I.int8_linear(x, lin.weight.detach().to(BF).requires_grad_()), [x], dy)[0]
+    assert lin.weight.grad.dtype == F32 and torch.equal(x.grad, want)
+    grad, lin.weight.grad = lin.weight.grad, None
+    y = lin(x)
+    lin.weight.main_grad = torch.zeros(4096, 2048, device="cuda")  # named after the forward pass
+    y.backward(dy)
+    assert lin.weight.grad is None and bool(((lin.weight.main_grad - grad).abs() <= 2.0 ** -8 * grad.abs() + 2.0 ** -22).all())
