@@ -832,3 +832,40 @@ def test_converted_weights_are_not_kept():
     lin.weight.main_grad = torch.zeros(4096, 2048, device="cuda")  # named after the forward pass
     y.backward(dy)
     assert lin.weight.grad is None and bool(((lin.weight.main_grad - grad).abs() <= 2.0 ** -8 * grad.abs() + 2.0 ** -22).all())
+
+
+# Blocks that go on to a second and a third row: the next row's reads under way, two sets of partial results.  Aligned rows of 8208 to 12288 columns run on two blocks per SM;
+# rows that start anywhere have forms for 512, 768 and 1024 threads and one that reads twice; up to 512 columns a warp has a row.
+MANY = [(1500, 8208), (1500, 11008), (1500, 12288), (3000, 4096), (1000, 14336), (3000, 528), (3000, 4095), (1500, 8191), (1500, 11007), (1000, 14335), (12000, 256), (9000, 511)]
+
+
+@pytest.mark.parametrize("rows,cols", MANY)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype,wtype", [(BF, BF), (BF, F32), (F32, F32)])
+def test_norms_of_many_rows(rows, cols, residual, dtype, wtype):
+    x, w = rand(rows, cols, seed=cols, dtype=dtype) * torch.logspace(-2, 2, rows, device="cuda")[:, None].to(dtype), (1 + rand(cols, seed=1, std=0.1, dtype=F32)).to(wtype)
+    r = rand(rows, cols, seed=2, dtype=dtype) if residual else None
+    got, h = I.rms_norm_int8(x, w, 1e-5, residual=r)
+    want = x if r is None else (x.float() + r.float()).to(dtype)
+    assert h is None or torch.equal(h, want)
+    d = want.double()
+    check_rows(got, d * w.double(), (d.square().mean(-1, keepdim=True) + 1e-5).rsqrt(), slack=0.0 if dtype == wtype == BF else 2.0 ** -22)
+
+
+@pytest.mark.parametrize("rows,cols", MANY)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("joint", [False, True])
+def test_gated_activations_of_many_rows(rows, cols, dtype, joint):
+    y = rand(rows, 2 * cols, seed=cols, std=3.0, dtype=dtype)
+    g, u = (y[:, :cols], y[:, cols:]) if joint else (y[:, :cols].contiguous(), y[:, cols:].contiguous())
+    u.mul_(torch.logspace(-2, 2, rows, device="cuda")[:, None])
+    check_rows(I.gated_activation_int8(g, u, Act.silu), torch.nn.functional.silu(g.double()) * u.double(), slack=2.0 ** -18)
+
+
+@pytest.mark.parametrize("rows,cols", MANY)
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantize_many_rows_and_back(rows, cols, dtype):
+    x = rand(rows, cols, seed=cols, dtype=dtype) * torch.logspace(-2, 2, rows, device="cuda")[:, None].to(dtype)
+    held_rows = I.quantize_rows(x)
+    check_rows(held_rows, x, slack=0.0 if dtype == BF else 2.0 ** -23)
+    assert torch.equal(held_rows.dequantize(dtype), (held_rows.values.float() * held_rows.scale[:, None]).to(dtype))
