@@ -787,7 +787,9 @@ int launch_pair(const void* A, const void* B, long long lda, long long ldb, Para
 // not keep the memory busy, and all that run should run at once; a split costs a start, the exchange of its sums (which grows with the rows) and the rows
 // of activations once more.  us for 1, 2, 4, 8 splits: 4096 x 4096, 1 row 10.8, 7.8, 5.3, 6.4, 64 rows 11.6, 10.4, 8.2, 20, 128 rows 12.3, 13.0, 10.9; 6144 x 4096, 16
 // rows 11.2, 8.7, 6.9, 7.9; 8192 x 2048, 16 rows 7.4, 5.7, 6.3, 10.3; 512 x 8192, 1 row 19.5, 11.4, 7.0, 5.0; 28672 x 4096, 1 row 20.7, 25, 25, 32; 4096 x 14336, 1 row 33,
-// 19, 12.7, 12.1.
+// 19, 12.7, 12.1.  Where four splits end, 1 / 2 / 3 / 4 splits: 40 tiles of K = 4096, 16 rows 11.0 / 8.7 / 7.1 / 7.4, 64 rows 12.1 / 11.4 / 9.8 / 10.3; 48 tiles 11.4 / 8.8 / 8.4 / 7.8 and
+// 12.5 / 11.7 / 11.2 / 10.7 (three are 144 CTAs, one per SM, but each reads a third of K); 56 11.8 / 9.4 / 9.2 / 8.6 and 12.8 / 12.2 / 11.7 / 11.1; 68 12.6 / 10.7 / 9.7 / 9.4 and 13.3 / 13.2 / 12.3 / 12.0;
+// 72, whose clusters of four do not all run at once, 12.8 / 11.0 / 10.1 / 13.4 and 13.4 / 13.5 / 12.6 / 18.4.  Of K = 2048, 16 rows, 48 tiles 7.0 / 5.5 / 6.0 / 5.5, 56 7.2 / 5.5 / 6.4 / 5.9.
 struct Plan {
   int form, rows, splits;  // rows: of activations per tile of the stream form
 };
@@ -796,7 +798,7 @@ inline Plan choose(int M, int N, int K) {
   if (M <= 16 && K <= 1024 && N <= 4096) return {1, 0, 0};
   if (M <= 64) {
     int splits = 1;
-    if (3 * columns <= sms) splits = 4;  // 48 tiles
+    if (k_blocks >= 32 ? 13 * columns <= 6 * sms : 3 * columns <= sms) splits = 4;  // 68 and 49 tiles
     else if (2 * columns <= sms && M <= 32) splits = 2;
     if (k_blocks >= 32 && (16 * columns <= sms || (k_blocks >= 96 && M <= 32 && 4 * columns <= sms))) splits = 8;
     while (splits > 1 && k_blocks < 4 * splits) splits /= 2;

@@ -361,8 +361,9 @@ MANY_ROWS = 2048
 def _side_by_side(rows: int, cols: int, outs: int) -> bool:
     """Whether the output gradients of several projections, ``outs`` columns in all, are copied side by side for one product each way.  That moves 4 bytes
     per row and output; a sum over the projections in fp32 moves 18 or more per row and column.  Forward and backward, us side by side / in fp32: 8192 rows of
-    4096 by 4096 + 1024 + 1024 868 / 1034, 16384 of 2048 by 2048 + 512 + 512 516 / 828, 4096 of 2048 by two of 8192 639 / 682; two of 11008 by
-    8192 rows of 4096 2904 / 2898, by 32768 12731 / 12044."""
+    4096 by 4096 + 1024 + 1024 868 / 1034, 16384 of 2048 by 2048 + 512 + 512 516 / 828, 4096 of 2048 by two of 8192 639 / 682.  From some 4 outputs per column on
+    there is little between them: 8192 rows of 4096 by two of 8192 2126 / 2193, of 10240 2782 / 2910, of 11008 3026 / 3055, of 14336 4061 / 4029; 32768 rows by two of 8192 9249 / 9041, of
+    11008 13409 / 12612; 32768 of 1024 by two of 4096 1515 / 1363."""
     return rows <= 4096 or outs <= 5 * cols
 
 

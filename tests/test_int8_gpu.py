@@ -869,3 +869,10 @@ def test_quantize_many_rows_and_back(rows, cols, dtype):
     held_rows = I.quantize_rows(x)
     check_rows(held_rows, x, slack=0.0 if dtype == BF else 2.0 ** -23)
     assert torch.equal(held_rows.dequantize(dtype), (held_rows.values.float() * held_rows.scale[:, None]).to(dtype))
+
+
+@pytest.mark.parametrize("M", [1, 16, 33, 64, 65])
+@pytest.mark.parametrize("N", [6144, 7168, 8699, 9216])
+@pytest.mark.parametrize("K", [2048, 4096])
+def test_products_on_both_sides_of_the_lines_of_the_rule(M, N, K):
+    check_product(int8(M, K, 1), int8(N, K, 2), rand(N), rand(M, N))
