@@ -142,8 +142,8 @@ def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{what} has no gradient of its own: train with int8_linear_many, or call it under torch.no_grad()")
-        if t is not None and forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
-            raise RuntimeError(f"{what} has no forward-mode derivative: call it with the primal values")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it with the primal values")
 
 
 def _rows_of(t: torch.Tensor, align: int = 1) -> Tuple[torch.Tensor, int, int, int]:
