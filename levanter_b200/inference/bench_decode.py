@@ -120,7 +120,7 @@ def main(argv=None):
     ap.add_argument("--tp", type=int, default=1, help="tensor-parallel ranks (launch with torchrun, one rank per GPU)")
     ap.add_argument("--prompt-min", type=int, default=0, help="with --prompt-max: prompt lengths uniform in [min, max]")
     ap.add_argument("--prompt-max", type=int, default=0)
-    ap.add_argument("--int8", action="store_true", help="hold the weights of attention and MLP layers in 8 bits")
+    ap.add_argument("--int8", action="store_true", help="hold the weights of attention layers and gated MLPs in 8 bits")
     ap.add_argument("--quiet", action="store_true", help="return the result without printing it")
     a = ap.parse_args(argv)
     return run(a)

@@ -71,7 +71,7 @@ class InferenceEngineConfig:
     seed: int = 0
     enable_logprobs: bool = False
     use_cuda_graph: bool = False  # capture the decode call (fixed shapes) and replay it
-    quantization: Optional[QuantizationConfig] = None  # {int8: true}: attention and MLP weights in 8 bits, their inputs quantised token by token
+    quantization: Optional[QuantizationConfig] = None  # {int8: true}: weights of attention and gated MLPs in 8 bits, their inputs quantised token by token
 
     @property
     def imputed_max_pages(self) -> int:

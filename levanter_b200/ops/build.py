@@ -32,7 +32,7 @@ SERVING_SOURCES = ("attention_any", "depth_stream", "elementwise", "flash_attn_f
                    "residual_stream", "sampler")
 
 # Kernels whose results are 32-bit throughout (norms of an fp32 stream, router scores, rotary angles, recurrences, fp32 attention, the
-# loss): no fast-math exponentials, divisions or square roots.
+# loss): no fast-math exponentials, divisions or square roots but those that a source names itself, with the reason.
 ACCURATE_SOURCES = ("attention_any", "cross_entropy", "delta_chunks", "depth_stream", "gated_scan", "gemm_int8", "int8_rows", "linear_attention", "linear_attention_umma", "moe_experts", "qkv_prep",
                     "residual_stream")
 

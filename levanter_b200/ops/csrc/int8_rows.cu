@@ -13,10 +13,11 @@
 // between the reduction and the write, and the reads of a block's next row are under way meanwhile:
 //   - rows of whole groups of 16 bf16 elements that start on 32 bytes, above 512 and up to 16384 columns: a block per row, one load of 32 bytes per thread
 //     and input (rows16_kernel).  16384 x 4096: norm with residual 73 us (470 MB, 6.4 TB/s), without 48 (4.2), a row as it is 38 (5.3); gated activation of
-//     8192 x 11008 84 (5.4).  A norm without residual waits for its reduction: of 4096 columns it holds half of what an SM could read in that time.
+//     8192 x 11008 84 (5.4), of which 70 would be the bytes.  A norm without residual waits for its reduction: of 4096 columns it holds half of what an SM could read in that time.
 //   - the others (quantize_kernel): up to 512 columns a warp per row; up to 16384 a block per row, eight elements per thread and turn; beyond that (norms with
 //     residual: beyond 12288, in fp32 8192) the row is read twice.  Rows of 4095 or 11007 columns, which start anywhere: 16384 x 4095 norm with residual 200 us, a row
-//     as it is 65; gated activation of 8192 x 11007 187.
+//     as it is 65; gated activation of 8192 x 11007 187 (floors 73, 31 and 70): one aligned load more per eight elements and a shift per word, and the registers that
+//     they take leave one block per SM.  fp32 norms with residual of more than 8192 columns read twice what they could read once: 8192 x 11008 268 us, floor 181.
 //   - back: 31 us for 16384 x 4096 (201 MB, 6.4 TB/s), 42 for 8192 x 11008; rows of odd widths 45 and 58.
 // Few rows are bound by a launch: one row of 4096 takes 2.0 us in a graph.
 #include <initializer_list>
@@ -34,7 +35,10 @@ constexpr float kMostScale = 0x1.020406p+121f;   // times 127 it is still a fini
 
 enum Act : int { kSilu = 0, kGeluTanh = 1, kGelu = 2, kRelu = 3, kQuickGelu = 4 };
 
-// x sigmoid(a x) of two numbers, 2^-20 relative: far below half a step of the 8 bits.  An exponential that runs over makes the quotient 0, as it should be.
+// x sigmoid(a x) of two numbers with the quick exponential and reciprocal, for fp32 gates as well: right to 2^-20 where |a x| is up to 8 and to 2^-23 |a x| beyond (the
+// exponent's argument is rounded).  Half a step of the 8 bits is 2^-8 of the row's largest element, so an element goes to the other whole number only where it lies
+// that close to the border.  With expf and a division, fp32 rows of 8192 x 11008 take 334 us instead of 233 and 65536 x 256 105 instead of 54.  An exponential
+// that runs over makes the quotient 0, as it should be.
 __device__ __forceinline__ F32x2 swish2(F32x2 x, float a) {
   const float k = -1.4426950408889634f * a;  // log2 e
   float e0, e1;
@@ -551,7 +555,7 @@ __device__ __forceinline__ void rows_in_64_bits(Normed<T> src, long long row, lo
       }
     }
     const double top = most / sqrt(sum / cols + static_cast<double>(src.eps));  // of the normed row
-    const bool finite = most <= 1.7e308 && sum <= 1.7e308, live = finite && top >= kTiny;
+    const bool finite = most <= 1.7e308 && sum <= 1.7e308 && top == top, live = finite && top >= kTiny;
 #pragma unroll 1
     for (int c = t; c < cols; c += group)
       q[row * ldq + c] = live ? static_cast<int8_t>(__double2int_rn(127.0 * (static_cast<double>(src.element(row, c)) * src.weight(c)) / most)) : 0;

@@ -7,7 +7,7 @@ token, a row of a weight matrix ``[out, in]`` one per output channel (:class:`In
 quantised rows and weights on the tensor cores, in whole numbers, and applies both scales, bias and residual to the sums (``csrc/gemm_int8.cu``).
 
 :func:`int8_linear_many` is the differentiable form, which :class:`Int8Linear` trains with: activations and weights are quantised, several projections of the
-same rows share them, and the 8-bit rows are all that is kept of the activations for the backward pass.  Its gradients are those of the product at
+same rows share them, and the 8-bit rows of both are what is kept for the backward pass.  Its gradients are those of the product at
 the values that the whole numbers stand for (the rounding counts as having slope one).  :class:`Int8ServingLinear` holds a layer's weights in
 8 bits for serving.
 
@@ -435,7 +435,8 @@ def _gemm_rows(d: torch.Tensor) -> torch.Tensor:
 
 
 class _Int8ManyFn(torch.autograd.Function):
-    """Projections of the same rows.  Kept for the backward pass: the rows and the weights in 8 bits, 1 byte per activation instead of 2, once for all projections.
+    """Projections of the same rows.  Kept for the backward pass: the rows and the weights in 8 bits, once for all projections.  bf16 layers keep 2 bytes per activation and
+    the parameters, which are there anyhow; this is 1 per activation and 1 per weight, so less of it where there are more rows than outputs.
 
     ``dx = sum dy w'`` and ``dw = dy^T x'`` are bf16 products of what the whole numbers stand for, rounded to bf16 (2^-8 of each value at most, as any operand
     of a bf16 layer); output gradients are not quantised, their rows span too many magnitudes for one scale.  The sum over several projections is rounded

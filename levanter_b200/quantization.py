@@ -7,10 +7,10 @@ maxima (delayed scaling, as in the reference); ``scaling: block`` uses one power
 contraction dimension, applied by the tensor core (``tcgen05.mma kind::mxf8f6f4.block_scale``).  ``block_size`` is accepted
 for configs that name it; the hardware's block is 32 whatever it says.
 ``int8: true`` selects 8-bit integer products for the forward pass (``ops/int8.py``): one scale per token and per output channel, taken from the values
-themselves, gradients from bf16 products, activations kept for the backward pass in 8 bits.
+themselves, gradients from bf16 products, activations and weights kept for the backward pass in 8 bits.
 ``quantize_linear_layers`` swaps matching ``Linear`` modules for ``Fp8Linear`` or ``Int8Linear``;
 master weights, optimizer state and checkpoints are unchanged.
-``quantize_for_serving`` replaces the projections of attention and MLP layers by ones that hold their weights in 8 bits (``int8: true``)."""
+``quantize_for_serving`` replaces the projections of attention layers and gated MLPs by ones that hold their weights in 8 bits (``int8: true``)."""
 from __future__ import annotations
 
 import re
@@ -66,7 +66,8 @@ def quantize_linear_layers(model: nn.Module, config: QuantizationConfig) -> nn.M
 
 
 def quantize_for_serving(model: nn.Module, config: QuantizationConfig) -> nn.Module:
-    """Hold the weights of the targeted projections of attention and MLP layers in 8 bits, one scale per output channel (in place; returns the model).  The
+    """Hold the weights of the targeted projections of ``Attention`` layers and ``LlamaMlp`` blocks (shared experts among them) in 8 bits, one scale per output channel
+    (in place; returns the model).  Other layers stay as they are: routed experts, MLPs without a gate, other mixers, embeddings and head.  The
     model serves from then on: those weights are not parameters any more, and engines made of it before (their CUDA graphs read the old weights) are done.  A model that is quantised already comes back as it is."""
     if config.fp8:
         raise ValueError("serving holds weights in 8-bit integers: use QuantizationConfig(int8=True)")
