@@ -106,6 +106,8 @@ def gemm(
     else:
         if out.shape != (M, N) or out.stride(1) != 1:
             raise ValueError("out has the wrong shape or is not row-major")
+        if out.data_ptr() % 16 and out.stride(0) * out.element_size() % 16 == 0:
+            raise ValueError("out has to start on 16 bytes")  # such rows are written 16 bytes at a time
     flags = 0
     if out.dtype == torch.float32:
         flags |= F_OUT_F32

@@ -876,3 +876,22 @@ def test_quantize_many_rows_and_back(rows, cols, dtype):
 @pytest.mark.parametrize("K", [2048, 4096])
 def test_products_on_both_sides_of_the_lines_of_the_rule(M, N, K):
     check_product(int8(M, K, 1), int8(N, K, 2), rand(N), rand(M, N))
+
+
+@pytest.mark.parametrize("outs,cols", [(40, 100), (40, 96), (13, 77)])
+def test_gradient_buffers_of_any_size_and_those_that_start_anywhere(outs, cols):
+    """A buffer whose rows would be written 16 bytes at a time has to start on 16 bytes; others may start anywhere."""
+    x, w, dy = rand(70, cols).requires_grad_(), rand(outs, cols, seed=2).requires_grad_(), rand(70, outs, seed=3)
+    want = torch.autograd.grad(I.int8_linear(x, w), [w], dy)[0]
+    flat = torch.zeros(outs * cols + 16, device="cuda")
+    for first in (4, 1):
+        flat.zero_()
+        w.main_grad = flat[first:first + outs * cols].view(outs, cols)
+        if first == 1 and cols % 4 == 0:
+            with pytest.raises(ValueError, match="16 bytes"):
+                I.int8_linear(x, w).backward(dy)
+            continue
+        I.int8_linear(x, w).backward(dy)
+        lib.check_status()
+        assert w.grad is None and bool(((w.main_grad - want.float()).abs() <= 2.0 ** -8 * want.float().abs() + 2.0 ** -22).all())
+        assert not flat[:first].any() and not flat[first + outs * cols:].any()
