@@ -194,9 +194,10 @@ class InferenceEngine:
 
     @classmethod
     def from_model_with_config(cls, model, tokenizer, config: InferenceEngineConfig) -> "InferenceEngine":
-        if config.quantization is not None:
-            model = quantize_for_serving(model, config.quantization)
         table = PageTable.init(config.imputed_max_pages, config.max_seqs, config.page_size, config.max_pages_per_seq)
+        if config.quantization is not None:
+            model.initial_cache  # noqa: B018 - a model that the engine cannot serve is left as it is
+            model = quantize_for_serving(model, config.quantization)
         try:
             device = next(model.parameters()).device
         except (AttributeError, StopIteration, TypeError):

@@ -569,13 +569,17 @@ class Int8ServingLinear(nn.Module):
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor]):
         super().__init__()
-        if weight.dim() != 2 or weight.dtype not in _FLOATS or not 0 < weight.shape[1] <= MAX_COLS:
-            raise ValueError(f"a weight [out, in] in bf16 or fp32 with up to {MAX_COLS} columns expected, got {tuple(weight.shape)} {weight.dtype}")
+        self.check_weight(weight)
         self.out_features, self.in_features = weight.shape
         rows = _quantize(weight.detach())
         self.register_buffer("weight", rows.values)
         self.register_buffer("weight_scale", rows.scale)
         self.register_buffer("bias", None if bias is None else bias.detach())
+
+    @staticmethod
+    def check_weight(weight: torch.Tensor) -> None:
+        if weight.dim() != 2 or weight.dtype not in _FLOATS or not 0 < weight.shape[1] <= MAX_COLS:
+            raise ValueError(f"a weight [out, in] in bf16 or fp32 with up to {MAX_COLS} columns expected, got {tuple(weight.shape)} {weight.dtype}")
 
     @staticmethod
     def from_linear(linear: nn.Module) -> "Int8ServingLinear":

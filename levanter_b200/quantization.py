@@ -78,18 +78,21 @@ def quantize_for_serving(model: nn.Module, config: QuantizationConfig) -> nn.Mod
     from .nn import Linear
     from .ops.int8 import Int8Linear, Int8ServingLinear
 
-    held = 0
-    for name, mod in list(model.named_modules()):
+    held, found = 0, []
+    for name, mod in model.named_modules():
         if not isinstance(mod, (Attention, LlamaMlp)):
             continue
         if mod.tp is not None and mod.tp.size > 1:
             raise ValueError(f"{name}: int8 serving weights are not split over tensor-parallel ranks")
-        for child_name, child in list(mod.named_children()):
+        for child_name, child in mod.named_children():
+            held += type(child) is Int8ServingLinear
             if type(child) in (Linear, Int8Linear) and config.matches(f"{name}.{child_name}"):
-                setattr(mod, child_name, Int8ServingLinear.from_linear(child))
-            held += type(getattr(mod, child_name)) is Int8ServingLinear
-    if held == 0:
+                Int8ServingLinear.check_weight(child.weight)
+                found.append((mod, child_name))
+    if held == 0 and not found:
         raise ValueError("no projection of an attention or MLP layer matches the quantization targets")
+    for mod, child_name in found:  # (nothing has been replaced where one of them is refused)
+        setattr(mod, child_name, Int8ServingLinear.from_linear(getattr(mod, child_name)))
     return model
 
 

@@ -620,3 +620,24 @@ def test_weights_read_one_by_one_are_noted(path, targets, monkeypatch):
     with torch.no_grad():
         mlp.add_to_stream(x, x) if path == "add_to_stream" else getattr(mlp, path)(x)
     assert {t.data_ptr() for m in (mlp.gate_proj, mlp.up_proj) for t in (m.weight, m.weight_scale)} <= set(noted)
+
+
+def test_what_is_refused_is_left_as_it_was():
+    """Quantising for serving changes a model in place: not before all of it can be done."""
+    from levanter_b200.data.passthrough_tokenizer import PassthroughTokenizer
+    from levanter_b200.inference.engine import InferenceEngine, InferenceEngineConfig
+    from levanter_b200.models.gemma import GemmaConfig
+
+    def untouched(model):
+        return not any(isinstance(m, I.Int8ServingLinear) for m in model.modules())
+
+    model = llama().build(100, seed=0)
+    model.transformer.layers[1].mlp.half()
+    with pytest.raises(ValueError, match="float16"):
+        quantize_for_serving(model, QuantizationConfig(int8=True))
+    assert untouched(model)
+    model = GemmaConfig(seq_len=64, hidden_dim=64, intermediate_dim=128, num_layers=1, num_heads=4, num_kv_heads=2, gradient_checkpointing=False).build(100, seed=0)
+    cfg = InferenceEngineConfig(max_pages=32, max_seqs=4, page_size=8, max_pages_per_seq=8, compute_dtype=torch.float32, quantization=QuantizationConfig(int8=True))
+    with pytest.raises(AttributeError):  # the engine has no cache for it
+        InferenceEngine.from_model_with_config(model, PassthroughTokenizer(100), cfg)
+    assert untouched(model)
