@@ -509,13 +509,13 @@ __device__ __forceinline__ float warp_ss(F32x2 ss2) {
 // Rows whose sum of squares left the range of fp32: elements from some 1e19 on and, with an eps below 2^-90, those that are smaller than that.  (`top`: of a row
 // without NaN and not of zeros; it may have run over itself.)  One thread of a row notes them by a scale that no row has, and when a block is through with its
 // rows it makes them again, so that the loop over the rows holds no code of this.
-constexpr float kAgain = -1.f;
+constexpr float kNoted = -1.f;
 template <class Src>
 __device__ __forceinline__ float noted(const Src& src, const RowScale& r, uint32_t top, float ss, int* again) {
   if constexpr (Src::kSum) {
     if (!(src.mean(ss) >= 0x1p-90f && src.mean(ss) <= 3.402823466e+38f) && top != 0 && top <= 0x7F800000u) {
       *again = 1;
-      return kAgain;
+      return kNoted;
     }
   }
   return r.step();
@@ -527,7 +527,7 @@ __device__ __forceinline__ void rows_in_64_bits(Normed<T> src, long long row, lo
   const int lane = threadIdx.x & 31, t = kWarp ? lane : static_cast<int>(threadIdx.x), group = kWarp ? 32 : static_cast<int>(blockDim.x);
 #pragma unroll 1
   for (; row < rows; row += step) {
-    if (scale[row] != kAgain) continue;
+    if (scale[row] != kNoted) continue;
     double most = 0.0, sum = 0.0;
 #pragma unroll 1
     for (int c = t; c < cols; c += group) {
